@@ -62,7 +62,9 @@ typedef enum sbx_status {
     SBX_HIP_ERROR = 3         /* a HIP runtime call or kernel launch failed                */
 } sbx_status;
 
-typedef enum sbx_dtype { SBX_F32 = 0, SBX_F64 = 1 } sbx_dtype;
+/* SBX_BF16 and SBX_F16: the dropout and MXFP4 entry points only (the others
+ * return SBX_UNSUPPORTED). */
+typedef enum sbx_dtype { SBX_F32 = 0, SBX_F64 = 1, SBX_BF16 = 2, SBX_F16 = 3 } sbx_dtype;
 
 /* Replaces oneapi::mkl::blas::row_major::gemm<float> (gemm.cpp:63) and
  * column_major::gemm<float> (gemm.cpp:76), reached from the FLOAT32 case of
@@ -212,6 +214,73 @@ int sbx_dsyrk_strided_batched(void* stream, int layout, int upper, int trans, in
                               int64_t k, double alpha, const double* A, int64_t lda,
                               int64_t str_a, double beta, double* C, int64_t ldc, int64_t str_c,
                               int64_t batch);
+
+/* ---- Dropout and MXFP4: a dense layer's training and serving in 4 bits ----
+ *
+ * None of these has a counterpart in the reference.  They make a feed-forward
+ * block whose products run on the 4-bit matrix cores: quantise activations,
+ * weights and gradients along the axis that a product sums over, multiply, and
+ * drop activations out on their way.  All matrices are row-major; nothing is
+ * allocated, except the product's split-K partials, in the stream's workspace. */
+
+/* Dropout, Y = keep ? X / (1 - p) : 0 (rows x cols, F32, F64, BF16 or F16).
+ * keep is a function of (seed, stream_id, row, column) alone, by the
+ * counter-based Philox4x32-10: 16 bits h per element -- word c % 8 / 2, half
+ * c % 2, of the counter (c / 8, row, stream_id, 0x44524F50) under the key seed --
+ * and an element stays if h >= t, t = floor(65536 p + 0.5).  The factor is
+ * 65536 / (65536 - t) exactly, so the mean is kept whatever p rounds to; p = 1
+ * drops everything.  The mask is never stored: the backward pass is the same
+ * call on dY with the same p, seed and stream_id.
+ * gate (may be NULL): values that pass only where gate > 0, else 0.  Backward:
+ * the output of the ReLU that the dropout followed, so the call is the gradient
+ * through both; forward: gate == X is the ReLU itself.
+ * Dropped and gated values are 0 whatever X holds there, NaN included.  Y may
+ * be X or the gate itself (same leading dimension).  0 <= p <= 1. */
+int sbx_dropout(void* stream, int dtype, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                const void* gate, int64_t ldg, void* Y, int64_t ldy, double p, uint64_t seed,
+                uint32_t stream_id);
+
+/* Quantisation to MXFP4, the OCP microscaling format with 4-bit e2m1 elements
+ * (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), of V: the rows x cols matrix X
+ * (F32, BF16 or F16) after sbx_dropout's p, seed, stream_id and gate (p = 0 and
+ * gate = NULL: X itself; V is held in 32 bits, not rounded to dtype).
+ *   P, S (NULL: not wanted): V in blocks of 32 along its rows.  Element
+ * (r, c) is half c % 2 (0: low) of byte P[r*ldp + c/2]; a row's last block is
+ * filled with zeros.  Block b of row r has its scale 2^(code - 127) at
+ * S[(b/8)*lds + 8*r + b%8]: 8 blocks of a row lie together (codes past a row's
+ * last block are 0), groups of 8 blocks lds bytes apart.
+ *   PT, ST: the same of V^T (cols x rows), blocks of 32 along V's columns.
+ * code = max(floor(log2 max|v|) - 2, -127) + 127 over the block; elements are
+ * v / 2^(code - 127) rounded to nearest even, saturated at 6.  A block with an
+ * infinity or NaN has code 255: all of it is NaN.
+ * P, PT 16-byte aligned, ldp >= 16*ceil(cols/32) and a multiple of 16; S, ST
+ * 8-byte aligned, lds >= 8*rows and a multiple of 8 (ldpt, ldst: of rows and
+ * cols). */
+int sbx_mx4_quantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* X,
+                     int64_t ldx, const void* gate, int64_t ldg, double p, uint64_t seed,
+                     uint32_t stream_id, void* P, int64_t ldp, void* S, int64_t lds, void* PT,
+                     int64_t ldpt, void* ST, int64_t ldst);
+
+/* The values an MXFP4 matrix (P, S as above) stands for, rounded to dtype
+ * (F32: exact). */
+int sbx_mx4_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* P,
+                       int64_t ldp, const void* S, int64_t lds, void* Y, int64_t ldy);
+
+/* C = epilogue(alpha * A * B^T + beta * C): A (m x k) and B (n x k) MXFP4
+ * matrices (A, SA with lda, ldsa; B, SB with ldb, ldsb, as written by
+ * sbx_mx4_quantize), C (m x n) of dtype F32, BF16 or F16 in `layout`.  Products
+ * are exact, sums are held in 32 bits and rounded to dtype once.  What lies
+ * past the k-th term's block is not used, nor are the codes there.  BLAS
+ * semantics as for GEMM (beta == 0: C is not read; alpha == 0 or k == 0: A and
+ * B are not).  A layer's three products are this one on the right quantisations:
+ *   forward Y = X W^T    : X along rows, W (n x k) along rows
+ *   dX = dY W            : dY along rows, W's PT
+ *   dW = dY^T X          : dY's PT, X's PT
+ * k <= 2^23 and lda, ldb < 2^23 - 15 (else SBX_UNSUPPORTED). */
+int sbx_mx4_gemm(void* stream, int dtype, int layout, int64_t m, int64_t n, int64_t k, float alpha,
+                 const void* A, int64_t lda, const void* SA, int64_t ldsa, const void* B,
+                 int64_t ldb, const void* SB, int64_t ldsb, float beta, void* C, int64_t ldc,
+                 int epilogue);
 
 /* Name of the plan (kernel tile and k-split) the dispatcher would launch for
  * this problem (tiling heuristics introspection for benchmarks).  A name is a

@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libsbx.so")
 # stamps for measurements; use_probe_library() selects it before first use.
 PROBE_LIB_PATH = os.path.join(_HERE, "lib", "libsbx_probe.so")
 
-F32, F64 = 0, 1
+F32, F64, BF16, F16 = 0, 1, 2, 3  # BF16, F16: dropout and MXFP4 calls only
 ALGO_AUTO, ALGO_GENERIC, ALGO_MFMA, ALGO_MFMA_TILE, ALGO_MFMA_SMALL = 0, 1, 2, 3, 4
 EPILOGUE_NONE, EPILOGUE_RELU = 0, 1
 STATUS = {0: "SBX_OK", 1: "SBX_INVALID_ARGUMENT", 2: "SBX_UNSUPPORTED", 3: "SBX_HIP_ERROR"}
@@ -132,6 +132,18 @@ def lib() -> ctypes.CDLL:
     L.sbx_fill_normal.restype = i32
     L.sbx_fill_normal.argtypes = [vp, i32, vp, i64, ctypes.c_uint64, ctypes.c_uint32,
                                   ctypes.c_double]
+    L.sbx_dropout.restype = i32
+    L.sbx_dropout.argtypes = [vp, i32, i64, i64, vp, i64, vp, i64, vp, i64, ctypes.c_double,
+                              ctypes.c_uint64, ctypes.c_uint32]
+    L.sbx_mx4_quantize.restype = i32
+    L.sbx_mx4_quantize.argtypes = [vp, i32, i64, i64, vp, i64, vp, i64, ctypes.c_double,
+                                   ctypes.c_uint64, ctypes.c_uint32, vp, i64, vp, i64, vp, i64,
+                                   vp, i64]
+    L.sbx_mx4_dequantize.restype = i32
+    L.sbx_mx4_dequantize.argtypes = [vp, i32, i64, i64, vp, i64, vp, i64, vp, i64]
+    L.sbx_mx4_gemm.restype = i32
+    L.sbx_mx4_gemm.argtypes = [vp, i32, i32, i64, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp,
+                               i64, vp, i64, ctypes.c_float, vp, i64, i32]
     L.sbx_version.restype = ctypes.c_char_p
     L.sbx_version.argtypes = []
     if LIB_PATH == PROBE_LIB_PATH:
@@ -283,6 +295,48 @@ def syrk(dtype, layout, upper, trans, n, k, alpha, A, lda, str_a, beta, C, ldc, 
     f = lib().sbx_ssyrk_strided_batched if dtype == F32 else lib().sbx_dsyrk_strided_batched
     _check(f(_stream(stream), int(layout), int(upper), int(trans), n, k, alpha, _ptr(A), lda,
              str_a, beta, _ptr(C), ldc, str_c, batch), "sbx_syrk")
+
+
+def dropout(dtype, rows, cols, X, ldx, Y, ldy, p, seed, stream_id, gate=None, ldg=0,
+            stream=None) -> None:
+    """sbx_dropout: Y = keep ? X / (1 - p) : 0, where gate > 0 if there is one.
+    The mask comes from (seed, stream_id) and the element's place, so the
+    backward pass is the same call on the gradient."""
+    _check(lib().sbx_dropout(_stream(stream), dtype, rows, cols, _ptr(X), ldx, _ptr(gate), ldg,
+                             _ptr(Y), ldy, p, seed, stream_id), "sbx_dropout")
+
+
+def mx4_shapes(rows, cols):
+    """Shapes (uint8) of a rows x cols MXFP4 matrix without padding: packed
+    elements (leading dimension: the second) and scale codes (leading
+    dimension: 8 * rows)."""
+    nb = -(-cols // 32)
+    return (rows, 16 * nb), (-(-nb // 8), rows, 8)
+
+
+def mx4_quantize(dtype, rows, cols, X, ldx, P=None, ldp=0, S=None, lds=0, PT=None, ldpt=0,
+                 ST=None, ldst=0, p=0.0, seed=0, stream_id=0, gate=None, ldg=0,
+                 stream=None) -> None:
+    """sbx_mx4_quantize: X, after dropout and gate, to MXFP4 along its rows
+    (P, S), its columns (PT, ST) or both in one pass."""
+    _check(lib().sbx_mx4_quantize(_stream(stream), dtype, rows, cols, _ptr(X), ldx, _ptr(gate),
+                                  ldg, p, seed, stream_id, _ptr(P), ldp, _ptr(S), lds, _ptr(PT),
+                                  ldpt, _ptr(ST), ldst), "sbx_mx4_quantize")
+
+
+def mx4_dequantize(dtype, rows, cols, P, ldp, S, lds, Y, ldy, stream=None) -> None:
+    """sbx_mx4_dequantize: the values an MXFP4 matrix stands for."""
+    _check(lib().sbx_mx4_dequantize(_stream(stream), dtype, rows, cols, _ptr(P), ldp, _ptr(S),
+                                    lds, _ptr(Y), ldy), "sbx_mx4_dequantize")
+
+
+def mx4_gemm(dtype, layout, m, n, k, alpha, A, lda, SA, ldsa, B, ldb, SB, ldsb, beta, C, ldc,
+             epilogue=EPILOGUE_NONE, stream=None) -> None:
+    """sbx_mx4_gemm: C = epilogue(alpha * A * B^T + beta * C) of two MXFP4
+    matrices quantised along k."""
+    _check(lib().sbx_mx4_gemm(_stream(stream), dtype, int(layout), m, n, k, alpha, _ptr(A), lda,
+                              _ptr(SA), ldsa, _ptr(B), ldb, _ptr(SB), ldsb, beta, _ptr(C), ldc,
+                              int(epilogue)), "sbx_mx4_gemm")
 
 
 def gemm_select(dtype, layout, transA, transB, m, n, k, lda, ldb, ldc, batch=1) -> str:

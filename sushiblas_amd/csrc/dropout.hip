@@ -1,0 +1,90 @@
+// dropout.hip -- dropout whose mask is a function of the element's place, so
+// that none is stored (see DropoutArgs): Y = keep ? X * scale : 0, and with a
+// gate only where gate > 0.  Forward and backward pass are the same kernel.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mx4.hpp"
+
+namespace sbx {
+namespace {
+
+template <typename T>
+struct Arith {
+    typedef float type;
+};
+template <>
+struct Arith<double> {
+    typedef double type;
+};
+
+// Eight values, from memory that is aligned to the element only (the device
+// serves such 16-byte accesses).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+    T v[8];
+};
+
+// Threads form TX chunks of 8 columns by 256 / TX rows.
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64_t ldy, int tx)
+{
+    typedef typename Arith<T>::type R;
+    const uint32_t chunk = blockIdx.x * tx + threadIdx.x % tx;
+    const int64_t c0 = (int64_t)chunk * 8;
+    if (c0 >= a.cols) return;
+    const R scale = (R)a.scale;
+    const int rows_per = 256 / tx;
+    for (int64_t row = (int64_t)blockIdx.y * rows_per + threadIdx.x / tx; row < a.rows;
+         row += (int64_t)gridDim.y * rows_per) {
+        const T* x = (const T*)a.X + row * a.ldx + c0;
+        const T* g = a.gate ? (const T*)a.gate + row * a.ldg + c0 : nullptr;
+        T* y = Y + row * ldy + c0;
+        const uint32_t keep = a.threshold ? keep_bits(a, (uint32_t)row, chunk) : 0xffu;
+        if (c0 + 8 <= a.cols) {
+            const Eight<T> xv = *(const Eight<T>*)x;
+            Eight<T> yv;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                yv.v[i] = keep >> i & 1 ? (T)((R)xv.v[i] * scale) : (T)0;
+            if (g) {
+                const Eight<T> gv = *(const Eight<T>*)g;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) yv.v[i] = gv.v[i] > (T)0 ? yv.v[i] : (T)0;
+            }
+            *(Eight<T>*)y = yv;
+        } else {
+            for (int i = 0; c0 + i < a.cols; ++i) {
+                const bool on = (keep >> i & 1) && (!g || g[i] > (T)0);
+                y[i] = on ? (T)((R)x[i] * scale) : (T)0;
+            }
+        }
+    }
+}
+
+template <typename T>
+hipError_t launch(const DropoutArgs& a, void* Y, int64_t ldy, hipStream_t s)
+{
+    const int64_t chunks = (a.cols + 7) / 8;
+    int tx = 1;
+    while (tx < 256 && tx < chunks) tx *= 2;
+    const int64_t gx = (chunks + tx - 1) / tx, rows_per = 256 / tx;
+    int64_t gy = (a.rows + rows_per - 1) / rows_per;
+    if (gy > 65535) gy = 65535;
+    dropout_kernel<T><<<dim3((unsigned)gx, (unsigned)gy), 256, 0, s>>>(a, (T*)Y, ldy, tx);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_dropout(int dtype, const DropoutArgs& a, void* Y, int64_t ldy, hipStream_t s)
+{
+    switch (dtype) {
+    case 0: return launch<float>(a, Y, ldy, s);
+    case 1: return launch<double>(a, Y, ldy, s);
+    case 2: return launch<bf16_t>(a, Y, ldy, s);
+    default: return launch<f16_t>(a, Y, ldy, s);
+    }
+}
+
+}  // namespace sbx

@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "launch.hpp"
+#include "philox.hpp"
 
 namespace sbx {
 
@@ -204,20 +205,7 @@ namespace {
 __device__ inline void philox_block(uint64_t seed, uint32_t stream, uint64_t block,
                                     uint32_t (&w)[4])
 {
-    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = stream, c3 = 0;
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint32_t lo0 = 0xD2511F53u * c0, hi0 = __umulhi(0xD2511F53u, c0);
-        const uint32_t lo1 = 0xCD9E8D57u * c2, hi1 = __umulhi(0xCD9E8D57u, c2);
-        c0 = hi1 ^ c1 ^ k0;
-        c1 = lo1;
-        c2 = hi0 ^ c3 ^ k1;
-        c3 = lo0;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-    w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
+    sbx::philox4x32(seed, (uint32_t)block, (uint32_t)(block >> 32), stream, 0, w);
 }
 
 __device__ inline double u53(uint32_t a, uint32_t b)

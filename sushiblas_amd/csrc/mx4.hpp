@@ -1,0 +1,83 @@
+// mx4.hpp -- the dropout and the microscaled 4-bit (MXFP4) operators: their
+// arguments, launchers and shared device code.
+//
+// An MXFP4 matrix is the OCP microscaling format with e2m1 elements: blocks of
+// 32 along a row, v = element * 2^(code - 127), one e8m0 code per block (255:
+// the block is NaN).  Elements are packed two a byte, the even one in the low
+// half; a row's last block is filled with zeros, so a row takes 16 bytes per
+// block.  Codes lie in groups of 8 blocks (256 elements): block b of row r has
+// its code at S[(b / 8) * lds + 8 * r + b % 8].  So the codes that a tile of
+// rows needs for 256 elements are one run of memory, and a lane of a matrix
+// instruction has the codes of its row in one 8-byte load.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "philox.hpp"
+
+namespace sbx {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// Matrices the elementwise operators read, with their dropout.
+//   keep(r, c): 16 bits of Philox (key = seed, counter = (c / 8, r, stream_id,
+//   kDropoutTag); word c % 8 / 2, its half c % 2) against `threshold`.  The
+//   counter comes from the place in the matrix alone, so a backward pass, or
+//   another kernel, makes the same mask again and none is stored.  The last
+//   counter word keeps it apart from the fills (0 there).
+struct DropoutArgs {
+    const void* X;
+    int64_t ldx;
+    const void* gate;  // null, or values that pass where they are > 0
+    int64_t ldg;
+    int64_t rows, cols;
+    uint64_t seed;
+    uint32_t stream_id;
+    uint32_t threshold;  // 65536 * p, rounded; 0: no dropout
+    double scale;        // 65536 / (65536 - threshold): the mean stays, whatever p rounds to
+};
+
+constexpr uint32_t kDropoutTag = 0x44524F50;
+
+struct Mx4Out {
+    uint8_t* P;  // null: not wanted
+    int64_t ldp;
+    uint8_t* S;
+    int64_t lds;
+};
+
+struct Mx4GemmArgs {
+    const uint8_t *A, *SA, *B, *SB;
+    int64_t lda, ldsa, ldb, ldsb;
+    void* C;
+    int64_t ldc;
+    int m, n, k;
+    float alpha, beta;
+    int relu;
+};
+
+// dtype: an sbx_dtype that the caller has checked.
+hipError_t launch_dropout(int dtype, const DropoutArgs& a, void* Y, int64_t ldy, hipStream_t s);
+hipError_t launch_mx4_quantize(int dtype, const DropoutArgs& a, const Mx4Out& rows,
+                               const Mx4Out& cols, hipStream_t s);
+hipError_t launch_mx4_dequantize(int dtype, int64_t rows, int64_t cols, const uint8_t* P,
+                                 int64_t ldp, const uint8_t* S, int64_t lds, void* Y, int64_t ldy,
+                                 hipStream_t s);
+hipError_t launch_mx4_gemm(int dtype, const Mx4GemmArgs& a, hipStream_t s);
+
+// The eight keep decisions of columns 8 * chunk .. + 7 of a row, one bit each.
+__device__ inline uint32_t keep_bits(const DropoutArgs& a, uint32_t row, uint32_t chunk)
+{
+    uint32_t w[4], bits = 0;
+    philox4x32(a.seed, chunk, row, a.stream_id, kDropoutTag, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bits |= (uint32_t)((w[i] & 0xffff) >= a.threshold) << (2 * i);
+        bits |= (uint32_t)((w[i] >> 16) >= a.threshold) << (2 * i + 1);
+    }
+    return bits;
+}
+
+}  // namespace sbx
