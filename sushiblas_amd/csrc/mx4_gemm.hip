@@ -17,20 +17,28 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRsrcWord3 = 0x00020000;
 constexpr int kOutside = (int)0x80000000u;  // an offset past every descriptor's end: reads zeros
 
-// c += b * a^T.  As assembly, so that the sums stay where they are: given the
-// builtin, the compiler moves the 256 sums of a 128 x 128 wave between registers
-// (400 moves per 128 products).  It knows nothing of the unit's latency then: the
-// caller keeps two instructions between a VALU write of an operand and its use here
-// (there are none in the loop), and waits (settle) before it reads sums.
+// c += b * a^T, with byte H of the codes.  As assembly, so that the sums stay
+// where they are: given the builtin, the compiler moves the 256 sums of a 128 x 128
+// wave between registers (400 moves per 128 products).  It knows nothing of the
+// unit's latency then: the caller keeps two instructions between a VALU write of an
+// operand and its use here, and waits (settle) before it reads sums.
+template <int H>
 __device__ inline void mma(f32x4& c, i32x4 b, int code_b, i32x4 a, int code_a)
 {
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-                 : "+a"(c)
-                 : "v"(b), "v"(a), "v"(code_b), "v"(code_a));
+    if constexpr (H == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(c)
+                     : "v"(b), "v"(a), "v"(code_b), "v"(code_a));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] "
+                     "cbsz:4 blgp:4"
+                     : "+a"(c)
+                     : "v"(b), "v"(a), "v"(code_b), "v"(code_a));
 }
 
 template <int MB, int NB>
@@ -55,86 +63,85 @@ __device__ inline i32x4 descriptor(const uint8_t* base, int64_t bytes)
     return d;
 }
 
-// 16 (or 4) bytes per lane from memory to LDS at `lds` + 16 (4) * lane.  As
-// assembly, because the compiler makes every LDS read after the builtin wait
-// for all of them; load_stage's caller waits.  They write no register.
-__device__ inline void load16_lds(uint32_t lds, int voff, i32x4 rsrc, int soff)
+// Loads 16 bytes per lane straight to LDS, to `lds` + 16 * lane.  As assembly, because
+// the compiler makes every LDS read after the builtin wait for all such loads; the caller
+// waits.  It writes no register.
+__device__ inline void load_lds(uint32_t lds, int voff, i32x4 rsrc, int soff)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
                  "v"(voff), "s"(rsrc), "s"(soff)
                  : "memory");
 }
-__device__ inline void load4_lds(uint32_t lds, int voff, i32x4 rsrc)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds),
-                 "v"(voff), "s"(rsrc)
-                 : "memory");
-}
 template <int N>
 __device__ inline void wait_loads_and_barrier()
 {
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// 16 bytes of results, from or to memory that is aligned to the element only.
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-    T v[8];
+struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    T v[16 / sizeof(T)];
 };
 
-// Eight neighbouring results of a row, `left` of them inside C.
 template <typename T>
-__device__ inline void store8(T* c, const float (&acc)[8], int left, const Mx4GemmArgs& p)
+__device__ inline T result(float acc, float c, const Mx4GemmArgs& p)
 {
-    if (left >= 8) {
-        Eight<T> o, in;
-        if (p.beta != 0.0f) in = *(const Eight<T>*)c;
+    const float v = p.beta != 0.0f ? p.alpha * acc + p.beta * c : p.alpha * acc;
+    return (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
+}
+
+// Neighbouring results of a row, `left` of them inside C.
+template <typename T>
+__device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], int left, const Mx4GemmArgs& p)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (left >= V) {
+        Vec<T> o, in;
+        if (p.beta != 0.0f) in = *(const Vec<T>*)c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = p.alpha * acc[e];
-            if (p.beta != 0.0f) v += p.beta * (float)in.v[e];
-            o.v[e] = (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
-        }
-        *(Eight<T>*)c = o;
+        for (int e = 0; e < V; ++e) o.v[e] = result<T>(acc[e], p.beta != 0.0f ? (float)in.v[e] : 0.0f, p);
+        // (past the L2s, that keep the operands then: 8192^2 x 512 to bf16 60.5 -> 55.1 us, 4096^2 x 1024
+        // 23.4 -> 16.7 us)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), (u32x4*)c);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (e < left) {
-                float v = p.alpha * acc[e];
-                if (p.beta != 0.0f) v += p.beta * (float)c[e];
-                c[e] = (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
-            }
-        }
+        for (int e = 0; e < V; ++e)
+            if (e < left) c[e] = result<T>(acc[e], p.beta != 0.0f ? (float)c[e] : 0.0f, p);
     }
 }
 
-// Tile of (32 MB) x (32 NB) of C by 2 x 2 waves of 16 MB x 16 NB, 128 terms at a
-// time through a ring of four LDS stages.
+// Tile of BM x BN = (16 MB WM) x (16 NB WN) of C by WM x WN waves of 16 MB x 16 NB,
+// 256 terms at a time through two LDS stages.
 //
-// A stage holds the tile's rows of 64 bytes (4 blocks) and their 4 codes.  It is
-// filled by loads that go straight to LDS, which place lanes' 16 bytes one after
-// another: a wave's instruction fills 16 rows, and the order in which a row's four
-// blocks lie is permuted by the address each lane reads instead, so that the 16
-// lanes of a fragment read meet no bank twice (block b of row x at place
-// b ^ swizzle(x)).
-//   Stage t + 3 is asked for while t is multiplied and t + 1 is read from LDS
-// into the other set of registers, so a load has two stages' time to arrive and
-// neither LDS latency nor memory's is waited for.  One barrier per stage: after it,
-// t + 1 is there for all waves, and all have read t, the last reader of t - 1's
-// place being past its reads since before the last barrier.
+// A stage holds the tile's rows of 128 bytes (8 blocks, a cache line) and their 8 codes.
+// It is filled by loads that go straight to LDS, which place lanes' 16 bytes one after
+// another: a wave's instruction fills 8 rows, and the order in which a row's blocks lie
+// is permuted by the address each lane reads instead: block b of row x at place
+// b ^ swizzle(x).  LDS has 64 banks, and serves 16 bytes a lane to lanes 0-3, 12-15,
+// 20-27, then to the others of 0-31, then 32-63 likewise; with the swizzles below no
+// two of such 16 lanes of a fragment read meet (SQ_LDS_BANK_CONFLICT: 0).
+//   A stage is multiplied in two halves; lane group q takes block 2q + h of a row in
+// half h, so its codes for both are one 16-bit read.
+//   While a half is multiplied, the next is read from LDS: A's block i into its own
+// place once the pass over it is done, B's blocks into a second set.  Between the
+// halves of stage t every wave has read all of it: a barrier there frees its place for
+// t + 2, and sees t + 1 arrived, asked for a whole stage's time before.
 //   B's block j holds the tile's rows 32 (j / 2) + 4 (j % 2) + 8 (i / 4) + i % 4 at
 // its index i, so that a lane's results of blocks j, j + 1 are 8 neighbouring columns.
-template <typename T, int MB, int NB>
-__global__ void __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
+template <typename T, int WM, int WN, int MB, int NB>
+__global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
 {
-    constexpr int BM = 32 * MB, BN = 32 * NB;
-    constexpr int OFF_B = BM * 64, OFF_SA = OFF_B + BN * 64, OFF_SB = OFF_SA + BM * 4;
-    constexpr int STAGE = OFF_SB + BN * 4;
-    constexpr int LA = BM / 64, LB = BN / 64;            // 16-byte loads per wave and stage
-    constexpr int SI = (BM + BN) / 64;                   // wave-wide loads of codes per stage
-    constexpr int LS = SI >= 4 ? SI / 4 : 1;             // of them per wave (waves over SI repeat one)
-    constexpr int LOADS = LA + LB + LS;
-    static_assert(BM % 64 == 0 && BN % 64 == 0, "whole wave-wide loads");
-    __shared__ __align__(16) char lds[4 * STAGE];
+    constexpr int WAVES = WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN;
+    constexpr int CA = BM * 8 < 1024 ? 1024 : BM * 8, CB = BN * 8 < 1024 ? 1024 : BN * 8;  // codes
+    constexpr int OFF_B = BM * 128, OFF_SA = OFF_B + BN * 128, OFF_SB = OFF_SA + CA;
+    constexpr int STAGE = OFF_SB + CB;
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // loads per wave and stage
+    constexpr int NCA = CA / 1024, NC = NCA + CB / 1024;     // of codes, one by each of the first waves
+    static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && NC <= WAVES && (LA + LB) % MB == 0,
+                  "whole wave-wide loads");
+    static_assert(MB >= NB && NB % 2 == 0, "");
+    __shared__ __align__(16) char lds[2 * STAGE];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -147,161 +154,219 @@ __global__ void __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) mx4_gemm_kernel(Mx
     const int group = 8 * tiles_n, g0 = id / group * 8;
     const int gh = tiles_m - g0 < 8 ? tiles_m - g0 : 8;
     const int m0 = (g0 + id % group % gh) * BM, n0 = id % group / gh * BN;
-    const int nb = (p.k + 31) / 32, nk = (nb + 3) / 4;
+    const int nb = (p.k + 31) / 32, nk = (nb + 7) / 8;
 
     const int rows_a = p.m - m0 < BM ? p.m - m0 : BM, rows_b = p.n - n0 < BN ? p.n - n0 : BN;
     i32x4 da = descriptor(p.A + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + 16 * nb);
     i32x4 db = descriptor(p.B + (int64_t)n0 * p.ldb, (int64_t)(rows_b - 1) * p.ldb + 16 * nb);
 
-    // what this lane loads: a row's 16 bytes
-    auto swz_a = [](int x) { return ((x >> 1 ^ x >> 3) & 1) | (x >> 1 & 2); };
-    auto swz_b = [](int x) { return ((x >> 1 ^ x >> 4) & 1) | (x >> 2 & 2); };
-    // (A's rows of a wave's loads are 16 apart and permuted alike, B's in two ways)
-    int va[LA], vb[LB];
-    const int ca = lane % 4 ^ swz_a(lane / 4);
-    const int cb[2] = {lane % 4 ^ swz_b(wave * LB * 16 + lane / 4), lane % 4 ^ swz_b((wave * LB + 1) * 16 + lane / 4)};
+    // what this lane loads: 16 bytes of a row (rows past the operand's end lie past the
+    // descriptor's); the swizzles of rows 8 apart are alike or two
+    auto swz_a = [](int x) { return (x >> 1 & 1) ^ (x & 8 ? 6 : 0); };
+    auto swz_b = [](int x) { return (x >> 1 & 1) ^ (x & 16 ? 6 : 0); };
+    int va[LA], vb[LB], ca[LA], cb[LB];
 #pragma unroll
-    for (int j = 0; j < LA; ++j) va[j] = (int)(((wave * LA + j) * 16 + lane / 4) * p.lda) + ca * 16;
-#pragma unroll
-    for (int j = 0; j < LB; ++j) vb[j] = (int)(((wave * LB + j) * 16 + lane / 4) * p.ldb) + cb[j % 2] * 16;
-
-    // codes: 64 rows of A or of B, their groups' addresses in turn
-    uint64_t sp[LS];
-    int64_t ss[LS];
-    int sn[LS];
-#pragma unroll
-    for (int j = 0; j < LS; ++j) {
-        const int i = (wave * LS + j) % SI;
-        const bool b = i >= BM / 64;
-        const int x = (b ? i - BM / 64 : i) * 64;
-        const int left = (b ? rows_b : rows_a) - x;
-        sp[j] = b ? (uint64_t)(p.SB + 8 * (int64_t)(n0 + x)) : (uint64_t)(p.SA + 8 * (int64_t)(m0 + x));
-        ss[j] = b ? p.ldsb : p.ldsa;
-        sn[j] = left > 0 ? 8 * left : 0;
+    for (int j = 0; j < LA; ++j) {
+        const int x = (wave * LA + j) * 8 + lane / 8;
+        ca[j] = lane % 8 ^ swz_a(x);
+        va[j] = (int)(x * p.lda) + ca[j] * 16;
     }
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+        const int x = (wave * LB + j) * 8 + lane / 8;
+        cb[j] = lane % 8 ^ swz_b(x);
+        vb[j] = (int)(x * p.ldb) + cb[j] * 16;
+    }
+    // and codes: the first NC waves, 128 rows of A or of B each
+    const bool code_b = wave >= NCA;
+    const int code_row = (code_b ? wave - NCA : wave) * 128;
+    const int code_left = (code_b ? rows_b : rows_a) - code_row;
+    const uint8_t* code_at = code_b ? p.SB + 8 * (int64_t)(n0 + code_row) : p.SA + 8 * (int64_t)(m0 + code_row);
+    const int64_t code_step = code_b ? p.ldsb : p.ldsa;
 
-    auto load_stage = [&](int t) {  // for t = 0, 1, 2 ..
-        const uint32_t at = lds0 + (t & 3) * STAGE;
-        // blocks past the last one are zeros, whatever lies there
-        const bool out_a = 4 * t + ca >= nb, out_b[2] = {4 * t + cb[0] >= nb, 4 * t + cb[1] >= nb};
-#pragma unroll
-        for (int j = 0; j < LA; ++j)
-            load16_lds(at + (wave * LA + j) * 1024, out_a ? kOutside : va[j], da, t * 64);
-#pragma unroll
-        for (int j = 0; j < LB; ++j)
-            load16_lds(at + OFF_B + (wave * LB + j) * 1024, out_b[j % 2] ? kOutside : vb[j], db, t * 64);
-#pragma unroll
-        for (int j = 0; j < LS; ++j) {
-            const i32x4 d = {(int)(uint32_t)sp[j], (int)(uint32_t)(sp[j] >> 32) & 0xffff, t < nk ? sn[j] : 0, kRsrcWord3};
-            load4_lds(at + OFF_SA + (wave * LS + j) % SI * 256, lane * 8 + t % 2 * 4, d);
-            sp[j] += t & 1 ? ss[j] : 0;
+    // Load x < LA + LB of stage t; the codes go with the last.  Blocks past the last one,
+    // and all of a stage past the last, are zeros, whatever lies there.
+    auto load_part = [&](int t, int x) {
+        const uint32_t at = lds0 + (t & 1) * STAGE;
+        const int left = nb - 8 * t;
+        if (x < LA)
+            load_lds(at + (wave * LA + x) * 1024, ca[x % LA] < left ? va[x % LA] : kOutside, da, t * 128);
+        else
+            load_lds(at + OFF_B + (wave * LB + x - LA) * 1024, cb[(x - LA) % LB] < left ? vb[(x - LA) % LB] : kOutside,
+                     db, t * 128);
+        if (x == LA + LB - 1 && wave < NC) {
+            const uint64_t s = (uint64_t)code_at;
+            const int n = left <= 0 || code_left <= 0 ? 0 : code_left > 128 ? 1024 : 8 * code_left;
+            load_lds(at + OFF_SA + wave * 1024, lane * 16,
+                     i32x4{(int)(uint32_t)s, (int)(uint32_t)(s >> 32) & 0xffff, n, kRsrcWord3}, 0);
+            code_at += code_step;
         }
     };
-
-    i32x4 fa[2][MB], fb[NB];
-    int sa[2][MB], sb[NB];
-    const int wm = wave % 2 * (16 * MB), wn = wave / 2 * (16 * NB);
-    const int rb = r / 4 * 8 + r % 4;
-    const int at_a = (wm + r) * 64 + (q ^ swz_a(r)) * 16, at_b = OFF_B + (wn + rb) * 64 + (q ^ swz_b(rb)) * 16;
-    const int at_sa = OFF_SA + (wm + r) * 4 + q, at_sb = OFF_SB + (wn + rb) * 4 + q;
-    auto read_a = [&](auto set, int i, const char* at) {
-        constexpr int S = decltype(set)::value;
-        fa[S][i] = *(const i32x4*)(at + at_a + i * 1024);
-        sa[S][i] = *(const uint8_t*)(at + at_sa + i * 64);
-    };
-    auto read_b = [&](int j, const char* at) {
-        fb[j] = *(const i32x4*)(at + at_b + j / 2 * 2048 + j % 2 * 256);
-        sb[j] = *(const uint8_t*)(at + at_sb + j / 2 * 128 + j % 2 * 16);
-    };
-    // Codes as whole registers: without this the compiler widens them from bytes
-    // at their use, too near before it (see mma).
-    auto whole = [](int& code) { asm volatile("" : "+v"(code)); };
     // Codes past the last block may be NaN's: the last stage's are cleared.
     auto clear_codes = [&](int t) {
-        if (t == nk - 1 && nb % 4) {
-            for (int i = threadIdx.x; i < BM + BN; i += 256)
-                ((uint32_t*)(lds + (t & 3) * STAGE + OFF_SA))[i] &= (1u << nb % 4 * 8) - 1;
+        if (t == nk - 1 && nb % 8) {
+            const uint64_t mask = (1ull << nb % 8 * 8) - 1;
+            for (int i = threadIdx.x; i < (CA + CB) / 8; i += 64 * WAVES)
+                ((uint64_t*)(lds + (t & 1) * STAGE + OFF_SA))[i] &= mask;
             __syncthreads();
         }
     };
 
+    i32x4 fa[MB], fb[2][NB];
+    int sa[MB], sb[NB], sb_next[NB];
+    const int wm = wave % WM * (16 * MB), wn = wave / WM * (16 * NB);
+    const int rb = r / 4 * 8 + r % 4;
+    int at_a[2], at_b[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        at_a[h] = (wm + r) * 128 + (2 * q + h ^ swz_a(r)) * 16;
+        at_b[h] = OFF_B + (wn + rb) * 128 + (2 * q + h ^ swz_b(rb)) * 16;
+    }
+    const int at_sa = OFF_SA + (wm + r) * 8 + 2 * q, at_sb = OFF_SB + (wn + rb) * 8 + 2 * q;
+    auto read_a = [&](auto half, int i, const char* at) {
+        fa[i] = *(const i32x4*)(at + at_a[decltype(half)::value] + i * 2048);
+    };
+    auto read_b = [&](auto half, int j, const char* at) {
+        constexpr int H = decltype(half)::value;
+        fb[H][j] = *(const i32x4*)(at + at_b[H] + j / 2 * 4096 + j % 2 * 512);
+    };
+    auto read_sa = [&](int i, const char* at) { sa[i] = *(const uint16_t*)(at + at_sa + i * 128); };
+    auto read_sb = [&](int j, const char* at) {
+        sb_next[j] = *(const uint16_t*)(at + at_sb + j / 2 * 256 + j % 2 * 32);
+    };
+    // Codes as whole registers: without this the compiler widens them at their use, too
+    // near before it (see mma).
+    auto whole = [](int& code) { asm volatile("" : "+v"(code)); };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+
     f32x4 acc[MB][NB] = {};
-    // Multiplies stage t, and reads t + 1: its A blocks into the other registers in the
-    // first half of the passes, its B block j into the place of pass j's.
-    auto step = [&](auto set, int t) {
-        constexpr int S = decltype(set)::value;
-        constexpr int PER = 2 * MB / NB;  // A blocks read in a pass
-        static_assert(PER * NB == 2 * MB && NB % 2 == 0, "");
-        wait_loads_and_barrier<LOADS>();
-        clear_codes(t + 1);
-        load_stage(t + 3);
-        const char* at = lds + ((t + 1) & 3) * STAGE;
+    // Multiplies half H of a stage and reads the next half, from the stage at `at`.
+    // beside(i): what else goes with pass i.  Reads begin after the first pass (so A's block
+    // i is read a pass later than its place is free).
+    auto multiply = [&](auto half, const char* at, auto&& beside) {
+        constexpr int H = decltype(half)::value;
+        constexpr std::integral_constant<int, 1 - H> next{};
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            whole(sb[j == 0 ? NB - 1 : j - 1]);  // what the pass before read
-            if (j > 0 && j <= NB / 2)
+        for (int i = 0; i < MB; ++i) {
+            if (i > 2 && H == 1) {  // codes read two passes before
+                whole(sa[i - 3]);
+                if (i - 3 < NB) whole(sb_next[i - 3]);
+            }
+            // one instruction of the reads after each product: a wave issues in order, and what
+            // comes in a row keeps the matrix unit waiting
+            const int x0 = i - 1, x1 = i == MB - 1 ? i : i - 1;  // A's blocks read in this pass
 #pragma unroll
-                for (int i = 0; i < PER; ++i) whole(sa[1 - S][(j - 1) * PER + i]);
+            for (int j = 0; j < NB; ++j) {
+                mma<H>(acc[i][j], fb[H][j], sb[j], fa[i], sa[i]);
+                if (i == 0) {
+                    if (j == 0) beside(i);
+                } else {
+                    if (j == 0) read_a(next, x0, at);
+                    if (j == (NB > 2 ? 1 : 0) && H == 1) read_sa(x0, at);
+                    if (j == NB / 2 && x0 < NB) read_b(next, x0, at);
+                    if (j == NB - 1 && x0 < NB && H == 1) read_sb(x0, at);
+                    if (j == NB - 1 && x1 > x0) {
+                        read_a(next, x1, at);
+                        if (H == 1) read_sa(x1, at);
+                        if (x1 < NB) {
+                            read_b(next, x1, at);
+                            if (H == 1) read_sb(x1, at);
+                        }
+                    }
+                    if (j == NB - 1) beside(i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (H == 1) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i) mma(acc[i][j], fb[j], sb[j], fa[S][i], sa[S][i]);
-            read_b(j, at);
-            if (j < NB / 2)
+            for (int i = MB - 3 > 0 ? MB - 3 : 0; i < MB; ++i) whole(sa[i]);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) read_a(std::integral_constant<int, 1 - S>{}, j * PER + i, at);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < NB; ++j) {
+                whole(sb_next[j]);
+                sb[j] = sb_next[j];
+                whole(sb[j]);
+            }
+            asm volatile("s_nop 1");
         }
     };
 
     if (nk > 0) {
         // (a descriptor that vector instructions wrote may be read 5 instructions later)
         asm volatile("s_nop 4" : "+s"(da), "+s"(db));
-        load_stage(0);
-        load_stage(1);
-        load_stage(2);
-        wait_loads_and_barrier<2 * LOADS>();
+#pragma unroll
+        for (int x = 0; x < 2 * (LA + LB); ++x) load_part(x / (LA + LB), x % (LA + LB));
+        wait_loads_and_barrier<LA + LB>();  // (the waves that load codes wait for one more)
         clear_codes(0);
 #pragma unroll
-        for (int i = 0; i < MB; ++i) read_a(std::integral_constant<int, 0>{}, i, lds);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) read_b(j, lds);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) whole(sa[0][i]);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) whole(sb[j]);
-        for (int t = 0; t < nk; t += 2) {  // (of an odd number, a stage of zeros is the last)
-            step(std::integral_constant<int, 0>{}, t);
-            step(std::integral_constant<int, 1>{}, t + 1);
+        for (int i = 0; i < MB; ++i) {
+            read_a(first, i, lds);
+            read_sa(i, lds);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is written to LDS past the end
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            read_b(first, j, lds);
+            read_sb(j, lds);
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) whole(sa[i]);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            sb[j] = sb_next[j];
+            whole(sb[j]);
+        }
+        asm volatile("s_nop 1");
+        for (int t = 0; t < nk; ++t) {
+            multiply(first, lds + (t & 1) * STAGE, [](int) {});
+            // (after the last stage: what lies there)
+            multiply(second, lds + ((t + 1) & 1) * STAGE, [&](int i) {
+                if (i == 0) {
+                    wait_loads_and_barrier<0>();
+                    clear_codes(t + 1);
+                }
+                // spread over the passes: a wave that asks for all of them at once waits its
+                // turn at the CU's one load unit instead of multiplying
+#pragma unroll
+                for (int x = 0; x < (LA + LB) / MB; ++x) load_part(t + 2, i * ((LA + LB) / MB) + x);
+            });
+        }
+        wait_loads_and_barrier<0>();  // nothing more is written to LDS
     }
     settle(acc);
 
-    T* C = (T*)p.C;
+    // Out through LDS, 16 rows of the wave's at a time, so that an instruction stores whole
+    // rows of them (from the registers it would store 32 columns of 16 rows).
+    constexpr int V = 16 / sizeof(T), COLS = 16 * NB, PITCH = COLS + 4;
+    constexpr int PER_ROW = COLS / V, ROWS = 64 / PER_ROW;  // lanes per row, rows per instruction
+    static_assert(2 * 16 * PITCH * 4 * WAVES <= 2 * STAGE, "");
+    float* out = (float*)lds + wave * 2 * 16 * PITCH;
+    const int n = n0 + wn + lane % PER_ROW * V;
+    T* C = (T*)p.C + n;
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-        const int m = m0 + wm + 16 * i + r;
-        if (m >= p.m) continue;
+        float* half = out + i % 2 * 16 * PITCH;
 #pragma unroll
-        for (int j = 0; j < NB; j += 2) {
-            const int n = n0 + wn + 16 * j + 8 * q;
-            float v[8];
+        for (int j = 0; j < NB; ++j)
+            *(f32x4*)(half + r * PITCH + j / 2 * 32 + 8 * q + j % 2 * 4) = acc[i][j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = acc[i][j][e];
-                v[4 + e] = acc[i][j + 1][e];
-            }
-            if (n < p.n) store8(C + (int64_t)m * p.ldc + n, v, p.n - n, p);
+        for (int x = 0; x < 16; x += ROWS) {
+            const int row = x + lane / PER_ROW, m = m0 + wm + 16 * i + row;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = half[row * PITCH + lane % PER_ROW * V + e];
+            if (m < p.m && n < p.n) store_results(C + (int64_t)m * p.ldc, v, p.n - n, p);
         }
     }
 }
 
-template <typename T, int MB, int NB>
+template <typename T, int WM, int WN, int MB, int NB>
 hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 {
-    constexpr int BM = 32 * MB, BN = 32 * NB;
+    constexpr int BM = 16 * MB * WM, BN = 16 * NB * WN;
     const int tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
     if ((int64_t)tm * tn > 0x7fffffff) return hipErrorInvalidValue;
-    mx4_gemm_kernel<T, MB, NB><<<(unsigned)(tm * tn), 256, 0, s>>>(a, tm, tn);
+    mx4_gemm_kernel<T, WM, WN, MB, NB><<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, tm, tn);
     return hipGetLastError();
 }
 
@@ -309,9 +374,9 @@ template <typename T>
 hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
 {
     auto tiles = [&](int64_t b) { return (a.m + b - 1) / b * ((a.n + b - 1) / b); };
-    if (tiles(256) >= 128) return launch_tile<T, 8, 8>(a, s);
-    if (tiles(128) >= 128) return launch_tile<T, 4, 4>(a, s);
-    return launch_tile<T, 2, 2>(a, s);
+    if (tiles(256) >= 128) return launch_tile<T, 2, 4, 8, 4>(a, s);
+    if (tiles(128) >= 128) return launch_tile<T, 2, 2, 4, 4>(a, s);
+    return launch_tile<T, 2, 2, 2, 2>(a, s);
 }
 
 }  // namespace
