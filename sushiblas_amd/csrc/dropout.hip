@@ -40,13 +40,14 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64
         const T* x = (const T*)a.X + row * a.ldx + c0;
         const T* g = a.gate ? (const T*)a.gate + row * a.ldg + c0 : nullptr;
         T* y = Y + row * ldy + c0;
-        const uint32_t keep = a.threshold ? keep_bits(a, (uint32_t)row, chunk) : 0xffu;
+        uint32_t keep[4];
+        if (a.threshold) keep_words(a, (uint32_t)row, chunk, keep);
         if (c0 + 8 <= a.cols) {
             const Eight<T> xv = *(const Eight<T>*)x;
             Eight<T> yv;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                yv.v[i] = keep >> i & 1 ? (T)((R)xv.v[i] * scale) : (T)0;
+                yv.v[i] = !a.threshold || kept(a, keep, i) ? (T)((R)xv.v[i] * scale) : (T)0;
             if (g) {
                 const Eight<T> gv = *(const Eight<T>*)g;
 #pragma unroll
@@ -54,8 +55,10 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64
             }
             *(Eight<T>*)y = yv;
         } else {
-            for (int i = 0; c0 + i < a.cols; ++i) {
-                const bool on = (keep >> i & 1) && (!g || g[i] > (T)0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (c0 + i >= a.cols) continue;
+                const bool on = (!a.threshold || kept(a, keep, i)) && (!g || g[i] > (T)0);
                 y[i] = on ? (T)((R)x[i] * scale) : (T)0;
             }
         }

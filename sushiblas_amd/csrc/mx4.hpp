@@ -67,17 +67,14 @@ hipError_t launch_mx4_dequantize(int dtype, int64_t rows, int64_t cols, const ui
                                  hipStream_t s);
 hipError_t launch_mx4_gemm(int dtype, const Mx4GemmArgs& a, hipStream_t s);
 
-// The eight keep decisions of columns 8 * chunk .. + 7 of a row, one bit each.
-__device__ inline uint32_t keep_bits(const DropoutArgs& a, uint32_t row, uint32_t chunk)
+// The random numbers of columns 8 * chunk .. + 7 of a row, and whether number e stays.
+__device__ inline void keep_words(const DropoutArgs& a, uint32_t row, uint32_t chunk, uint32_t (&w)[4])
 {
-    uint32_t w[4], bits = 0;
     philox4x32(a.seed, chunk, row, a.stream_id, kDropoutTag, w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bits |= (uint32_t)((w[i] & 0xffff) >= a.threshold) << (2 * i);
-        bits |= (uint32_t)((w[i] >> 16) >= a.threshold) << (2 * i + 1);
-    }
-    return bits;
+}
+__device__ inline bool kept(const DropoutArgs& a, const uint32_t (&w)[4], int e)
+{
+    return (e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffff) >= a.threshold;
 }
 
 }  // namespace sbx
