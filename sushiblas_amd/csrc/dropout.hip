@@ -18,13 +18,6 @@ struct Arith<double> {
     typedef double type;
 };
 
-// Eight values, from memory that is aligned to the element only (the device
-// serves such 16-byte accesses).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-    T v[8];
-};
-
 // Threads form TX chunks of 8 columns by 256 / TX rows.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64_t ldy, int tx)
@@ -53,7 +46,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64
 #pragma unroll
                 for (int i = 0; i < 8; ++i) yv.v[i] = gv.v[i] > (T)0 ? yv.v[i] : (T)0;
             }
-            *(Eight<T>*)y = yv;
+            store_past(y, yv);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

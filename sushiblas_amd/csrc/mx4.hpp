@@ -77,4 +77,26 @@ __device__ inline bool kept(const DropoutArgs& a, const uint32_t (&w)[4], int e)
     return (e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffff) >= a.threshold;
 }
 
+// Eight neighbouring values, in memory that is aligned to the element only (the device
+// serves such 16-byte accesses).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+    T v[8];
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Stores them past the L2s.
+template <typename T>
+__device__ inline void store_past(T* to, const Eight<T>& y)
+{
+    struct Words {
+        u32x4 w[sizeof(T) / 2];
+    };
+    const Words w = __builtin_bit_cast(Words, y);
+    typedef u32x4 __attribute__((aligned(2))) loose_t;  // (16-byte accesses need no alignment)
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) __builtin_nontemporal_store(w.w[i], (loose_t*)to + i);
+}
+
 }  // namespace sbx

@@ -17,7 +17,6 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRsrcWord3 = 0x00020000;
 constexpr int kOutside = (int)0x80000000u;  // an offset past every descriptor's end: reads zeros
@@ -39,6 +38,13 @@ __device__ inline void mma(f32x4& c, i32x4 b, int code_b, i32x4 a, int code_a)
                      "cbsz:4 blgp:4"
                      : "+a"(c)
                      : "v"(b), "v"(a), "v"(code_b), "v"(code_a));
+}
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ inline i32x8 widen(i32x4 v)
+{
+    return i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
 }
 
 template <int MB, int NB>
@@ -360,6 +366,151 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
     }
 }
 
+// Products with a narrow operand Y of up to 128 rows (tokens, or the columns of a narrow C) and
+// any number of rows of the wide one X (XA: A, else B), which is read from memory once: a
+// workgroup takes 16 XB rows of X and all of Y, its eight waves each an eighth of the terms, in
+// groups of 256 by turns, straight from memory to registers (a lane's 32 neighbouring bytes of a
+// row; the group after is under way meanwhile).  The waves' sums are added up in LDS, in order.
+constexpr int kSkinnyWaves = 8;
+
+template <int N>
+struct Group {
+    i32x4 v[N][2];
+    int code[N];  // two codes in its low bytes
+};
+
+// The rows of an operand that a workgroup takes, and the lane's place in them.
+struct Strip {
+    __amdgpu_buffer_rsrc_t rows;
+    const uint8_t* codes;
+    int64_t lds;
+    int count, ld, at, code_at;
+
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n,
+                                int most, int nb, int lane)
+    {
+        count = min(n - first, most);
+        ld = (int)ld_;
+        lds = lds_;
+        rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P) + first * ld_, (short)0,
+                                                 (count - 1) * ld + 16 * nb, kRsrcWord3);
+        codes = S + 8 * (int64_t)first;
+        at = lane % 16 * ld + lane / 16 * 32;
+        code_at = lane % 16 * 8 + lane / 16 * 2;
+    }
+
+    // Group g (256 terms) of N times 16 rows, zeros past the last row.  blocks: of the lane's
+    // two, those inside (what lies past the last block is not used).
+    template <int N>
+    __device__ inline void load(Group<N>& d, int g, bool tail, int blocks) const
+    {
+        const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(codes) + g * lds, (short)0, 8 * count, kRsrcWord3);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int from = 16 * i * ld + g * 128;
+            d.v[i][0] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, from, 0));
+            d.v[i][1] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 16, from, 0));
+            d.code[i] = __builtin_amdgcn_raw_buffer_load_b16(c, code_at + 128 * i, 0, 0);
+        }
+        if (tail) {
+            const i32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                d.v[i][0] = blocks >= 1 ? d.v[i][0] : zero;
+                d.v[i][1] = blocks >= 2 ? d.v[i][1] : zero;
+                d.code[i] = blocks >= 2 ? d.code[i] : blocks == 1 ? d.code[i] & 0xff : 0;
+            }
+        }
+    }
+};
+
+// AHEAD: the next group's loads are under way while one is multiplied (or else the SIMD's other
+// wave's are).
+template <typename T, int YB, int XB, bool AHEAD, bool XA>
+__global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 8 ? 2 : 4) mx4_skinny_kernel(Mx4GemmArgs p)
+{
+    const int nx = XA ? p.m : p.n, ny = XA ? p.n : p.m;
+    constexpr int PITCH = 16 * YB + 4;
+    __shared__ float part[kSkinnyWaves][16 * PITCH];
+
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int r = lane % 16, q = lane / 16;
+    const int x0 = blockIdx.x * (16 * XB);
+    const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
+    Strip sx, sy;
+    sx.init(XA ? p.A : p.B, XA ? p.lda : p.ldb, XA ? p.SA : p.SB, XA ? p.ldsa : p.ldsb, x0, nx, 16 * XB, nb, lane);
+    sy.init(XA ? p.B : p.A, XA ? p.ldb : p.lda, XA ? p.SB : p.SA, XA ? p.ldsb : p.ldsa, 0, ny, 16 * YB, nb, lane);
+
+    f32x4 acc[XB][YB] = {};
+    Group<XB> x;
+    Group<YB> y;
+    auto load = [&](Group<XB>& x, Group<YB>& y, int g) {
+        const bool tail = 8 * g + 8 > nb;
+        const int blocks = nb - 8 * g - 2 * q;
+        sx.load(x, g, tail, blocks);
+        sy.load(y, g, tail, blocks);
+    };
+    auto multiply = [&](const Group<XB>& x, const Group<YB>& y) {
+#pragma unroll
+        for (int i = 0; i < XB; ++i)
+#pragma unroll
+            for (int j = 0; j < YB; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    widen(x.v[i][0]), widen(y.v[j][0]), acc[i][j], 4, 4, 0, x.code[i], 0, y.code[j]);
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    widen(x.v[i][1]), widen(y.v[j][1]), acc[i][j], 4, 4, 1, x.code[i], 1, y.code[j]);
+            }
+    };
+    if constexpr (AHEAD) {
+        Group<XB> xn;
+        Group<YB> yn;
+        if (wave < groups) load(x, y, wave);
+        for (int g = wave; g < groups; g += 2 * kSkinnyWaves) {
+            if (g + kSkinnyWaves < groups) load(xn, yn, g + kSkinnyWaves);
+            multiply(x, y);
+            if (g + kSkinnyWaves >= groups) break;
+            if (g + 2 * kSkinnyWaves < groups) load(x, y, g + 2 * kSkinnyWaves);
+            multiply(xn, yn);
+        }
+    } else {
+        for (int g = wave; g < groups; g += kSkinnyWaves) {
+            load(x, y, g);
+            multiply(x, y);
+        }
+    }
+    T* C = (T*)p.C;
+#pragma unroll
+    for (int i = 0; i < XB; ++i) {
+        if (i > 0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < YB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[wave][(4 * q + e) * PITCH + 16 * j + r] = acc[i][j][e];
+        __syncthreads();
+        for (int t = threadIdx.x; t < 16 * 16 * YB; t += 64 * kSkinnyWaves) {
+            const int dx = XA ? t / (16 * YB) : t % 16, dy = XA ? t % (16 * YB) : t / 16;  // C's rows run along n
+            const int xr = x0 + 16 * i + dx;
+            if (xr >= nx || dy >= ny) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSkinnyWaves; ++w) v += part[w][dx * PITCH + dy];
+            T* c = C + (XA ? (int64_t)xr * p.ldc + dy : (int64_t)dy * p.ldc + xr);
+            *c = result<T>(v, p.beta != 0.0f ? (float)*c : 0.0f, p);
+        }
+    }
+}
+
+template <typename T, int YB, int XB, bool AHEAD>
+hipError_t launch_skinny(const Mx4GemmArgs& a, hipStream_t s)
+{
+    if (a.m <= a.n)
+        mx4_skinny_kernel<T, YB, XB, AHEAD, false><<<(unsigned)((a.n + 16 * XB - 1) / (16 * XB)), 64 * kSkinnyWaves, 0, s>>>(a);
+    else
+        mx4_skinny_kernel<T, YB, XB, AHEAD, true><<<(unsigned)((a.m + 16 * XB - 1) / (16 * XB)), 64 * kSkinnyWaves, 0, s>>>(a);
+    return hipGetLastError();
+}
+
 template <typename T, int WM, int WN, int MB, int NB>
 hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 {
@@ -373,6 +524,11 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 template <typename T>
 hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
 {
+    const int narrow = a.m < a.n ? a.m : a.n;
+    if (narrow <= 16) return launch_skinny<T, 1, 1, true>(a, s);
+    if (narrow <= 32) return launch_skinny<T, 2, 1, true>(a, s);
+    if (narrow <= 64) return launch_skinny<T, 4, 2, true>(a, s);
+    if (narrow <= 128) return launch_skinny<T, 8, 2, false>(a, s);
     auto tiles = [&](int64_t b) { return (a.m + b - 1) / b * ((a.n + b - 1) / b); };
     if (tiles(256) >= 128) return launch_tile<T, 2, 4, 8, 4>(a, s);
     if (tiles(128) >= 128) return launch_tile<T, 2, 2, 4, 4>(a, s);

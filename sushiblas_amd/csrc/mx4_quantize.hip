@@ -13,42 +13,40 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// The code of a block whose largest magnitude has these bits (an integer
-// comparison orders magnitudes, NaN last).
+// The code of a block whose largest magnitude has these bits.
 __device__ inline uint32_t block_code(uint32_t top)
 {
     const uint32_t e = top >> 23;
-    return e >= 255 ? 255u : e > 2 ? e - 2 : 0u;
+    return e == 255 ? 255u : __builtin_elementwise_sub_sat(e, 2u);
 }
 
-// The same from bits that other lanes hold too (DPP: lane ^ 1 and ^ 2; lane ^ 8 of 16).
+// The larger magnitude, NaN if there is one.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(fabsf(a), fabsf(b)); }
+
+// The larger bits (magnitudes are in integer order, NaN last) of two lanes.
 template <int CTRL>
-__device__ inline uint32_t max_dpp(uint32_t x)
+__device__ inline uint32_t max_dpp(uint32_t x, uint32_t other)
 {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
-    return x > y ? x : y;
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)other, CTRL, 0xf, 0xf, true));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor8 = 0x128;
-
-__device__ inline uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor8 = 0x128;  // DPP: lane ^ 1, ^ 2, ^ 8 of 16
 
 // The scale a conversion takes: its exponent field is what counts (0: 2^-127).
 __device__ inline float scale_of(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
 
-constexpr int RPT = 4, ROWS = 8 * RPT;  // rows of a lane, of a workgroup
-
-// Eight values of a row, from memory that is aligned to the element only.
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-    T v[8];
-};
+constexpr int RPT = 4;     // rows of a lane
+constexpr int TILE = 128;  // rows and columns of a workgroup
 
 // The lane's rows of 8 values; past an edge, values from the nearest place inside.
 template <typename T>
 __device__ inline void load_rows(Eight<T> (&x)[RPT], const void* X, int64_t ld, int64_t r0, int64_t c0,
-                                 bool whole, const DropoutArgs& a)
+                                 bool inside, bool whole, const DropoutArgs& a)
 {
-    if (whole) {  // (the wave's 64 columns are inside)
+    if (inside) {
+        const T* from = (const T*)X + r0 * ld + c0;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) x[i] = *(const Eight<T>*)(from + i * ld);
+    } else if (whole) {  // (the wave's 64 columns are inside)
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             const int64_t r = r0 + i < a.rows ? r0 + i : a.rows - 1;
@@ -66,28 +64,32 @@ __device__ inline void load_rows(Eight<T> (&x)[RPT], const void* X, int64_t ld, 
     }
 }
 
-// A workgroup takes 32 rows by 256 columns, a lane 4 rows (RPT) by 8 columns: its loads are
-// 16 bytes of 16-bit values, and its 8 columns of a row one call of the generator.  A row's
-// block lies in 4 neighbouring lanes, a column's in 8 lanes 8 apart, so one pass over X makes
-// both forms in registers.  What leaves in small pieces (4 bytes of P, 2 of PT a lane) the L2
-// gathers into lines.  MASKED: with dropout or a gate.
-//   Bound by HBM where X is large: 8192^2 bf16, both forms, 35.5 us for 205 MB (5.8 TB/s);
-// 8 or 16 rows a lane store larger pieces but leave fewer waves (34.9 and 37.0 us; with
-// dropout and gate 73.0, 73.2 and 112 us).
+// A workgroup takes 128 by 128 values, a wave 32 rows by 64 columns, a lane 4 rows (RPT) by 8
+// columns: its loads are 16 bytes of 16-bit values, and its 8 columns of a row one call of the
+// generator.  A row's block lies in 4 neighbouring lanes, a column's in 8 lanes 8 apart, so one
+// pass over X makes both forms in registers.  They are gathered in LDS and leave 64 bytes of a
+// row at a time, past the L2s.  MASKED: with dropout or a gate.
+//   Bound by HBM: 8192^2 bf16 37.4 us to both forms (205 MB, 5.5 TB/s), 27.1 to the rows' alone
+// (170 MB, 6.3 TB/s); stored through the L2s 45.9 and 33.7 us, straight from the lanes (4 bytes of
+// P, 2 of PT each: the L2s take as long for a request of 16 bytes as for one of 64) 53.2 and 34.8.
+// With dropout and gate 57.3 us, the generator's and the selects' VALU work beside.
 template <typename T, bool MASKED>
-__global__ void __launch_bounds__(256) quantize_kernel(DropoutArgs a, Mx4Out ro, Mx4Out co, int col_tiles)
+__global__ void __launch_bounds__(512) quantize_kernel(DropoutArgs a, Mx4Out ro, Mx4Out co, int col_tiles)
 {
-    __shared__ __align__(8) uint8_t row_codes[ROWS][8];
-    __shared__ uint8_t col_codes[256];
+    constexpr int PITCH_P = 72, PITCH_PT = 68;  // (no bank is met twice by a wave's writes)
+    __shared__ uint32_t row_codes[TILE], col_codes[TILE];
+    __shared__ __align__(8) uint8_t row_elems[TILE * PITCH_P];
+    __shared__ __align__(4) uint8_t col_elems[TILE * PITCH_PT];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int64_t tile_r = (int64_t)(blockIdx.x / col_tiles) * ROWS, tile_c = (int64_t)(blockIdx.x % col_tiles) * 256;
-    const int64_t r0 = tile_r + lane / 8 * RPT, c0 = tile_c + wave * 64 + lane % 8 * 8;
-    const int64_t nb_r = (a.cols + 31) / 32, nb_c = (a.rows + 31) / 32;  // blocks of a row, of a column
+    const int64_t tile_r = (int64_t)(blockIdx.x / col_tiles) * TILE, tile_c = (int64_t)(blockIdx.x % col_tiles) * TILE;
+    const int rl = wave / 2 * 32 + lane / 8 * RPT, cl = wave % 2 * 64 + lane % 8 * 8;  // in the tile
+    const int64_t r0 = tile_r + rl, c0 = tile_c + cl;
 
     Eight<T> x[RPT], g[RPT];
-    const bool whole = tile_c + wave * 64 + 64 <= a.cols;
-    load_rows<T>(x, a.X, a.ldx, r0, c0, whole, a);
-    if (MASKED && a.gate) load_rows<T>(g, a.gate, a.ldg, r0, c0, whole, a);
+    const bool inside = tile_r + TILE <= a.rows && tile_c + TILE <= a.cols;
+    const bool whole = tile_c + wave % 2 * 64 + 64 <= a.cols;
+    load_rows<T>(x, a.X, a.ldx, r0, c0, inside, whole, a);
+    if (MASKED && a.gate) load_rows<T>(g, a.gate, a.ldg, r0, c0, inside, whole, a);
     uint32_t keep[RPT][4];  // (made while the loads are on their way)
     if (MASKED && a.threshold) {
 #pragma unroll
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(DropoutArgs a, Mx4Out ro,
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = (float)g[i].v[e] > 0.0f ? v[i][e] : 0.0f;
     }
-    if (tile_r + ROWS > a.rows || tile_c + 256 > a.cols) {  // zeros outside
+    if (!inside) {  // zeros outside
 #pragma unroll
         for (int i = 0; i < RPT; ++i)
 #pragma unroll
@@ -121,47 +123,77 @@ __global__ void __launch_bounds__(256) quantize_kernel(DropoutArgs a, Mx4Out ro,
     if (ro.P) {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[i][e]));
-            const uint32_t code = block_code(max_dpp<kXor2>(max_dpp<kXor1>(top)));
+            const float top = larger(larger(larger(v[i][0], v[i][1]), larger(v[i][2], v[i][3])),
+                                     larger(larger(v[i][4], v[i][5]), larger(v[i][6], v[i][7])));
+            uint32_t bits = __builtin_bit_cast(uint32_t, top);
+            bits = max_dpp<kXor1>(bits, bits);
+            bits = max_dpp<kXor2>(bits, bits);
+            const uint32_t code = block_code(bits);
             const float scale = scale_of(code);
             uint32_t w = 0;
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][0], v[i][1], scale, 0);
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][2], v[i][3], scale, 1);
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][4], v[i][5], scale, 2);
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][6], v[i][7], scale, 3);
-            if (code == 255) w = 0;
-            if (r0 + i < a.rows && c0 < 32 * nb_r) *(uint32_t*)(ro.P + (r0 + i) * ro.ldp + c0 / 2) = w;
-            if (lane % 4 == 0) row_codes[lane / 8 * RPT + i][wave * 2 + lane % 8 / 4] = (uint8_t)code;
+            w = code == 255 ? 0 : w;
+            *(uint32_t*)(row_elems + (rl + i) * PITCH_P + cl / 2) = w;
+            ((uint8_t*)(row_codes + rl + i))[cl / 32] = (uint8_t)code;  // (by four lanes)
         }
     }
     if (co.P) {
+        // The columns' largest: 8 of 4 rows in each lane; lanes 32, 16 and 8 apart trade halves
+        // of theirs until each has one column's of all 32 rows.
+        uint32_t t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            t[e] = __builtin_bit_cast(uint32_t, larger(larger(v[0][e], v[1][e]), larger(v[2][e], v[3][e])));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const auto x = __builtin_amdgcn_permlane32_swap(t[e], t[e + 4], false, false);
+            t[e] = max(x[0], x[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const auto x = __builtin_amdgcn_permlane16_swap(t[e], t[e + 2], false, false);
+            t[e] = max(x[0], x[1]);
+        }
+        const bool odd = lane & 8;
+        // byte wave / 2 of a column's word, 8 columns of this lane
+        uint32_t* codes = col_codes + cl;
+        ((uint8_t*)(codes + lane / 8))[wave / 2] =
+            (uint8_t)block_code(max_dpp<kXor8>(odd ? t[1] : t[0], odd ? t[0] : t[1]));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < RPT; ++i) top = max(top, magnitude(v[i][e]));
-            top = max_dpp<kXor8>(top);
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const uint32_t code = block_code(top);
-            const float scale = scale_of(code);
+            const uint32_t c = ((const uint8_t*)(codes + e))[wave / 2];
             uint32_t w = 0;
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0][e], v[1][e], scale, 0);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2][e], v[3][e], scale, 1);
-            if (c0 + e < a.cols && r0 < 32 * nb_c)
-                *(uint16_t*)(co.P + (c0 + e) * co.ldp + r0 / 2) = (uint16_t)(code == 255 ? 0 : w);
-            if (lane < 8) col_codes[wave * 64 + lane * 8 + e] = (uint8_t)code;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0][e], v[1][e], scale_of(c), 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2][e], v[3][e], scale_of(c), 1);
+            *(uint16_t*)(col_elems + (cl + e) * PITCH_PT + rl / 2) = (uint16_t)(c == 255 ? 0 : w);
         }
     }
     __syncthreads();
-    // 8 codes of a row, one of a column; those past the last block are 0, and so are all of a
-    // tile past the last row, there to complete a column's group
-    if (ro.P && threadIdx.x < ROWS && tile_r + threadIdx.x < a.rows)
-        *(uint2*)(ro.S + tile_c / 256 * ro.lds + (tile_r + threadIdx.x) * 8) = *(const uint2*)row_codes[threadIdx.x];
-    if (co.P && tile_c + threadIdx.x < a.cols)
-        co.S[tile_r / 256 * co.lds + (tile_c + threadIdx.x) * 8 + tile_r / 32 % 8] = col_codes[threadIdx.x];
+    // Codes past the last block are 0, and so are all of a tile past the last row or column, there
+    // to complete a group of 8.
+    const int t = threadIdx.x;
+    if (ro.P) {
+        const int64_t row = tile_r + t / 4, c = tile_c + t % 4 * 32;
+        if (row < a.rows && c < a.cols) {
+            const uint2* w = (const uint2*)(row_elems + t / 4 * PITCH_P + t % 4 * 16);
+            __builtin_nontemporal_store(u32x4{w[0].x, w[0].y, w[1].x, w[1].y}, (u32x4*)(ro.P + row * ro.ldp + c / 2));
+        }
+        if (t < TILE && tile_r + t < a.rows)
+            *(uint32_t*)(ro.S + tile_c / 256 * ro.lds + (tile_r + t) * 8 + tile_c / 32 % 8) = row_codes[t];
+    }
+    if (co.P) {
+        const int64_t col = tile_c + t / 4, r = tile_r + t % 4 * 32;
+        if (col < a.cols && r < a.rows) {
+            const uint32_t* w = (const uint32_t*)(col_elems + t / 4 * PITCH_PT + t % 4 * 16);
+            __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, (u32x4*)(co.P + col * co.ldp + r / 2));
+        }
+        if (t < TILE && tile_c + t < a.cols)
+            *(uint32_t*)(co.S + tile_r / 256 * co.lds + (tile_c + t) * 8 + tile_r / 32 % 8) = col_codes[t];
+    }
 }
 
 // Threads form TX chunks of 8 columns by 256 / TX rows, kRows times.
@@ -197,7 +229,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t c
         for (int e = 0; e < 8; ++e) y.v[e] = (T)(code[i] == 255 ? __builtin_nanf("") : v[e / 2][e % 2]);
         T* to = Y + r * ldy + c0;
         if (c0 + 8 <= cols)
-            *(Eight<T>*)to = y;
+            store_past(to, y);
         else
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -208,14 +240,14 @@ __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t c
 template <typename T>
 hipError_t quantize(const DropoutArgs& a, const Mx4Out& rows, const Mx4Out& cols, hipStream_t s)
 {
-    // whole groups of 256 rows where the columns' codes are wanted: each is written to its end
-    const int64_t r = cols.P ? (a.rows + 255) / 256 * 256 : a.rows;
-    const int64_t rt = (r + ROWS - 1) / ROWS, ct = (a.cols + 255) / 256;
+    // whole groups of 8 blocks along a form's axis: their codes are written to the end
+    const int64_t rt = cols.P ? (a.rows + 255) / 256 * 2 : (a.rows + TILE - 1) / TILE;
+    const int64_t ct = rows.P ? (a.cols + 255) / 256 * 2 : (a.cols + TILE - 1) / TILE;
     if (rt * ct > 0x7fffffff) return hipErrorInvalidValue;
     if (a.threshold || a.gate)
-        quantize_kernel<T, true><<<(unsigned)(rt * ct), 256, 0, s>>>(a, rows, cols, (int)ct);
+        quantize_kernel<T, true><<<(unsigned)(rt * ct), 512, 0, s>>>(a, rows, cols, (int)ct);
     else
-        quantize_kernel<T, false><<<(unsigned)(rt * ct), 256, 0, s>>>(a, rows, cols, (int)ct);
+        quantize_kernel<T, false><<<(unsigned)(rt * ct), 512, 0, s>>>(a, rows, cols, (int)ct);
     return hipGetLastError();
 }
 
