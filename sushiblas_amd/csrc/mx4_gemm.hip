@@ -135,8 +135,8 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
 // t + 2, and sees t + 1 arrived, asked for a whole stage's time before.
 //   B's block j holds the tile's rows 32 (j / 2) + 4 (j % 2) + 8 (i / 4) + i % 4 at
 // its index i, so that a lane's results of blocks j, j + 1 are 8 neighbouring columns.
-template <typename T, int WM, int WN, int MB, int NB>
-__global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
+template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
+__global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
 {
     constexpr int WAVES = WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN;
     constexpr int CA = BM * 8 < 1024 ? 1024 : BM * 8, CB = BN * 8 < 1024 ? 1024 : BN * 8;  // codes
@@ -147,11 +147,12 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
     static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && NC <= WAVES && (LA + LB) % MB == 0,
                   "whole wave-wide loads");
     static_assert(MB >= NB && NB % 2 == 0, "");
-    __shared__ __align__(16) char lds[2 * STAGE];
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    __shared__ __align__(16) char lds_all[KG * NS * STAGE];
+    const int lane = threadIdx.x % 64, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kg = wave_all / WAVES, wave = wave_all % WAVES;  // group, and wave of the group
     const int r = lane % 16, q = lane / 16;
+    char* lds = lds_all + kg * NS * STAGE;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds_all + kg * NS * STAGE;
     // Neighbouring tiles to one XCD (workgroups are dealt to the 8 in turn), in columns of 8
     // tiles of rows: the XCD's tiles of one time share both operands in its L2.
     int id = blockIdx.x;
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
     const int group = 8 * tiles_n, g0 = id / group * 8;
     const int gh = tiles_m - g0 < 8 ? tiles_m - g0 : 8;
     const int m0 = (g0 + id % group % gh) * BM, n0 = id % group / gh * BN;
-    const int nb = (p.k + 31) / 32, nk = (nb + 7) / 8;
+    const int nb = (p.k + 31) / 32, nk = (nb + 8 * KG - 1) / (8 * KG);  // stages of a group
 
     const int rows_a = p.m - m0 < BM ? p.m - m0 : BM, rows_b = p.n - n0 < BN ? p.n - n0 : BN;
     i32x4 da = descriptor(p.A + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + 16 * nb);
@@ -189,31 +190,33 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
     const int code_left = (code_b ? rows_b : rows_a) - code_row;
     const uint8_t* code_at = code_b ? p.SB + 8 * (int64_t)(n0 + code_row) : p.SA + 8 * (int64_t)(m0 + code_row);
     const int64_t code_step = code_b ? p.ldsb : p.ldsa;
+    code_at += kg * code_step;
 
     // Load x < LA + LB of stage t; the codes go with the last.  Blocks past the last one,
     // and all of a stage past the last, are zeros, whatever lies there.
     auto load_part = [&](int t, int x) {
-        const uint32_t at = lds0 + (t & 1) * STAGE;
-        const int left = nb - 8 * t;
+        const uint32_t at = lds0 + t % NS * STAGE;
+        const int tk = t * KG + kg, left = nb - 8 * tk;
         if (x < LA)
-            load_lds(at + (wave * LA + x) * 1024, ca[x % LA] < left ? va[x % LA] : kOutside, da, t * 128);
+            load_lds(at + (wave * LA + x) * 1024, ca[x % LA] < left ? va[x % LA] : kOutside, da, tk * 128);
         else
             load_lds(at + OFF_B + (wave * LB + x - LA) * 1024, cb[(x - LA) % LB] < left ? vb[(x - LA) % LB] : kOutside,
-                     db, t * 128);
+                     db, tk * 128);
         if (x == LA + LB - 1 && wave < NC) {
             const uint64_t s = (uint64_t)code_at;
             const int n = left <= 0 || code_left <= 0 ? 0 : code_left > 128 ? 1024 : 8 * code_left;
             load_lds(at + OFF_SA + wave * 1024, lane * 16,
                      i32x4{(int)(uint32_t)s, (int)(uint32_t)(s >> 32) & 0xffff, n, kRsrcWord3}, 0);
-            code_at += code_step;
+            code_at += KG * code_step;
         }
     };
     // Codes past the last block may be NaN's: the last stage's are cleared.
     auto clear_codes = [&](int t) {
         if (t == nk - 1 && nb % 8) {
             const uint64_t mask = (1ull << nb % 8 * 8) - 1;
-            for (int i = threadIdx.x; i < (CA + CB) / 8; i += 64 * WAVES)
-                ((uint64_t*)(lds + (t & 1) * STAGE + OFF_SA))[i] &= mask;
+            if (nb / 8 == t * KG + kg)
+                for (int i = threadIdx.x % (64 * WAVES); i < (CA + CB) / 8; i += 64 * WAVES)
+                    ((uint64_t*)(lds + t % NS * STAGE + OFF_SA))[i] &= mask;
             __syncthreads();
         }
     };
@@ -302,8 +305,8 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
         // (a descriptor that vector instructions wrote may be read 5 instructions later)
         asm volatile("s_nop 4" : "+s"(da), "+s"(db));
 #pragma unroll
-        for (int x = 0; x < 2 * (LA + LB); ++x) load_part(x / (LA + LB), x % (LA + LB));
-        wait_loads_and_barrier<LA + LB>();  // (the waves that load codes wait for one more)
+        for (int x = 0; x < NS * (LA + LB); ++x) load_part(x / (LA + LB), x % (LA + LB));
+        wait_loads_and_barrier<(NS - 1) * (LA + LB)>();  // (the waves that load codes wait for more)
         clear_codes(0);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
@@ -324,40 +327,59 @@ __global__ void __launch_bounds__(64 * WM * WN, MB * NB > 32 ? 1 : 2) mx4_gemm_k
         }
         asm volatile("s_nop 1");
         for (int t = 0; t < nk; ++t) {
-            multiply(first, lds + (t & 1) * STAGE, [](int) {});
+            multiply(first, lds + t % NS * STAGE, [](int) {});
             // (after the last stage: what lies there)
-            multiply(second, lds + ((t + 1) & 1) * STAGE, [&](int i) {
+            multiply(second, lds + (t + 1) % NS * STAGE, [&](int i) {
                 if (i == 0) {
-                    wait_loads_and_barrier<0>();
+                    wait_loads_and_barrier<(NS - 2) * (LA + LB)>();
                     clear_codes(t + 1);
                 }
                 // spread over the passes: a wave that asks for all of them at once waits its
                 // turn at the CU's one load unit instead of multiplying
 #pragma unroll
-                for (int x = 0; x < (LA + LB) / MB; ++x) load_part(t + 2, i * ((LA + LB) / MB) + x);
+                for (int x = 0; x < (LA + LB) / MB; ++x) load_part(t + NS, i * ((LA + LB) / MB) + x);
             });
         }
         wait_loads_and_barrier<0>();  // nothing more is written to LDS
     }
     settle(acc);
 
+    // The groups' sums: each takes over half of the rows, and gives the others'.
+    constexpr int MINE = MB / KG;
+    if constexpr (KG == 2) {
+        f32x4* trade = (f32x4*)lds_all;
+        static_assert(WAVES * MB * NB * 64 * 16 <= KG * NS * STAGE, "");
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                trade[((kg * WAVES + wave) * MINE + i) * NB * 64 + j * 64 + lane] = kg ? acc[i][j] : acc[MINE + i][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                acc[i][j] = (kg ? acc[MINE + i][j] : acc[i][j]) +
+                            trade[(((1 - kg) * WAVES + wave) * MINE + i) * NB * 64 + j * 64 + lane];
+        __syncthreads();
+    }
     // Out through LDS, 16 rows of the wave's at a time, so that an instruction stores whole
     // rows of them (from the registers it would store 32 columns of 16 rows).
     constexpr int V = 16 / sizeof(T), COLS = 16 * NB, PITCH = COLS + 4;
     constexpr int PER_ROW = COLS / V, ROWS = 64 / PER_ROW;  // lanes per row, rows per instruction
-    static_assert(2 * 16 * PITCH * 4 * WAVES <= 2 * STAGE, "");
-    float* out = (float*)lds + wave * 2 * 16 * PITCH;
+    static_assert(2 * 16 * PITCH * 4 * WAVES <= NS * STAGE, "");
+    float* out = (float*)lds_all + wave_all * 2 * 16 * PITCH;
     const int n = n0 + wn + lane % PER_ROW * V;
     T* C = (T*)p.C + n;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
+    for (int i = 0; i < MINE; ++i) {
         float* half = out + i % 2 * 16 * PITCH;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
             *(f32x4*)(half + r * PITCH + j / 2 * 32 + 8 * q + j % 2 * 4) = acc[i][j];
 #pragma unroll
         for (int x = 0; x < 16; x += ROWS) {
-            const int row = x + lane / PER_ROW, m = m0 + wm + 16 * i + row;
+            const int row = x + lane / PER_ROW, m = m0 + wm + 16 * (kg * MINE + i) + row;
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = half[row * PITCH + lane % PER_ROW * V + e];
@@ -381,10 +403,9 @@ struct Group {
 
 // The rows of an operand that a workgroup takes, and the lane's place in them.
 struct Strip {
-    __amdgpu_buffer_rsrc_t rows;
-    const uint8_t* codes;
+    const uint8_t *rows, *codes;
     int64_t lds;
-    int count, ld, at, code_at;
+    int bytes, count, ld, at, code_at;
 
     __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n,
                                 int most, int nb, int lane)
@@ -392,43 +413,47 @@ struct Strip {
         count = min(n - first, most);
         ld = (int)ld_;
         lds = lds_;
-        rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P) + first * ld_, (short)0,
-                                                 (count - 1) * ld + 16 * nb, kRsrcWord3);
+        rows = P + first * ld_;
+        bytes = (count - 1) * ld + 16 * nb;
         codes = S + 8 * (int64_t)first;
         at = lane % 16 * ld + lane / 16 * 32;
         code_at = lane % 16 * 8 + lane / 16 * 2;
     }
 
-    // Group g (256 terms) of N times 16 rows, zeros past the last row.  blocks: of the lane's
-    // two, those inside (what lies past the last block is not used).
+    // Group g (256 terms) of N times 16 rows; zeros, not from memory, past the last row and past
+    // the last group (left <= 0 blocks).
     template <int N>
-    __device__ inline void load(Group<N>& d, int g, bool tail, int blocks) const
+    __device__ inline void load(Group<N>& d, int g, int left) const
     {
+        const __amdgpu_buffer_rsrc_t v = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(rows), (short)0,
+                                                                           left > 0 ? bytes : 0, kRsrcWord3);
         const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(codes) + g * lds, (short)0, 8 * count, kRsrcWord3);
+            const_cast<uint8_t*>(codes) + g * lds, (short)0, left > 0 ? 8 * count : 0, kRsrcWord3);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int from = 16 * i * ld + g * 128;
-            d.v[i][0] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, from, 0));
-            d.v[i][1] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 16, from, 0));
+            d.v[i][0] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at, from, 0));
+            d.v[i][1] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at + 16, from, 0));
             d.code[i] = __builtin_amdgcn_raw_buffer_load_b16(c, code_at + 128 * i, 0, 0);
-        }
-        if (tail) {
-            const i32x4 zero = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                d.v[i][0] = blocks >= 1 ? d.v[i][0] : zero;
-                d.v[i][1] = blocks >= 2 ? d.v[i][1] : zero;
-                d.code[i] = blocks >= 2 ? d.code[i] : blocks == 1 ? d.code[i] & 0xff : 0;
-            }
         }
     }
 };
 
-// AHEAD: the next group's loads are under way while one is multiplied (or else the SIMD's other
-// wave's are).
-template <typename T, int YB, int XB, bool AHEAD, bool XA>
-__global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 8 ? 2 : 4) mx4_skinny_kernel(Mx4GemmArgs p)
+// What lies past the last block is not used: `mine` of the lane's two blocks are inside.
+template <int N>
+__device__ inline void clip(Group<N>& d, int mine)
+{
+    const i32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        d.v[i][0] = mine >= 1 ? d.v[i][0] : zero;
+        d.v[i][1] = mine >= 2 ? d.v[i][1] : zero;
+        d.code[i] = mine >= 2 ? d.code[i] : mine == 1 ? d.code[i] & 0xff : 0;
+    }
+}
+
+template <typename T, int YB, int XB, bool XA>
+__global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 4 ? 2 : 4) mx4_skinny_kernel(Mx4GemmArgs p)
 {
     const int nx = XA ? p.m : p.n, ny = XA ? p.n : p.m;
     constexpr int PITCH = 16 * YB + 4;
@@ -436,22 +461,23 @@ __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 8 ? 2 : 4) mx4_s
 
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r = lane % 16, q = lane / 16;
-    const int x0 = blockIdx.x * (16 * XB);
+    const int x0 = blockIdx.x * (16 * XB), y0 = blockIdx.y * (16 * YB);
     const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
     Strip sx, sy;
     sx.init(XA ? p.A : p.B, XA ? p.lda : p.ldb, XA ? p.SA : p.SB, XA ? p.ldsa : p.ldsb, x0, nx, 16 * XB, nb, lane);
-    sy.init(XA ? p.B : p.A, XA ? p.ldb : p.lda, XA ? p.SB : p.SA, XA ? p.ldsb : p.ldsa, 0, ny, 16 * YB, nb, lane);
+    sy.init(XA ? p.B : p.A, XA ? p.ldb : p.lda, XA ? p.SB : p.SA, XA ? p.ldsb : p.ldsa, y0, ny, 16 * YB, nb, lane);
 
     f32x4 acc[XB][YB] = {};
-    Group<XB> x;
-    Group<YB> y;
     auto load = [&](Group<XB>& x, Group<YB>& y, int g) {
-        const bool tail = 8 * g + 8 > nb;
-        const int blocks = nb - 8 * g - 2 * q;
-        sx.load(x, g, tail, blocks);
-        sy.load(y, g, tail, blocks);
+        sx.load(x, g, nb - 8 * g);
+        sy.load(y, g, nb - 8 * g);
     };
-    auto multiply = [&](const Group<XB>& x, const Group<YB>& y) {
+    auto multiply = [&](Group<XB>& x, Group<YB>& y, int g) {
+        const int left = nb - 8 * g;
+        if (left < 8) {
+            clip(x, left - 2 * q);
+            clip(y, left - 2 * q);
+        }
 #pragma unroll
         for (int i = 0; i < XB; ++i)
 #pragma unroll
@@ -462,22 +488,16 @@ __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 8 ? 2 : 4) mx4_s
                     widen(x.v[i][1]), widen(y.v[j][1]), acc[i][j], 4, 4, 1, x.code[i], 1, y.code[j]);
             }
     };
-    if constexpr (AHEAD) {
-        Group<XB> xn;
-        Group<YB> yn;
-        if (wave < groups) load(x, y, wave);
-        for (int g = wave; g < groups; g += 2 * kSkinnyWaves) {
-            if (g + kSkinnyWaves < groups) load(xn, yn, g + kSkinnyWaves);
-            multiply(x, y);
-            if (g + kSkinnyWaves >= groups) break;
-            if (g + 2 * kSkinnyWaves < groups) load(x, y, g + 2 * kSkinnyWaves);
-            multiply(xn, yn);
-        }
-    } else {
-        for (int g = wave; g < groups; g += kSkinnyWaves) {
-            load(x, y, g);
-            multiply(x, y);
-        }
+    // (no branch around loads, also past the last group: the compiler would wait for all of them)
+    constexpr int W = kSkinnyWaves;
+    Group<XB> x0g, x1g;
+    Group<YB> y0g, y1g;
+    load(x0g, y0g, wave);
+    for (int g = wave; g < groups; g += 2 * W) {
+        load(x1g, y1g, g + W);
+        multiply(x0g, y0g, g);
+        load(x0g, y0g, g + 2 * W);
+        multiply(x1g, y1g, g + W);
     }
     T* C = (T*)p.C;
 #pragma unroll
@@ -491,48 +511,91 @@ __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 8 ? 2 : 4) mx4_s
         for (int t = threadIdx.x; t < 16 * 16 * YB; t += 64 * kSkinnyWaves) {
             const int dx = XA ? t / (16 * YB) : t % 16, dy = XA ? t % (16 * YB) : t / 16;  // C's rows run along n
             const int xr = x0 + 16 * i + dx;
-            if (xr >= nx || dy >= ny) continue;
+            if (xr >= nx || y0 + dy >= ny) continue;
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < kSkinnyWaves; ++w) v += part[w][dx * PITCH + dy];
-            T* c = C + (XA ? (int64_t)xr * p.ldc + dy : (int64_t)dy * p.ldc + xr);
+            T* c = C + (XA ? (int64_t)xr * p.ldc + y0 + dy : (int64_t)(y0 + dy) * p.ldc + xr);
             *c = result<T>(v, p.beta != 0.0f ? (float)*c : 0.0f, p);
         }
     }
 }
 
-template <typename T, int YB, int XB, bool AHEAD>
+template <typename T, int YB, int XB>
 hipError_t launch_skinny(const Mx4GemmArgs& a, hipStream_t s)
 {
+    auto grid = [](int x, int y) {
+        return dim3((unsigned)((x + 16 * XB - 1) / (16 * XB)), (unsigned)((y + 16 * YB - 1) / (16 * YB)));
+    };
     if (a.m <= a.n)
-        mx4_skinny_kernel<T, YB, XB, AHEAD, false><<<(unsigned)((a.n + 16 * XB - 1) / (16 * XB)), 64 * kSkinnyWaves, 0, s>>>(a);
+        mx4_skinny_kernel<T, YB, XB, false><<<grid(a.n, a.m), 64 * kSkinnyWaves, 0, s>>>(a);
     else
-        mx4_skinny_kernel<T, YB, XB, AHEAD, true><<<(unsigned)((a.m + 16 * XB - 1) / (16 * XB)), 64 * kSkinnyWaves, 0, s>>>(a);
+        mx4_skinny_kernel<T, YB, XB, true><<<grid(a.m, a.n), 64 * kSkinnyWaves, 0, s>>>(a);
     return hipGetLastError();
 }
 
-template <typename T, int WM, int WN, int MB, int NB>
+template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
 hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 {
     constexpr int BM = 16 * MB * WM, BN = 16 * NB * WN;
     const int tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
     if ((int64_t)tm * tn > 0x7fffffff) return hipErrorInvalidValue;
-    mx4_gemm_kernel<T, WM, WN, MB, NB><<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, tm, tn);
+    mx4_gemm_kernel<T, WM, WN, KG, MB, NB, NS><<<(unsigned)(tm * tn), 64 * WM * WN * KG, 0, s>>>(a, tm, tn);
     return hipGetLastError();
+}
+
+// The kernels' times, in us, for choosing one: `fixed` and, per `terms` terms, `step` for each
+// round of `per_cu` workgroups on each CU, fitted to the times beside.  (Rates of the tiles: the
+// 256^2 one asks the L2s for half of what 128^2 does, and 128^2 for half of 64^2, and an L2 serves
+// a CU some 60 bytes per ns; what counts for few tiles is a stage's latency, that more stages or
+// groups of waves in flight hide.)
+//                     1024^2 x 8192  4096 x 1024 x 4096  2048 x 4096^2  4096^2 x 1024  4096^3
+//   64^2, 2 groups             12.4                28.2           53.4           62.4   105.2
+//   128^2, 4 stages            20.2                14.2           27.2           25.3    50.7
+//   128^2, 2 per CU            26.4                17.6           22.8           20.6    43.7
+//   256^2                      45.4                28.3           29.5           16.7    36.2
+struct TilePlan {
+    int size, per_cu, terms;
+    double step, fixed;
+};
+constexpr TilePlan kTilePlans[] = {{64, 1, 512, 0.53, 3.4}, {128, 1, 256, 0.58, 5.0}, {128, 2, 256, 1.05, 5.0},
+                                   {256, 1, 256, 1.65, 9.0}};
+constexpr int kCus = 256;
+
+double tile_us(const TilePlan& t, const Mx4GemmArgs& a)
+{
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    const int64_t rounds = up(up(a.m, t.size) * up(a.n, t.size), t.per_cu * kCus);
+    return (double)rounds * (t.fixed + (double)up(a.k, t.terms) * t.step);
 }
 
 template <typename T>
 hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
 {
-    const int narrow = a.m < a.n ? a.m : a.n;
-    if (narrow <= 16) return launch_skinny<T, 1, 1, true>(a, s);
-    if (narrow <= 32) return launch_skinny<T, 2, 1, true>(a, s);
-    if (narrow <= 64) return launch_skinny<T, 4, 2, true>(a, s);
-    if (narrow <= 128) return launch_skinny<T, 8, 2, false>(a, s);
-    auto tiles = [&](int64_t b) { return (a.m + b - 1) / b * ((a.n + b - 1) / b); };
-    if (tiles(256) >= 128) return launch_tile<T, 2, 4, 8, 4>(a, s);
-    if (tiles(128) >= 128) return launch_tile<T, 2, 2, 4, 4>(a, s);
-    return launch_tile<T, 2, 2, 2, 2>(a, s);
+    const int narrow = a.m < a.n ? a.m : a.n, wide = a.m < a.n ? a.n : a.m;
+    // One narrow block: the wide operand at the rate memory gives it.  Two blocks of it a
+    // workgroup where that leaves one for each CU (1 x 8192 x 8192: 9.2 against 9.5 us, 16 rows
+    // 10.3 against 11.7; the 64^2 tile 11.5 and 11.2).
+    if (narrow <= 16 && wide > 16 * kCus) return launch_skinny<T, 1, 2>(a, s);
+    double best = 1e30;
+    int pick = 0;
+    for (int i = 0; i < 4; ++i) {
+        const double t = tile_us(kTilePlans[i], a);
+        if (t < best) {
+            best = t;
+            pick = i;
+        }
+    }
+    // Small results over many terms (256^2 x 8192: 6.6 against 10.9 us on the 64^2 tile, 128 x 1024 x
+    // 8192 10.8 against 10.8): 2048 terms of a block take its waves about 1 us.
+    const double blocks = ((narrow + 15) / 16) * (double)((wide + 15) / 16) / kCus;
+    if (narrow <= 16 || 2.2 + (a.k + 2047) / 2048 * (blocks < 1 ? 1 : blocks) < best) return launch_skinny<T, 1, 1>(a, s);
+    switch (pick) {
+    case 0: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
+    case 1: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
+    case 2: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
+    default: return launch_tile<T, 2, 4, 1, 8, 4, 2>(a, s);
+    }
 }
 
 }  // namespace
