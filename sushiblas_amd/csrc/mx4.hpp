@@ -56,6 +56,7 @@ struct Mx4GemmArgs {
     int m, n, k;
     float alpha, beta;
     int relu;
+    int past;  // C's rows are whole 64-byte lines
 };
 
 // dtype: an sbx_dtype that the caller has checked.

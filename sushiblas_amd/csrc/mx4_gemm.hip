@@ -107,9 +107,14 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
         if (p.beta != 0.0f) in = *(const Vec<T>*)c;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.v[e] = result<T>(acc[e], p.beta != 0.0f ? (float)in.v[e] : 0.0f, p);
-        // (past the L2s, that keep the operands then: 8192^2 x 512 to bf16 60.5 -> 55.1 us, 4096^2 x 1024
-        // 23.4 -> 16.7 us)
-        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), (u32x4*)c);
+        // Rows of whole 64 bytes go past the L2s, that keep the operands then (8192^2 x 512 to bf16
+        // 60.5 -> 55.1 us, 4096^2 x 1024 23.4 -> 16.7 us); of others an L2 has to put the pieces
+        // together (4095 x 3001 x 2047 to fp32 28.7 us, past them 32.8).
+        typedef u32x4 __attribute__((aligned(2))) loose_t;
+        if (p.past)
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), (loose_t*)c);
+        else
+            *(Vec<T>*)c = o;
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)

@@ -68,13 +68,13 @@ __device__ inline void load_rows(Eight<T> (&x)[RPT], const void* X, int64_t ld, 
 // columns: its loads are 16 bytes of 16-bit values, and its 8 columns of a row one call of the
 // generator.  A row's block lies in 4 neighbouring lanes, a column's in 8 lanes 8 apart, so one
 // pass over X makes both forms in registers.  They are gathered in LDS and leave 64 bytes of a
-// row at a time, past the L2s.  MASKED: with dropout or a gate.
+// row at a time, past the L2s.
 //   Bound by HBM: 8192^2 bf16 37.4 us to both forms (205 MB, 5.5 TB/s), 27.1 to the rows' alone
 // (170 MB, 6.3 TB/s); stored through the L2s 45.9 and 33.7 us, straight from the lanes (4 bytes of
 // P, 2 of PT each: the L2s take as long for a request of 16 bytes as for one of 64) 53.2 and 34.8.
 // With dropout and gate 57.3 us, the generator's and the selects' VALU work beside.
-template <typename T, bool MASKED>
-__global__ void __launch_bounds__(512) quantize_kernel(DropoutArgs a, Mx4Out ro, Mx4Out co, int col_tiles)
+template <typename T, bool DROP, bool GATE>
+__global__ void __launch_bounds__(512, 4) quantize_kernel(DropoutArgs a, Mx4Out ro, Mx4Out co, int col_tiles)
 {
     constexpr int PITCH_P = 72, PITCH_PT = 68;  // (no bank is met twice by a wave's writes)
     __shared__ uint32_t row_codes[TILE], col_codes[TILE];
@@ -89,29 +89,19 @@ __global__ void __launch_bounds__(512) quantize_kernel(DropoutArgs a, Mx4Out ro,
     const bool inside = tile_r + TILE <= a.rows && tile_c + TILE <= a.cols;
     const bool whole = tile_c + wave % 2 * 64 + 64 <= a.cols;
     load_rows<T>(x, a.X, a.ldx, r0, c0, inside, whole, a);
-    if (MASKED && a.gate) load_rows<T>(g, a.gate, a.ldg, r0, c0, inside, whole, a);
-    uint32_t keep[RPT][4];  // (made while the loads are on their way)
-    if (MASKED && a.threshold) {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) keep_words(a, (uint32_t)(r0 + i), (uint32_t)(c0 / 8), keep[i]);
-    }
+    if (GATE) load_rows<T>(g, a.gate, a.ldg, r0, c0, inside, whole, a);
     float v[RPT][8];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i)
+    for (int i = 0; i < RPT; ++i) {
+        uint32_t keep[4];
+        if (DROP) keep_words(a, (uint32_t)(r0 + i), (uint32_t)(c0 / 8), keep);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = (float)x[i].v[e];
-    if (MASKED && a.threshold) {
-        const float scale = (float)a.scale;
-#pragma unroll
-        for (int i = 0; i < RPT; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = kept(a, keep[i], e) ? v[i][e] * scale : 0.0f;
-    }
-    if (MASKED && a.gate) {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = (float)g[i].v[e] > 0.0f ? v[i][e] : 0.0f;
+        for (int e = 0; e < 8; ++e) {
+            v[i][e] = (float)x[i].v[e];
+            if (DROP) v[i][e] *= (float)a.scale;
+            if (DROP || GATE)
+                v[i][e] = (!DROP || kept(a, keep, e)) && (!GATE || (float)g[i].v[e] > 0.0f) ? v[i][e] : 0.0f;
+        }
     }
     if (!inside) {  // zeros outside
 #pragma unroll
@@ -244,10 +234,11 @@ hipError_t quantize(const DropoutArgs& a, const Mx4Out& rows, const Mx4Out& cols
     const int64_t rt = cols.P ? (a.rows + 255) / 256 * 2 : (a.rows + TILE - 1) / TILE;
     const int64_t ct = rows.P ? (a.cols + 255) / 256 * 2 : (a.cols + TILE - 1) / TILE;
     if (rt * ct > 0x7fffffff) return hipErrorInvalidValue;
-    if (a.threshold || a.gate)
-        quantize_kernel<T, true><<<(unsigned)(rt * ct), 512, 0, s>>>(a, rows, cols, (int)ct);
-    else
-        quantize_kernel<T, false><<<(unsigned)(rt * ct), 512, 0, s>>>(a, rows, cols, (int)ct);
+    const unsigned grid = (unsigned)(rt * ct);
+    if (a.threshold && a.gate) quantize_kernel<T, true, true><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
+    else if (a.threshold) quantize_kernel<T, true, false><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
+    else if (a.gate) quantize_kernel<T, false, true><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
+    else quantize_kernel<T, false, false><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
     return hipGetLastError();
 }
 
