@@ -221,7 +221,7 @@ int sbx_dsyrk_strided_batched(void* stream, int layout, int upper, int trans, in
  * block whose products run on the 4-bit matrix cores: quantise activations,
  * weights and gradients along the axis that a product sums over, multiply, and
  * drop activations out on their way.  All matrices are row-major; nothing is
- * allocated, except the product's split-K partials, in the stream's workspace. */
+ * allocated and no workspace used. */
 
 /* Dropout, Y = keep ? X / (1 - p) : 0 (rows x cols, F32, F64, BF16 or F16).
  * keep is a function of (seed, stream_id, row, column) alone, by the

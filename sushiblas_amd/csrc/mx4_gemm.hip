@@ -552,18 +552,20 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 // The kernels' times, in us, for choosing one: `fixed` and, per `terms` terms, `step` for each
 // round of `per_cu` workgroups on each CU, fitted to the times beside.  (Rates of the tiles: the
 // 256^2 one asks the L2s for half of what 128^2 does, and 128^2 for half of 64^2, and an L2 serves
-// a CU some 60 bytes per ns; what counts for few tiles is a stage's latency, that more stages or
-// groups of waves in flight hide.)
-//                     1024^2 x 8192  4096 x 1024 x 4096  2048 x 4096^2  4096^2 x 1024  4096^3
-//   64^2, 2 groups             12.4                28.2           53.4           62.4   105.2
-//   128^2, 4 stages            20.2                14.2           27.2           25.3    50.7
-//   128^2, 2 per CU            26.4                17.6           22.8           20.6    43.7
-//   256^2                      45.4                28.3           29.5           16.7    36.2
+// a CU some 60 bytes per ns; what counts for few tiles is a stage's latency, that more stages,
+// groups of waves or workgroups on a CU hide: four of the 64^2 with one group fit on one.)
+//                     512^3  1024^2 x 2048  x 8192  2048^2 x 512  1500^2 x 300  4096 x 1024 x 4096  4096^2 x 1024  4096^3
+//   64^2, 1 group       4.5            7.1    16.2           8.1           6.8                18.4
+//   64^2, 2 groups      5.1            7.1    13.5          16.7          12.8                29.3           62.4   105.2
+//   128^2, 4 stages     6.0            8.4    21.0           7.5           7.7                15.2           25.3    50.7
+//   128^2, 2 per CU     7.1           10.2    26.3           8.3           9.6                17.2           20.6    43.7
+//   256^2                                     45.4                                            28.3           16.7    36.2
 struct TilePlan {
     int size, per_cu, terms;
     double step, fixed;
 };
-constexpr TilePlan kTilePlans[] = {{64, 1, 512, 0.53, 3.4}, {128, 1, 256, 0.58, 5.0}, {128, 2, 256, 1.05, 5.0},
+constexpr TilePlan kTilePlans[] = {{64, 1, 256, 0.39, 3.7},  {64, 2, 256, 0.55, 4.5},  {64, 4, 256, 0.75, 6.6},
+                                   {64, 1, 512, 0.53, 4.8},  {128, 1, 256, 0.56, 5.8}, {128, 2, 256, 1.05, 5.5},
                                    {256, 1, 256, 1.65, 9.0}};
 constexpr int kCus = 256;
 
@@ -584,7 +586,7 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
     if (narrow <= 16 && wide > 16 * kCus) return launch_skinny<T, 1, 2>(a, s);
     double best = 1e30;
     int pick = 0;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 7; ++i) {
         const double t = tile_us(kTilePlans[i], a);
         if (t < best) {
             best = t;
@@ -596,9 +598,12 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
     const double blocks = ((narrow + 15) / 16) * (double)((wide + 15) / 16) / kCus;
     if (narrow <= 16 || 2.2 + (a.k + 2047) / 2048 * (blocks < 1 ? 1 : blocks) < best) return launch_skinny<T, 1, 1>(a, s);
     switch (pick) {
-    case 0: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
-    case 1: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
-    case 2: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
+    case 0:
+    case 1:
+    case 2: return launch_tile<T, 2, 2, 1, 2, 2, 2>(a, s);
+    case 3: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
+    case 4: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
+    case 5: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
     default: return launch_tile<T, 2, 4, 1, 8, 4, 2>(a, s);
     }
 }

@@ -101,6 +101,15 @@ def test_gemm_larger(cuda, m, n, k):
     _run(cuda, "bf16", m, n, k, relu=True)
 
 
+@pytest.mark.parametrize("m,n,k", [(600, 600, 31), (640, 577, 1000), (1025, 1000, 1700), (1500, 1500, 300),
+                                   (450, 500, 6500), (1000, 1000, 4128), (1100, 1150, 2900), (129, 4096, 900),
+                                   (1800, 2040, 1300), (3000, 3100, 200), (65, 65, 65), (4100, 4090, 96)])
+def test_gemm_tiles(cuda, m, n, k):
+    """Few and many tiles of every kind, with terms that end inside a stage."""
+    _run(cuda, "f16", m, n, k, beta=1.0)
+    _run(cuda, "f32", m, n, k, layout=1)
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("layout", [0, 1])
 @pytest.mark.parametrize("alpha,beta,relu", [(1.5, 0.0, False), (1.0, 1.0, False), (-0.5, 0.5, True),
