@@ -123,7 +123,7 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
 }
 
 // Tile of BM x BN = (16 MB WM) x (16 NB WN) of C by WM x WN waves of 16 MB x 16 NB,
-// 256 terms at a time through two LDS stages.
+// 256 terms at a time through NS LDS stages; KG groups of such waves share the terms.
 //
 // A stage holds the tile's rows of 128 bytes (8 blocks, a cache line) and their 8 codes.
 // It is filled by loads that go straight to LDS, which place lanes' 16 bytes one after
@@ -138,20 +138,22 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
 // place once the pass over it is done, B's blocks into a second set.  Between the
 // halves of stage t every wave has read all of it: a barrier there frees its place for
 // t + 2, and sees t + 1 arrived, asked for a whole stage's time before.
-//   B's block j holds the tile's rows 32 (j / 2) + 4 (j % 2) + 8 (i / 4) + i % 4 at
-// its index i, so that a lane's results of blocks j, j + 1 are 8 neighbouring columns.
+//   B's block j holds the tile's rows 16 G (j / G) + 4 (j % G) + 4 G (i / 4) + i % 4 at
+// its index i (G: 2, or all 3 blocks), so that a lane's results of G blocks are 4 G
+// neighbouring columns.
 template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
 __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
 {
     constexpr int WAVES = WM * WN, BM = 16 * MB * WM, BN = 16 * NB * WN;
-    constexpr int CA = BM * 8 < 1024 ? 1024 : BM * 8, CB = BN * 8 < 1024 ? 1024 : BN * 8;  // codes
+    constexpr int CA = (BM + 127) / 128 * 1024, CB = (BN + 127) / 128 * 1024;  // codes
     constexpr int OFF_B = BM * 128, OFF_SA = OFF_B + BN * 128, OFF_SB = OFF_SA + CA;
     constexpr int STAGE = OFF_SB + CB;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // loads per wave and stage
     constexpr int NCA = CA / 1024, NC = NCA + CB / 1024;     // of codes, one by each of the first waves
-    static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && NC <= WAVES && (LA + LB) % MB == 0,
-                  "whole wave-wide loads");
-    static_assert(MB >= NB && NB % 2 == 0, "");
+    constexpr int PER_PASS = (LA + LB + MB - 1) / MB;
+    static_assert(LA * 8 * WAVES == BM && LB * 8 * WAVES == BN && NC <= WAVES, "whole wave-wide loads");
+    static_assert(MB >= NB && (NB % 2 == 0 || NB == 3), "");
+    constexpr int GB = NB % 2 ? NB : 2;  // blocks of B that interleave
     __shared__ __align__(16) char lds_all[KG * NS * STAGE];
     const int lane = threadIdx.x % 64, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kg = wave_all / WAVES, wave = wave_all % WAVES;  // group, and wave of the group
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     // what this lane loads: 16 bytes of a row (rows past the operand's end lie past the
     // descriptor's); the swizzles of rows 8 apart are alike or two
     auto swz_a = [](int x) { return (x >> 1 & 1) ^ (x & 8 ? 6 : 0); };
-    auto swz_b = [](int x) { return (x >> 1 & 1) ^ (x & 16 ? 6 : 0); };
+    auto swz_b = [](int x) { return (x >> 1 & 1) ^ (x % (16 * GB) >= 8 * GB ? 6 : 0); };
     int va[LA], vb[LB], ca[LA], cb[LB];
 #pragma unroll
     for (int j = 0; j < LA; ++j) {
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     i32x4 fa[MB], fb[2][NB];
     int sa[MB], sb[NB], sb_next[NB];
     const int wm = wave % WM * (16 * MB), wn = wave / WM * (16 * NB);
-    const int rb = r / 4 * 8 + r % 4;
+    const int rb = r / 4 * (4 * GB) + r % 4;
     int at_a[2], at_b[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -242,11 +244,11 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     };
     auto read_b = [&](auto half, int j, const char* at) {
         constexpr int H = decltype(half)::value;
-        fb[H][j] = *(const i32x4*)(at + at_b[H] + j / 2 * 4096 + j % 2 * 512);
+        fb[H][j] = *(const i32x4*)(at + at_b[H] + j / GB * (GB * 2048) + j % GB * 512);
     };
     auto read_sa = [&](int i, const char* at) { sa[i] = *(const uint16_t*)(at + at_sa + i * 128); };
     auto read_sb = [&](int j, const char* at) {
-        sb_next[j] = *(const uint16_t*)(at + at_sb + j / 2 * 256 + j % 2 * 32);
+        sb_next[j] = *(const uint16_t*)(at + at_sb + j / GB * (GB * 128) + j % GB * 32);
     };
     // Codes as whole registers: without this the compiler widens them at their use, too
     // near before it (see mma).
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
                 // spread over the passes: a wave that asks for all of them at once waits its
                 // turn at the CU's one load unit instead of multiplying
 #pragma unroll
-                for (int x = 0; x < (LA + LB) / MB; ++x) load_part(t + NS, i * ((LA + LB) / MB) + x);
+                for (int x = i * PER_PASS; x < (i + 1) * PER_PASS && x < LA + LB; ++x) load_part(t + NS, x);
             });
         }
         wait_loads_and_barrier<0>();  // nothing more is written to LDS
@@ -371,24 +373,25 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     // Out through LDS, 16 rows of the wave's at a time, so that an instruction stores whole
     // rows of them (from the registers it would store 32 columns of 16 rows).
     constexpr int V = 16 / sizeof(T), COLS = 16 * NB, PITCH = COLS + 4;
-    constexpr int PER_ROW = COLS / V, ROWS = 64 / PER_ROW;  // lanes per row, rows per instruction
+    constexpr int PER_ROW = COLS / V, PIECES = 16 * PER_ROW;
     static_assert(2 * 16 * PITCH * 4 * WAVES <= NS * STAGE, "");
     float* out = (float*)lds_all + wave_all * 2 * 16 * PITCH;
-    const int n = n0 + wn + lane % PER_ROW * V;
-    T* C = (T*)p.C + n;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
         float* half = out + i % 2 * 16 * PITCH;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            *(f32x4*)(half + r * PITCH + j / 2 * 32 + 8 * q + j % 2 * 4) = acc[i][j];
+            *(f32x4*)(half + r * PITCH + j / GB * (16 * GB) + 4 * GB * q + j % GB * 4) = acc[i][j];
 #pragma unroll
-        for (int x = 0; x < 16; x += ROWS) {
-            const int row = x + lane / PER_ROW, m = m0 + wm + 16 * (kg * MINE + i) + row;
+        for (int x = 0; x < PIECES; x += 64) {
+            const int piece = PIECES % 64 && x + lane >= PIECES ? PIECES - 1 : x + lane;
+            const int row = piece / PER_ROW, col = piece % PER_ROW * V;
+            const int m = m0 + wm + 16 * (kg * MINE + i) + row, n = n0 + wn + col;
             float v[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = half[row * PITCH + lane % PER_ROW * V + e];
-            if (m < p.m && n < p.n) store_results(C + (int64_t)m * p.ldc, v, p.n - n, p);
+            for (int e = 0; e < V; ++e) v[e] = half[row * PITCH + col + e];
+            if (x + lane < PIECES && m < p.m && n < p.n)
+                store_results((T*)p.C + (int64_t)m * p.ldc + n, v, p.n - n, p);
         }
     }
 }
@@ -549,31 +552,38 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
     return hipGetLastError();
 }
 
-// The kernels' times, in us, for choosing one: `fixed` and, per `terms` terms, `step` for each
-// round of `per_cu` workgroups on each CU, fitted to the times beside.  (Rates of the tiles: the
-// 256^2 one asks the L2s for half of what 128^2 does, and 128^2 for half of 64^2, and an L2 serves
-// a CU some 60 bytes per ns; what counts for few tiles is a stage's latency, that more stages,
-// groups of waves or workgroups on a CU hide: four of the 64^2 with one group fit on one.)
-//                     512^3  1024^2 x 2048  x 8192  2048^2 x 512  1500^2 x 300  4096 x 1024 x 4096  4096^2 x 1024  4096^3
-//   64^2, 1 group       4.5            7.1    16.2           8.1           6.8                18.4
-//   64^2, 2 groups      5.1            7.1    13.5          16.7          12.8                29.3           62.4   105.2
-//   128^2, 4 stages     6.0            8.4    21.0           7.5           7.7                15.2           25.3    50.7
-//   128^2, 2 per CU     7.1           10.2    26.3           8.3           9.6                17.2           20.6    43.7
-//   256^2                                     45.4                                            28.3           16.7    36.2
+// The kernels' times, in us, for choosing one: a launch and, for each round of `per_cu` workgroups
+// on each CU, `fixed` (the first stage's arrival, and the results' way out) and `step` per `terms`
+// terms, fitted to the times beside (bf16 results; * fp32).  Rates of the tiles: the 256^2 one asks
+// the L2s for half of what 128^2 does, and 128^2 for half of 64^2, and an L2 serves a CU some 60
+// bytes per ns; what counts for few tiles is a stage's latency, that more stages, groups of waves
+// or workgroups on a CU hide: four of the 64^2 with one group fit on one.  Three quarters of a
+// 256^2 tile use all CUs where whole ones leave a quarter of them idle.
+//                   512^3  1024^2  1024^2  2048^2  4096 x 1024  4096^2  4096^3  4095 x 3001  6000^2
+//                          x 2048  x 8192   x 512       x 4096  x 1024               x 2047  x 1000
+//   64^2, 1 group     4.5     7.1    16.2     8.1         18.4
+//   64^2, 2 groups    5.1     7.1    13.5    16.7         29.3    62.4   105.2
+//   128^2, 4 stages   6.0     8.4    21.0     7.5         15.2    25.3    50.7
+//   128^2, 2 per CU   7.1    10.2    26.3     8.3         17.2    20.6    43.7        31.6*    43.8
+//   256 x 192                                                                         27.9*    45.7
+//   192 x 256                                                                                  40.6
+//   256^2                            45.4                 28.3    16.7    36.2        31.9*    46.4
 struct TilePlan {
-    int size, per_cu, terms;
+    int rows, cols, per_cu, terms;
     double step, fixed;
 };
-constexpr TilePlan kTilePlans[] = {{64, 1, 256, 0.39, 3.7},  {64, 2, 256, 0.55, 4.5},  {64, 4, 256, 0.75, 6.6},
-                                   {64, 1, 512, 0.53, 4.8},  {128, 1, 256, 0.56, 5.8}, {128, 2, 256, 1.05, 5.5},
-                                   {256, 1, 256, 1.65, 9.0}};
+constexpr TilePlan kTilePlans[] = {
+    {64, 64, 1, 256, 0.39, 1.2},    {64, 64, 2, 256, 0.55, 2.0},   {64, 64, 4, 256, 0.75, 3.3},
+    {64, 64, 1, 512, 0.53, 2.3},    {128, 128, 1, 256, 0.56, 3.3}, {128, 128, 2, 256, 0.95, 4.7},
+    {256, 192, 1, 256, 1.18, 10.5}, {192, 256, 1, 256, 1.12, 9.5}, {256, 256, 1, 256, 1.45, 10.0}};
+constexpr double kLaunchUs = 2.5;
 constexpr int kCus = 256;
 
 double tile_us(const TilePlan& t, const Mx4GemmArgs& a)
 {
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int64_t rounds = up(up(a.m, t.size) * up(a.n, t.size), t.per_cu * kCus);
-    return (double)rounds * (t.fixed + (double)up(a.k, t.terms) * t.step);
+    const int64_t rounds = up(up(a.m, t.rows) * up(a.n, t.cols), t.per_cu * kCus);
+    return kLaunchUs + (double)rounds * (t.fixed + (double)up(a.k, t.terms) * t.step);
 }
 
 template <typename T>
@@ -586,7 +596,7 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
     if (narrow <= 16 && wide > 16 * kCus) return launch_skinny<T, 1, 2>(a, s);
     double best = 1e30;
     int pick = 0;
-    for (int i = 0; i < 7; ++i) {
+    for (int i = 0; i < 9; ++i) {
         const double t = tile_us(kTilePlans[i], a);
         if (t < best) {
             best = t;
@@ -604,6 +614,8 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
     case 3: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
     case 4: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
     case 5: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
+    case 6: return launch_tile<T, 2, 4, 1, 8, 3, 2>(a, s);
+    case 7: return launch_tile<T, 2, 4, 1, 6, 4, 2>(a, s);
     default: return launch_tile<T, 2, 4, 1, 8, 4, 2>(a, s);
     }
 }

@@ -103,7 +103,8 @@ def test_gemm_larger(cuda, m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(600, 600, 31), (640, 577, 1000), (1025, 1000, 1700), (1500, 1500, 300),
                                    (450, 500, 6500), (1000, 1000, 4128), (1100, 1150, 2900), (129, 4096, 900),
-                                   (1800, 2040, 1300), (3000, 3100, 200), (65, 65, 65), (4100, 4090, 96)])
+                                   (1800, 2040, 1300), (3000, 3100, 200), (65, 65, 65), (4100, 4090, 96),
+                                   (4090, 3001, 1090), (3001, 4090, 1090), (2049, 6000, 1030), (6000, 2100, 770)])
 def test_gemm_tiles(cuda, m, n, k):
     """Few and many tiles of every kind, with terms that end inside a stage."""
     _run(cuda, "f16", m, n, k, beta=1.0)
