@@ -18,13 +18,14 @@ struct Arith<double> {
     typedef double type;
 };
 
-// Threads form TX chunks of 8 columns by 256 / TX rows.
+// Threads form TX pieces of 16 bytes of a row (8 columns share a call of the generator: threads
+// of fp32 make it twice, of fp64 four times) by 256 / TX rows.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64_t ldy, int tx)
 {
     typedef typename Arith<T>::type R;
-    const uint32_t chunk = blockIdx.x * tx + threadIdx.x % tx;
-    const int64_t c0 = (int64_t)chunk * 8;
+    constexpr int N = Piece<T>::N;
+    const int64_t c0 = ((int64_t)blockIdx.x * tx + threadIdx.x % tx) * N;
     if (c0 >= a.cols) return;
     const R scale = (R)a.scale;
     const int rows_per = 256 / tx;
@@ -34,22 +35,29 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64
         const T* g = a.gate ? (const T*)a.gate + row * a.ldg + c0 : nullptr;
         T* y = Y + row * ldy + c0;
         uint32_t keep[4];
-        if (a.threshold) keep_words(a, (uint32_t)row, chunk, keep);
-        if (c0 + 8 <= a.cols) {
-            const Eight<T> xv = *(const Eight<T>*)x;
-            Eight<T> yv;
+        if (a.threshold) {
+            keep_words(a, (uint32_t)row, (uint32_t)(c0 / 8), keep);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int from = N; from < 8; from += N)  // the piece's words first
+                if (c0 % 8 == from)
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) keep[i] = keep[from / 2 + i];
+        }
+        if (c0 + N <= a.cols) {
+            const Piece<T> xv = *(const Piece<T>*)x;
+            Piece<T> yv;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
                 yv.v[i] = !a.threshold || kept(a, keep, i) ? (T)((R)xv.v[i] * scale) : (T)0;
             if (g) {
-                const Eight<T> gv = *(const Eight<T>*)g;
+                const Piece<T> gv = *(const Piece<T>*)g;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) yv.v[i] = gv.v[i] > (T)0 ? yv.v[i] : (T)0;
+                for (int i = 0; i < N; ++i) yv.v[i] = gv.v[i] > (T)0 ? yv.v[i] : (T)0;
             }
             store_past(y, yv);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < N; ++i) {
                 if (c0 + i >= a.cols) continue;
                 const bool on = (!a.threshold || kept(a, keep, i)) && (!g || g[i] > (T)0);
                 y[i] = on ? (T)((R)x[i] * scale) : (T)0;
@@ -61,10 +69,10 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64
 template <typename T>
 hipError_t launch(const DropoutArgs& a, void* Y, int64_t ldy, hipStream_t s)
 {
-    const int64_t chunks = (a.cols + 7) / 8;
+    const int64_t pieces = (a.cols + Piece<T>::N - 1) / Piece<T>::N;
     int tx = 1;
-    while (tx < 256 && tx < chunks) tx *= 2;
-    const int64_t gx = (chunks + tx - 1) / tx, rows_per = 256 / tx;
+    while (tx < 256 && tx < pieces) tx *= 2;
+    const int64_t gx = (pieces + tx - 1) / tx, rows_per = 256 / tx;
     int64_t gy = (a.rows + rows_per - 1) / rows_per;
     if (gy > 65535) gy = 65535;
     dropout_kernel<T><<<dim3((unsigned)gx, (unsigned)gy), 256, 0, s>>>(a, (T*)Y, ldy, tx);

@@ -87,17 +87,21 @@ struct __attribute__((packed, aligned(sizeof(T)))) Eight {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Stores them past the L2s.
+// Sixteen bytes of neighbouring values: what a lane stores at once, so that a wave's instruction
+// writes whole lines (fp32 in two such pieces a lane, 32 bytes apart between lanes: 8192^2
+// dequantised 114 us, in one 46).
 template <typename T>
-__device__ inline void store_past(T* to, const Eight<T>& y)
+struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+
+// Stores it past the L2s.
+template <typename T>
+__device__ inline void store_past(T* to, const Piece<T>& y)
 {
-    struct Words {
-        u32x4 w[sizeof(T) / 2];
-    };
-    const Words w = __builtin_bit_cast(Words, y);
     typedef u32x4 __attribute__((aligned(2))) loose_t;  // (16-byte accesses need no alignment)
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) __builtin_nontemporal_store(w.w[i], (loose_t*)to + i);
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), (loose_t*)to);
 }
 
 }  // namespace sbx

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mx4.hpp"
 
 namespace sbx {
@@ -186,43 +188,49 @@ __global__ void __launch_bounds__(512, 4) quantize_kernel(DropoutArgs a, Mx4Out 
     }
 }
 
-// Threads form TX chunks of 8 columns by 256 / TX rows, kRows times.
-constexpr int kRows = 4;
+// Threads form TX pieces of 16 bytes of a row's values by 256 / TX rows, as many times as give a
+// thread 32 values.
+template <typename T>
+constexpr int kRows = 32 / Piece<T>::N;
 
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, const uint8_t* P, int64_t ldp,
                                                          const uint8_t* S, int64_t lds, T* Y, int64_t ldy, int tx,
                                                          int col_tiles)
 {
-    const int64_t c0 = ((int64_t)(blockIdx.x % col_tiles) * tx + threadIdx.x % tx) * 8;
+    constexpr int N = Piece<T>::N, R = kRows<T>;
+    typedef typename std::conditional<N == 8, uint32_t, uint16_t>::type elems_t;
+    const int64_t c0 = ((int64_t)(blockIdx.x % col_tiles) * tx + threadIdx.x % tx) * N;
     const int per = 256 / tx;
-    const int64_t r0 = (int64_t)(blockIdx.x / col_tiles) * (per * kRows) + threadIdx.x / tx;
+    const int64_t r0 = (int64_t)(blockIdx.x / col_tiles) * (per * R) + threadIdx.x / tx;
     if (c0 >= cols) return;
-    uint32_t w[kRows], code[kRows];
+    uint32_t w[R], code[R];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < R; ++i) {
         const int64_t r = r0 + i * per < rows ? r0 + i * per : rows - 1;  // (a row past the last is not stored)
-        w[i] = *(const uint32_t*)(P + r * ldp + c0 / 2);
+        w[i] = *(const elems_t*)(P + r * ldp + c0 / 2);
         code[i] = S[c0 / 256 * lds + r * 8 + c0 / 32 % 8];
     }
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < R; ++i) {
         const int64_t r = r0 + i * per;
         if (r >= rows) break;
         const float scale = scale_of(code[i]);
         f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 0),
-                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 1),
-                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 2),
-                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 3)};
-        Eight<T> y;
+                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 1)};
+        if constexpr (N == 8) {
+            v[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 2);
+            v[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 3);
+        }
+        Piece<T> y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y.v[e] = (T)(code[i] == 255 ? __builtin_nanf("") : v[e / 2][e % 2]);
+        for (int e = 0; e < N; ++e) y.v[e] = (T)(code[i] == 255 ? __builtin_nanf("") : v[e / 2][e % 2]);
         T* to = Y + r * ldy + c0;
-        if (c0 + 8 <= cols)
+        if (c0 + N <= cols)
             store_past(to, y);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < N; ++e)
                 if (c0 + e < cols) to[e] = y.v[e];
     }
 }
@@ -246,10 +254,11 @@ template <typename T>
 hipError_t dequantize(int64_t rows, int64_t cols, const uint8_t* P, int64_t ldp, const uint8_t* S,
                       int64_t lds, void* Y, int64_t ldy, hipStream_t s)
 {
-    const int64_t chunks = (cols + 7) / 8;
+    const int64_t pieces = (cols + Piece<T>::N - 1) / Piece<T>::N;
     int tx = 1;
-    while (tx < 256 && tx < chunks) tx *= 2;
-    const int64_t ct = (chunks + tx - 1) / tx, rt = (rows + 256 / tx * kRows - 1) / (256 / tx * kRows);
+    while (tx < 256 && tx < pieces) tx *= 2;
+    const int64_t per = 256 / tx * kRows<T>;
+    const int64_t ct = (pieces + tx - 1) / tx, rt = (rows + per - 1) / per;
     if (rt * ct > 0x7fffffff) return hipErrorInvalidValue;
     dequantize_kernel<T><<<(unsigned)(rt * ct), 256, 0, s>>>(rows, cols, P, ldp, S, lds, (T*)Y, ldy, tx, (int)ct);
     return hipGetLastError();
