@@ -109,7 +109,7 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
         for (int e = 0; e < V; ++e) o.v[e] = result<T>(acc[e], p.beta != 0.0f ? (float)in.v[e] : 0.0f, p);
         // Rows of whole 64 bytes go past the L2s, that keep the operands then (8192^2 x 512 to bf16
         // 60.5 -> 55.1 us, 4096^2 x 1024 23.4 -> 16.7 us); of others an L2 has to put the pieces
-        // together (4095 x 3001 x 2047 to fp32 28.7 us, past them 32.8).
+        // together (4095 x 3001 x 2047 to fp32 27.7 us, past them 38.4).
         typedef u32x4 __attribute__((aligned(2))) loose_t;
         if (p.past)
             __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), (loose_t*)c);
@@ -131,7 +131,8 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
 // is permuted by the address each lane reads instead: block b of row x at place
 // b ^ swizzle(x).  LDS has 64 banks, and serves 16 bytes a lane to lanes 0-3, 12-15,
 // 20-27, then to the others of 0-31, then 32-63 likewise; with the swizzles below no
-// two of such 16 lanes of a fragment read meet (SQ_LDS_BANK_CONFLICT: 0).
+// two of such 16 lanes of a fragment read meet (SQ_LDS_BANK_CONFLICT: 8 % of the LDS
+// cycles, one for each read of codes, which are 2 bytes a lane).
 //   A stage is multiplied in two halves; lane group q takes block 2q + h of a row in
 // half h, so its codes for both are one 16-bit read.
 //   While a half is multiplied, the next is read from LDS: A's block i into its own
@@ -141,6 +142,15 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
 //   B's block j holds the tile's rows 16 G (j / G) + 4 (j % G) + 4 G (i / 4) + i % 4 at
 // its index i (G: 2, or all 3 blocks), so that a lane's results of G blocks are 4 G
 // neighbouring columns.
+//   What bounds it.  8192^3 to bf16, 242-256 us over boxes (4.3-4.5 PFLOP/s; these products
+// straight from registers 8.66): power, at 1.9 GHz with the matrix units 56 % busy, and the
+// operands' way from the L2s (2.6 GB, 10 TB/s) beside; C's way out is not hidden.  A
+// stage's loads asked for at once 290 us against 284 spread, results straight from the registers
+// 284 against 261, reads of a pass in a row 261 against 256; four waves of 128 x 128 527 against
+// 503 us at 16384 terms.
+// 4096 x 1024 x 4096 on 128^2 tiles 15.2-16.9 us: the L2s, 134 MB at some 60 bytes per ns and CU.
+// 4095 x 3001 x 2047 to fp32 23.6-26.6 us: C, 49 MB in rows that no line begins with (of 3008
+// columns 24.3).  512^3 to fp32 4.6: launch, the first stage's way, C's.
 template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
 __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
 {
@@ -401,6 +411,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
 // workgroup takes 16 XB rows of X and all of Y, its eight waves each an eighth of the terms, in
 // groups of 256 by turns, straight from memory to registers (a lane's 32 neighbouring bytes of a
 // row; the group after is under way meanwhile).  The waves' sums are added up in LDS, in order.
+//   Bound by memory: 1 x 8192 x 8192 (36 MB) 8.4 us, 9.8 a call with the launch between, 1 x 28672
+// x 8192 27 us (4.6 TB/s; a copy reaches 5.2).  Blocks of 64 neighbouring bytes an instruction, in
+// place of 32 a lane, took as long.
 constexpr int kSkinnyWaves = 8;
 
 template <int N>

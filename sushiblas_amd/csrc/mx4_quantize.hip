@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(512, 4) quantize_kernel(DropoutArgs a, Mx4Out 
 
 // Threads form TX pieces of 16 bytes of a row's values by 256 / TX rows, as many times as give a
 // thread 32 values.
+//   Bound by HBM: 8192^2 to bf16 25.4 us (170 MB, 6.7 TB/s), to fp32 45.6 (304 MB, 6.7 TB/s); rows
+// that begin inside a line cost more: 8191 x 8190 33.4 and 67.0.
 template <typename T>
 constexpr int kRows = 32 / Piece<T>::N;
 
