@@ -57,6 +57,7 @@ struct Mx4GemmArgs {
     float alpha, beta;
     int relu;
     int past;  // C's rows are whole 64-byte lines
+    int down;  // fp32 pieces of 16 bytes are not aligned, and C is no more than the MALL's half
 };
 
 // dtype: an sbx_dtype that the caller has checked.

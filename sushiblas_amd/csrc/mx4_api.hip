@@ -142,6 +142,8 @@ int sbx_mx4_gemm(void* stream, int dtype, int layout, int64_t m, int64_t n, int6
     a.alpha = alpha; a.beta = beta;
     a.relu = epilogue == SBX_EPILOGUE_RELU;
     a.past = ((uintptr_t)C | (uint64_t)ldc * sbx::elem_size(dtype)) % 64 == 0;
+    a.down = dtype == SBX_F32 && ((uintptr_t)C | (uint64_t)ldc * 4) % 16 != 0 &&
+             ldc <= (32 << 20) / (layout == 0 ? m : n);
     if (layout == 1) {  // column-major C (m x n) is row-major C^T = B * A^T
         const uint8_t *t = a.A, *ts = a.SA;
         a.A = a.B; a.SA = a.SB; a.B = t; a.SB = ts;

@@ -97,16 +97,30 @@ __device__ inline T result(float acc, float c, const Mx4GemmArgs& p)
     return (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
 }
 
-// Neighbouring results of a row, `left` of them inside C.
+// A piece of neighbouring results of a row, `left` (or none) of them inside C, which is at c.
 template <typename T>
-__device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], int left, const Mx4GemmArgs& p)
+__device__ inline Vec<T> finish(const float (&acc)[16 / sizeof(T)], const T* c, int left, const Mx4GemmArgs& p)
+{
+    constexpr int V = 16 / sizeof(T);
+    Vec<T> o, in = {};
+    if (p.beta != 0.0f) {
+        if (left >= V)
+            in = *(const Vec<T>*)c;
+        else
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < left) in.v[e] = c[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.v[e] = result<T>(acc[e], (float)in.v[e], p);
+    return o;
+}
+
+template <typename T>
+__device__ inline void store(T* c, const Vec<T>& o, int left, const Mx4GemmArgs& p)
 {
     constexpr int V = 16 / sizeof(T);
     if (left >= V) {
-        Vec<T> o, in;
-        if (p.beta != 0.0f) in = *(const Vec<T>*)c;
-#pragma unroll
-        for (int e = 0; e < V; ++e) o.v[e] = result<T>(acc[e], p.beta != 0.0f ? (float)in.v[e] : 0.0f, p);
         // Rows of whole 64 bytes go past the L2s, that keep the operands then (8192^2 x 512 to bf16
         // 60.5 -> 55.1 us, 4096^2 x 1024 23.4 -> 16.7 us); of others an L2 has to put the pieces
         // together (4095 x 3001 x 2047 to fp32 27.7 us, past them 38.4).
@@ -118,7 +132,7 @@ __device__ inline void store_results(T* c, const float (&acc)[16 / sizeof(T)], i
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (e < left) c[e] = result<T>(acc[e], p.beta != 0.0f ? (float)c[e] : 0.0f, p);
+            if (e < left) c[e] = o.v[e];
     }
 }
 
@@ -380,10 +394,14 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
                             trade[(((1 - kg) * WAVES + wave) * MINE + i) * NB * 64 + j * 64 + lane];
         __syncthreads();
     }
-    // Out through LDS, 16 rows of the wave's at a time, so that an instruction stores whole
-    // rows of them (from the registers it would store 32 columns of 16 rows).
     constexpr int V = 16 / sizeof(T), COLS = 16 * NB, PITCH = COLS + 4;
     constexpr int PER_ROW = COLS / V, PIECES = 16 * PER_ROW;
+    // Out through LDS, 16 rows of the wave's at a time, so that an instruction stores whole
+    // rows of them (from the registers it would store 32 columns of 16 rows).  Neighbouring lanes
+    // store neighbouring pieces of a row; where those of fp32 are not aligned, the same piece of
+    // neighbouring rows instead: 3001 x 4095 x 2047 24.5 us in place of 32.0, 4095^2 x 1000 23.7
+    // in place of 34.1, 2047 x 2049 x 512 11.6 and 10.8.  Not for 16 bits (4095^2 x 1000 28.7
+    // against 23.3), nor for C's that the MALL does not hold (8191^2 x 500 128 against 105).
     static_assert(2 * 16 * PITCH * 4 * WAVES <= NS * STAGE, "");
     float* out = (float*)lds_all + wave_all * 2 * 16 * PITCH;
 #pragma unroll
@@ -395,13 +413,20 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
 #pragma unroll
         for (int x = 0; x < PIECES; x += 64) {
             const int piece = PIECES % 64 && x + lane >= PIECES ? PIECES - 1 : x + lane;
-            const int row = piece / PER_ROW, col = piece % PER_ROW * V;
-            const int m = m0 + wm + 16 * (kg * MINE + i) + row, n = n0 + wn + col;
+            int row = piece / PER_ROW, col = piece % PER_ROW * V;
+            if (V == 4 && p.down) {
+                constexpr int ROWS = PER_ROW % 8 ? 16 : 8;  // by 64 / ROWS pieces an instruction
+                row = x / 64 * ROWS % 16 + lane % ROWS;
+                col = (x / 64 * ROWS / 16 * (64 / ROWS) + lane / ROWS) * V;
+            }
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = half[row * PITCH + col + e];
-            if (x + lane < PIECES && m < p.m && n < p.n)
-                store_results((T*)p.C + (int64_t)m * p.ldc + n, v, p.n - n, p);
+            const int m = m0 + wm + 16 * (kg * MINE + i) + row, n = n0 + wn + col;
+            if (x + lane < PIECES && m < p.m) {
+                T* c = (T*)p.C + (int64_t)m * p.ldc + n;
+                store(c, finish<T>(v, c, p.n - n, p), p.n - n, p);
+            }
         }
     }
 }
