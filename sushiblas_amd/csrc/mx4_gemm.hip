@@ -162,7 +162,8 @@ __device__ inline void store(T* c, const Vec<T>& o, int left, const Mx4GemmArgs&
 // stage's loads asked for at once 290 us against 284 spread, results straight from the registers
 // 284 against 261, reads of a pass in a row 261 against 256; four waves of 128 x 128 527 against
 // 503 us at 16384 terms.
-// 4096 x 1024 x 4096 on 128^2 tiles 15.2-16.9 us: the L2s, 134 MB at some 60 bytes per ns and CU.
+// 4096 x 1024 x 4096 on 128^2 tiles 15.2-16.9 us: a stage 0.57 us, its products alone 0.25, its
+// LDS reads 0.29, both without the loads 0.48-0.51: LDS and the matrix units, which overlap in part.
 // 4095 x 3001 x 2047 to fp32 23.6-26.6 us: C, 49 MB in rows that no line begins with (of 3008
 // columns 24.3).  512^3 to fp32 4.6: launch, the first stage's way, C's.
 template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
@@ -592,11 +593,10 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 
 // The kernels' times, in us, for choosing one: a launch and, for each round of `per_cu` workgroups
 // on each CU, `fixed` (the first stage's arrival, and the results' way out) and `step` per `terms`
-// terms, fitted to the times beside (bf16 results; * fp32).  Rates of the tiles: the 256^2 one asks
-// the L2s for half of what 128^2 does, and 128^2 for half of 64^2, and an L2 serves a CU some 60
-// bytes per ns; what counts for few tiles is a stage's latency, that more stages, groups of waves
-// or workgroups on a CU hide: four of the 64^2 with one group fit on one.  Three quarters of a
-// 256^2 tile use all CUs where whole ones leave a quarter of them idle.
+// terms, fitted to the times beside (bf16 results; * fp32).  The 256^2 tile asks the L2s for half
+// of what 128^2 does, and 128^2 for half of 64^2; what counts for few tiles is a stage's latency,
+// that more stages, groups of waves or workgroups on a CU hide: four of the 64^2 with one group
+// fit on one.  Three quarters of a 256^2 tile use all CUs where whole ones leave a quarter idle.
 //                   512^3  1024^2  1024^2  2048^2  4096 x 1024  4096^2  4096^3  4095 x 3001  6000^2
 //                          x 2048  x 8192   x 512       x 4096  x 1024               x 2047  x 1000
 //   64^2, 1 group     4.5     7.1    16.2     8.1         18.4
