@@ -76,7 +76,7 @@ __device__ inline void load_lds(uint32_t lds, int voff, i32x4 rsrc, int soff)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
                  "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+                 : "memory", "m0");
 }
 template <int N>
 __device__ inline void wait_loads_and_barrier()
@@ -156,7 +156,7 @@ __device__ inline void store(T* c, const Vec<T>& o, int left, const Mx4GemmArgs&
 //   B's block j holds the tile's rows 16 G (j / G) + 4 (j % G) + 4 G (i / 4) + i % 4 at
 // its index i (G: 2, or all 3 blocks), so that a lane's results of G blocks are 4 G
 // neighbouring columns.
-//   What bounds it.  8192^3 to bf16, 242-256 us over boxes (4.3-4.5 PFLOP/s; these products
+//   What bounds it.  8192^3 to bf16, 242-256 us (4.3-4.5 PFLOP/s; these products
 // straight from registers 8.66): power, at 1.9 GHz with the matrix units 56 % busy, and the
 // operands' way from the L2s (2.6 GB, 10 TB/s) beside; C's way out is not hidden.  A
 // stage's loads asked for at once 290 us against 284 spread, results straight from the registers
