@@ -164,8 +164,8 @@ __device__ inline void store(T* c, const Vec<T>& o, int left, const Mx4GemmArgs&
 // 503 us at 16384 terms.
 // 4096 x 1024 x 4096 on 128^2 tiles 15.2-16.9 us: a stage 0.57 us, its products alone 0.25, its
 // LDS reads 0.29, both without the loads 0.48-0.51: LDS and the matrix units, which overlap in part.
-// 4095 x 3001 x 2047 to fp32 23.6-26.6 us: C, 49 MB in rows that no line begins with (of 3008
-// columns 24.3).  512^3 to fp32 4.6: launch, the first stage's way, C's.
+// 4095 x 3001 x 2047 to fp32 22.9-25.0 us: C, 49 MB in rows that no line begins with (of 3004
+// columns 22.5).  512^3 to fp32 4.6: launch, the first stage's way, C's.
 template <typename T, int WM, int WN, int KG, int MB, int NB, int NS>
 __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmArgs p, int tiles_m, int tiles_n)
 {
