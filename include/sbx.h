@@ -255,7 +255,9 @@ int sbx_dropout(void* stream, int dtype, int64_t rows, int64_t cols, const void*
  * infinity or NaN has code 255: all of it is NaN.
  * P, PT 16-byte aligned, ldp >= 16*ceil(cols/32) and a multiple of 16; S, ST
  * 8-byte aligned, lds >= 8*rows and a multiple of 8 (ldpt, ldst: of rows and
- * cols). */
+ * cols).  As everywhere here this is asked of a leading dimension also where one
+ * row, or one group of codes, leaves it without a use (the Python binding, which
+ * is given torch's strides, puts the packed one there). */
 int sbx_mx4_quantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* X,
                      int64_t ldx, const void* gate, int64_t ldg, double p, uint64_t seed,
                      uint32_t stream_id, void* P, int64_t ldp, void* S, int64_t lds, void* PT,

@@ -297,11 +297,18 @@ def syrk(dtype, layout, upper, trans, n, k, alpha, A, lda, str_a, beta, C, ldc, 
              str_a, beta, _ptr(C), ldc, str_c, batch), "sbx_syrk")
 
 
+# The dropout and MXFP4 calls below take leading dimensions from tensors.  torch
+# gives a dimension of one entry any stride it likes (8 bytes to the one group of
+# codes in S of a (rows, 1, 8) tensor made (1, rows, 8)), and no step is taken
+# along it: where there is one row, or one group of 8 blocks, the packed leading
+# dimension is passed in its place, whatever was given.
 def dropout(dtype, rows, cols, X, ldx, Y, ldy, p, seed, stream_id, gate=None, ldg=0,
             stream=None) -> None:
     """sbx_dropout: Y = keep ? X / (1 - p) : 0, where gate > 0 if there is one.
     The mask comes from (seed, stream_id) and the element's place, so the
     backward pass is the same call on the gradient."""
+    if rows == 1:
+        ldx = ldy = ldg = cols
     _check(lib().sbx_dropout(_stream(stream), dtype, rows, cols, _ptr(X), ldx, _ptr(gate), ldg,
                              _ptr(Y), ldy, p, seed, stream_id), "sbx_dropout")
 
@@ -314,11 +321,21 @@ def mx4_shapes(rows, cols):
     return (rows, 16 * nb), (-(-nb // 8), rows, 8)
 
 
+def _mx4_lds(rows, cols, ldp, lds):
+    """The leading dimensions of a rows x cols MXFP4 matrix: as given, but for one
+    row or one group of codes (up to 8 blocks)."""
+    return (16 * (-(-cols // 32)) if rows == 1 else ldp), (8 * rows if cols <= 256 else lds)
+
+
 def mx4_quantize(dtype, rows, cols, X, ldx, P=None, ldp=0, S=None, lds=0, PT=None, ldpt=0,
                  ST=None, ldst=0, p=0.0, seed=0, stream_id=0, gate=None, ldg=0,
                  stream=None) -> None:
     """sbx_mx4_quantize: X, after dropout and gate, to MXFP4 along its rows
     (P, S), its columns (PT, ST) or both in one pass."""
+    if rows == 1:
+        ldx = ldg = cols
+    ldp, lds = _mx4_lds(rows, cols, ldp, lds)
+    ldpt, ldst = _mx4_lds(cols, rows, ldpt, ldst)
     _check(lib().sbx_mx4_quantize(_stream(stream), dtype, rows, cols, _ptr(X), ldx, _ptr(gate),
                                   ldg, p, seed, stream_id, _ptr(P), ldp, _ptr(S), lds, _ptr(PT),
                                   ldpt, _ptr(ST), ldst), "sbx_mx4_quantize")
@@ -326,6 +343,9 @@ def mx4_quantize(dtype, rows, cols, X, ldx, P=None, ldp=0, S=None, lds=0, PT=Non
 
 def mx4_dequantize(dtype, rows, cols, P, ldp, S, lds, Y, ldy, stream=None) -> None:
     """sbx_mx4_dequantize: the values an MXFP4 matrix stands for."""
+    ldp, lds = _mx4_lds(rows, cols, ldp, lds)
+    if rows == 1:
+        ldy = cols
     _check(lib().sbx_mx4_dequantize(_stream(stream), dtype, rows, cols, _ptr(P), ldp, _ptr(S),
                                     lds, _ptr(Y), ldy), "sbx_mx4_dequantize")
 
@@ -334,6 +354,10 @@ def mx4_gemm(dtype, layout, m, n, k, alpha, A, lda, SA, ldsa, B, ldb, SB, ldsb, 
              epilogue=EPILOGUE_NONE, stream=None) -> None:
     """sbx_mx4_gemm: C = epilogue(alpha * A * B^T + beta * C) of two MXFP4
     matrices quantised along k."""
+    lda, ldsa = _mx4_lds(m, k, lda, ldsa)
+    ldb, ldsb = _mx4_lds(n, k, ldb, ldsb)
+    if (n if layout else m) == 1:
+        ldc = m if layout else n
     _check(lib().sbx_mx4_gemm(_stream(stream), dtype, int(layout), m, n, k, alpha, _ptr(A), lda,
                               _ptr(SA), ldsa, _ptr(B), ldb, _ptr(SB), ldsb, beta, _ptr(C), ldc,
                               int(epilogue)), "sbx_mx4_gemm")
