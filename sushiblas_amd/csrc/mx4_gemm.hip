@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "mx4.hpp"
+#include "mx4_strip.hpp"
 
 namespace sbx {
 namespace {
@@ -19,7 +20,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRsrcWord3 = 0x00020000;
-constexpr int kOutside = (int)0x80000000u;  // an offset past every descriptor's end: reads zeros
 
 // c += b * a^T, with byte H of the codes.  As assembly, so that the sums stay
 // where they are: given the builtin, the compiler moves the 256 sums of a 128 x 128
@@ -229,11 +229,12 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     auto load_part = [&](int t, int x) {
         const uint32_t at = lds0 + t % NS * STAGE;
         const int tk = t * KG + kg, left = nb - 8 * tk;
+        const int from = min(tk, (nb - 1) / 8) * 128;  // (counts inside alone: mx4_strip.hpp)
         if (x < LA)
-            load_lds(at + (wave * LA + x) * 1024, ca[x % LA] < left ? va[x % LA] : kOutside, da, tk * 128);
+            load_lds(at + (wave * LA + x) * 1024, ca[x % LA] < left ? va[x % LA] : kOutside, da, from);
         else
             load_lds(at + OFF_B + (wave * LB + x - LA) * 1024, cb[(x - LA) % LB] < left ? vb[(x - LA) % LB] : kOutside,
-                     db, tk * 128);
+                     db, from);
         if (x == LA + LB - 1 && wave < NC) {
             const uint64_t s = (uint64_t)code_at;
             const int n = left <= 0 || code_left <= 0 ? 0 : code_left > 128 ? 1024 : 8 * code_left;
@@ -448,55 +449,55 @@ struct Group {
     int code[N];  // two codes in its low bytes
 };
 
-// The rows of an operand that a workgroup takes, and the lane's place in them.
+// The rows of an operand that a workgroup takes, and the lane's place in them (mx4_strip.hpp).
+template <int N>
 struct Strip {
     const uint8_t *rows, *codes;
     int64_t lds;
-    int bytes, count, ld, at, code_at;
+    int bytes, count, ld, lane, at[N], code_at;
 
     __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n,
-                                int most, int nb, int lane)
+                                int nb, int lane_)
     {
-        count = min(n - first, most);
+        count = min(n - first, 16 * N);
         ld = (int)ld_;
         lds = lds_;
+        lane = lane_;
         rows = P + first * ld_;
-        bytes = (count - 1) * ld + 16 * nb;
+        bytes = strip_bytes(count, ld, nb);
         codes = S + 8 * (int64_t)first;
-        at = lane % 16 * ld + lane / 16 * 32;
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = strip_lane(lane, i, count, ld);
         code_at = lane % 16 * 8 + lane / 16 * 2;
     }
 
-    // Group g (256 terms) of N times 16 rows; zeros, not from memory, past the last row and past
-    // the last group (left <= 0 blocks).
-    template <int N>
+    // Group g (256 terms), with `left` blocks up to the last: zeros, not from memory, past it
+    // and past the last row.  The codes of a group's 8 blocks are all there.
     __device__ inline void load(Group<N>& d, int g, int left) const
     {
-        const __amdgpu_buffer_rsrc_t v = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(rows), (short)0,
-                                                                           left > 0 ? bytes : 0, kRsrcWord3);
+        const __amdgpu_buffer_rsrc_t v =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(rows), (short)0, bytes, kRsrcWord3);
         const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(codes) + g * lds, (short)0, left > 0 ? 8 * count : 0, kRsrcWord3);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int from = 16 * i * ld + g * 128;
-            d.v[i][0] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at, from, 0));
-            d.v[i][1] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at + 16, from, 0));
+            const int from = strip_scalar(i, g, count, ld, left);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                d.v[i][h] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                          v, strip_vector(at[i], lane, h, left), from, 0));
             d.code[i] = __builtin_amdgcn_raw_buffer_load_b16(c, code_at + 128 * i, 0, 0);
         }
     }
 };
 
-// What lies past the last block is not used: `mine` of the lane's two blocks are inside.
+// Codes past the last block may be NaN's and are cleared (the elements there are zeros):
+// `mine` of the lane's two blocks are inside.
 template <int N>
 __device__ inline void clip(Group<N>& d, int mine)
 {
-    const i32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        d.v[i][0] = mine >= 1 ? d.v[i][0] : zero;
-        d.v[i][1] = mine >= 2 ? d.v[i][1] : zero;
-        d.code[i] = mine >= 2 ? d.code[i] : mine == 1 ? d.code[i] & 0xff : 0;
-    }
+    for (int i = 0; i < N; ++i) d.code[i] = mine >= 2 ? d.code[i] : mine == 1 ? d.code[i] & 0xff : 0;
 }
 
 template <typename T, int YB, int XB, bool XA>
@@ -510,9 +511,10 @@ __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 4 ? 2 : 4) mx4_s
     const int r = lane % 16, q = lane / 16;
     const int x0 = blockIdx.x * (16 * XB), y0 = blockIdx.y * (16 * YB);
     const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
-    Strip sx, sy;
-    sx.init(XA ? p.A : p.B, XA ? p.lda : p.ldb, XA ? p.SA : p.SB, XA ? p.ldsa : p.ldsb, x0, nx, 16 * XB, nb, lane);
-    sy.init(XA ? p.B : p.A, XA ? p.ldb : p.lda, XA ? p.SB : p.SA, XA ? p.ldsb : p.ldsa, y0, ny, 16 * YB, nb, lane);
+    Strip<XB> sx;
+    Strip<YB> sy;
+    sx.init(XA ? p.A : p.B, XA ? p.lda : p.ldb, XA ? p.SA : p.SB, XA ? p.ldsa : p.ldsb, x0, nx, nb, lane);
+    sy.init(XA ? p.B : p.A, XA ? p.ldb : p.lda, XA ? p.SB : p.SA, XA ? p.ldsb : p.ldsa, y0, ny, nb, lane);
 
     f32x4 acc[XB][YB] = {};
     auto load = [&](Group<XB>& x, Group<YB>& y, int g) {

@@ -50,6 +50,13 @@ def test_product_of_one_group(cuda, k):
     _product(cuda, 500, 520, k)
 
 
+@pytest.mark.parametrize("k", TERMS + [700])
+@pytest.mark.parametrize("m,n", [(1, 5000), (3, 40), (4501, 1), (60, 70), (16, 4110)])
+def test_product_of_one_group_or_row_narrow(cuda, m, n, k):
+    """On the kernel for narrow operands, whose last workgroup has few of the wide one's rows."""
+    _product(cuda, m, n, k)
+
+
 @pytest.mark.parametrize("cols", TERMS)
 def test_quantize_and_back_one_group(cuda, cols):
     import torch
