@@ -222,6 +222,20 @@ def _check(status: int, where: str) -> None:
         raise SbxError(status, where)
 
 
+def _fp(dtype, single, double, where: str):
+    """The fp32 or fp64 entry point; other codes are refused as the dtype-generic
+    entry points refuse them."""
+    if dtype not in (F32, F64):
+        raise SbxError(2, where)
+    return single if dtype == F32 else double
+
+
+def _code(t) -> int:
+    """A tensor's F32 or F64 by its element size; of another size a code that every
+    entry point refuses."""
+    return {4: F32, 8: F64}.get(t.element_size(), -1)
+
+
 def gemm_ex(dtype, layout, transA, transB, m, n, k, alpha, A, lda, str_a, B, ldb, str_b, beta,
             C, ldc, str_c, batch=1, algo=ALGO_AUTO, stream=None) -> None:
     """sbx_gemm_ex: dtype-generic, optionally batched, with an algorithm override."""
@@ -263,7 +277,7 @@ def gemm_fused(dtype, layout, transA, transB, m, n, k, alpha, A, lda, str_a, B, 
 def relu(x, n=None, dtype=None, stream=None) -> None:
     """sbx_relu in place: x = x > 0 ? x : 0 over n contiguous elements."""
     if dtype is None:
-        dtype = F32 if x.element_size() == 4 else F64
+        dtype = _code(x)
     if n is None:
         n = x.numel()
     _check(lib().sbx_relu(_stream(stream), dtype, _ptr(x), n), "sbx_relu")
@@ -284,7 +298,7 @@ def dgemm(layout, transA, transB, m, n, k, alpha, A, lda, B, ldb, beta, C, ldc,
 def gemv(dtype, layout, trans, m, n, alpha, A, lda, x, incx, beta, y, incy,
          stream=None) -> None:
     """sbx_sgemv / sbx_dgemv: y = alpha*op(A)*x + beta*y."""
-    f = lib().sbx_sgemv if dtype == F32 else lib().sbx_dgemv
+    f = _fp(dtype, lib().sbx_sgemv, lib().sbx_dgemv, "sbx_gemv")
     _check(f(_stream(stream), int(layout), int(trans), m, n, alpha, _ptr(A), lda, _ptr(x), incx,
              beta, _ptr(y), incy), "sbx_gemv")
 
@@ -292,7 +306,7 @@ def gemv(dtype, layout, trans, m, n, alpha, A, lda, x, incx, beta, y, incy,
 def syrk(dtype, layout, upper, trans, n, k, alpha, A, lda, str_a, beta, C, ldc, str_c,
          batch=1, stream=None) -> None:
     """sbx_{s,d}syrk_strided_batched: one triangle of C = alpha*op(A)*op(A)^T + beta*C."""
-    f = lib().sbx_ssyrk_strided_batched if dtype == F32 else lib().sbx_dsyrk_strided_batched
+    f = _fp(dtype, lib().sbx_ssyrk_strided_batched, lib().sbx_dsyrk_strided_batched, "sbx_syrk")
     _check(f(_stream(stream), int(layout), int(upper), int(trans), n, k, alpha, _ptr(A), lda,
              str_a, beta, _ptr(C), ldc, str_c, batch), "sbx_syrk")
 
@@ -433,14 +447,14 @@ def syrk_select(dtype, layout, upper, trans, n, k, lda, ldc) -> str:
 
 def fill_uniform(t, seed: int, stream_id: int, stream=None) -> None:
     """Fill a float32/float64 device tensor with Philox uniform [-1, 1)."""
-    dtype = F32 if t.element_size() == 4 else F64
+    dtype = _code(t)
     _check(lib().sbx_fill_uniform(_stream(stream), dtype, _ptr(t), t.numel(), seed, stream_id),
            "sbx_fill_uniform")
 
 
 def fill_normal(t, seed: int, stream_id: int, scale: float = 1.0, stream=None) -> None:
     """Fill a float32/float64 device tensor with Philox N(0, 1) * scale."""
-    dtype = F32 if t.element_size() == 4 else F64
+    dtype = _code(t)
     _check(lib().sbx_fill_normal(_stream(stream), dtype, _ptr(t), t.numel(), seed, stream_id,
                                  scale), "sbx_fill_normal")
 
