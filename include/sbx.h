@@ -221,7 +221,9 @@ int sbx_dsyrk_strided_batched(void* stream, int layout, int upper, int trans, in
  * block whose products run on the 4-bit matrix cores: quantise activations,
  * weights and gradients along the axis that a product sums over, multiply, and
  * drop activations out on their way.  All matrices are row-major; nothing is
- * allocated and no workspace used. */
+ * allocated and no workspace used.  Sides are 2^30 at most (m, n too; and what
+ * would take 2^31 tiles of 128 x 128 to quantise, or 2^23 of 256 x 256 to
+ * multiply, is refused too): SBX_UNSUPPORTED. */
 
 /* Dropout, Y = keep ? X / (1 - p) : 0 (rows x cols, F32, F64, BF16 or F16).
  * keep is a function of (seed, stream_id, row, column) alone, by the

@@ -60,7 +60,18 @@ struct Mx4GemmArgs {
     int down;  // fp32 pieces of 16 bytes are not aligned, and C is no more than the MALL's half
 };
 
-// dtype: an sbx_dtype that the caller has checked.
+// A launch takes less than 2^32 threads along x: workgroups (of up to 512) past the kGridX-th go
+// on along z.  Some at the end have no tile then.
+constexpr int64_t kMaxThreads = 0xffffffff;
+constexpr int kGridX = 1 << 22;
+inline dim3 grid_of(int64_t blocks, unsigned y = 1)
+{
+    return dim3((unsigned)(blocks < kGridX ? blocks : kGridX), y, (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ inline uint32_t block_x() { return blockIdx.z * kGridX + blockIdx.x; }
+
+// dtype: an sbx_dtype that the caller has checked.  hipErrorNotSupported: a grid of more than a
+// launch takes.
 hipError_t launch_dropout(int dtype, const DropoutArgs& a, void* Y, int64_t ldy, hipStream_t s);
 hipError_t launch_mx4_quantize(int dtype, const DropoutArgs& a, const Mx4Out& rows,
                                const Mx4Out& cols, hipStream_t s);

@@ -54,7 +54,10 @@ int dropout_args(DropoutArgs* a, const void* X, int64_t ldx, const void* gate, i
     return SBX_OK;
 }
 
-int status_of(hipError_t e) { return e == hipSuccess ? SBX_OK : SBX_HIP_ERROR; }
+int status_of(hipError_t e)
+{
+    return e == hipSuccess ? SBX_OK : e == hipErrorNotSupported ? SBX_UNSUPPORTED : SBX_HIP_ERROR;
+}
 
 }  // namespace
 }  // namespace sbx

@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 4 ? 2 : 4) mx4_s
 
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r = lane % 16, q = lane / 16;
-    const int x0 = blockIdx.x * (16 * XB), y0 = blockIdx.y * (16 * YB);
+    const int x0 = block_x() * (16 * XB), y0 = blockIdx.y * (16 * YB);
+    if (x0 >= nx) return;
     const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
     Strip<XB> sx;
     Strip<YB> sy;
@@ -574,7 +575,7 @@ template <typename T, int YB, int XB>
 hipError_t launch_skinny(const Mx4GemmArgs& a, hipStream_t s)
 {
     auto grid = [](int x, int y) {
-        return dim3((unsigned)((x + 16 * XB - 1) / (16 * XB)), (unsigned)((y + 16 * YB - 1) / (16 * YB)));
+        return grid_of((x + 16 * XB - 1) / (16 * XB), (unsigned)((y + 16 * YB - 1) / (16 * YB)));
     };
     if (a.m <= a.n)
         mx4_skinny_kernel<T, YB, XB, false><<<grid(a.n, a.m), 64 * kSkinnyWaves, 0, s>>>(a);
@@ -588,7 +589,7 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
 {
     constexpr int BM = 16 * MB * WM, BN = 16 * NB * WN;
     const int tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
-    if ((int64_t)tm * tn > 0x7fffffff) return hipErrorInvalidValue;
+    if ((int64_t)tm * tn * (64 * WM * WN * KG) > kMaxThreads) return hipErrorNotSupported;
     mx4_gemm_kernel<T, WM, WN, KG, MB, NB, NS><<<(unsigned)(tm * tn), 64 * WM * WN * KG, 0, s>>>(a, tm, tn);
     return hipGetLastError();
 }
@@ -622,7 +623,8 @@ constexpr int kCus = 256;
 double tile_us(const TilePlan& t, const Mx4GemmArgs& a)
 {
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int64_t rounds = up(up(a.m, t.rows) * up(a.n, t.cols), t.per_cu * kCus);
+    const int64_t tiles = up(a.m, t.rows) * up(a.n, t.cols), rounds = up(tiles, t.per_cu * kCus);
+    if (tiles * 512 > kMaxThreads) return 1e30;  // more than a launch takes
     return kLaunchUs + (double)rounds * (t.fixed + (double)up(a.k, t.terms) * t.step);
 }
 
@@ -643,6 +645,7 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
             pick = i;
         }
     }
+    if (best == 1e30 && narrow > 16) return hipErrorNotSupported;
     // Small results over many terms (256^2 x 8192: 6.6 against 10.9 us on the 64^2 tile, 128 x 1024 x
     // 8192 10.8 against 10.8): 2048 terms of a block take its waves about 1 us.
     const double blocks = ((narrow + 15) / 16) * (double)((wide + 15) / 16) / kCus;

@@ -78,12 +78,13 @@ __device__ inline void load_rows(Eight<T> (&x)[RPT], const void* X, int64_t ld, 
 template <typename T, bool DROP, bool GATE>
 __global__ void __launch_bounds__(512, 4) quantize_kernel(DropoutArgs a, Mx4Out ro, Mx4Out co, int col_tiles)
 {
+    const uint32_t tile = block_x();  // (those past the last row's store nothing)
     constexpr int PITCH_P = 72, PITCH_PT = 68;  // (no bank is met twice by a wave's writes)
     __shared__ uint32_t row_codes[TILE], col_codes[TILE];
     __shared__ __align__(8) uint8_t row_elems[TILE * PITCH_P];
     __shared__ __align__(4) uint8_t col_elems[TILE * PITCH_PT];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int64_t tile_r = (int64_t)(blockIdx.x / col_tiles) * TILE, tile_c = (int64_t)(blockIdx.x % col_tiles) * TILE;
+    const int64_t tile_r = (int64_t)(tile / col_tiles) * TILE, tile_c = (int64_t)(tile % col_tiles) * TILE;
     const int rl = wave / 2 * 32 + lane / 8 * RPT, cl = wave % 2 * 64 + lane % 8 * 8;  // in the tile
     const int64_t r0 = tile_r + rl, c0 = tile_c + cl;
 
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(512, 4) quantize_kernel(DropoutArgs a, Mx4Out 
             const uint32_t* w = (const uint32_t*)(col_elems + t / 4 * PITCH_PT + t % 4 * 16);
             __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, (u32x4*)(co.P + col * co.ldp + r / 2));
         }
-        if (t < TILE && tile_c + t < a.cols)
+        if (t < TILE && tile_c + t < a.cols && tile_r / 256 * 256 < a.rows)
             *(uint32_t*)(co.S + tile_r / 256 * co.lds + (tile_c + t) * 8 + tile_r / 32 % 8) = col_codes[t];
     }
 }
@@ -243,8 +244,8 @@ hipError_t quantize(const DropoutArgs& a, const Mx4Out& rows, const Mx4Out& cols
     // whole groups of 8 blocks along a form's axis: their codes are written to the end
     const int64_t rt = cols.P ? (a.rows + 255) / 256 * 2 : (a.rows + TILE - 1) / TILE;
     const int64_t ct = rows.P ? (a.cols + 255) / 256 * 2 : (a.cols + TILE - 1) / TILE;
-    if (rt * ct > 0x7fffffff) return hipErrorInvalidValue;
-    const unsigned grid = (unsigned)(rt * ct);
+    if (rt * ct > 0x7fffffff) return hipErrorNotSupported;
+    const dim3 grid = grid_of(rt * ct);
     if (a.threshold && a.gate) quantize_kernel<T, true, true><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
     else if (a.threshold) quantize_kernel<T, true, false><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
     else if (a.gate) quantize_kernel<T, false, true><<<grid, 512, 0, s>>>(a, rows, cols, (int)ct);
@@ -261,7 +262,7 @@ hipError_t dequantize(int64_t rows, int64_t cols, const uint8_t* P, int64_t ldp,
     while (tx < 256 && tx < pieces) tx *= 2;
     const int64_t per = 256 / tx * kRows<T>;
     const int64_t ct = (pieces + tx - 1) / tx, rt = (rows + per - 1) / per;
-    if (rt * ct > 0x7fffffff) return hipErrorInvalidValue;
+    if (rt * ct * 256 > kMaxThreads) return hipErrorNotSupported;
     dequantize_kernel<T><<<(unsigned)(rt * ct), 256, 0, s>>>(rows, cols, P, ldp, S, lds, (T*)Y, ldy, tx, (int)ct);
     return hipGetLastError();
 }
