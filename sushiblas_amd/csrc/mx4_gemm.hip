@@ -647,9 +647,10 @@ hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
     }
     if (best == 1e30 && narrow > 16) return hipErrorNotSupported;
     // Small results over many terms (256^2 x 8192: 6.6 against 10.9 us on the 64^2 tile, 128 x 1024 x
-    // 8192 10.8 against 10.8): 2048 terms of a block take its waves about 1 us.
+    // 8192 10.8 against 10.8): up to 2048 terms of a block, none among them, take its waves about 1 us.
     const double blocks = ((narrow + 15) / 16) * (double)((wide + 15) / 16) / kCus;
-    if (narrow <= 16 || 2.2 + (a.k + 2047) / 2048 * (blocks < 1 ? 1 : blocks) < best) return launch_skinny<T, 1, 1>(a, s);
+    const int steps = a.k > 0 ? (a.k + 2047) / 2048 : 1;
+    if (narrow <= 16 || 2.2 + steps * (blocks < 1 ? 1 : blocks) < best) return launch_skinny<T, 1, 1>(a, s);
     switch (pick) {
     case 0:
     case 1:
