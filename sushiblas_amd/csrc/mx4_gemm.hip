@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "mx4.hpp"
+#include "mx4_plan.hpp"
 #include "mx4_strip.hpp"
 
 namespace sbx {
@@ -594,73 +595,20 @@ hipError_t launch_tile(const Mx4GemmArgs& a, hipStream_t s)
     return hipGetLastError();
 }
 
-// The kernels' times, in us, for choosing one: a launch and, for each round of `per_cu` workgroups
-// on each CU, `fixed` (the first stage's arrival, and the results' way out) and `step` per `terms`
-// terms, fitted to the times beside (bf16 results; * fp32).  The 256^2 tile asks the L2s for half
-// of what 128^2 does, and 128^2 for half of 64^2; what counts for few tiles is a stage's latency,
-// that more stages, groups of waves or workgroups on a CU hide: four of the 64^2 with one group
-// fit on one.  Three quarters of a 256^2 tile use all CUs where whole ones leave a quarter idle.
-//                   512^3  1024^2  1024^2  2048^2  4096 x 1024  4096^2  4096^3  4095 x 3001  6000^2
-//                          x 2048  x 8192   x 512       x 4096  x 1024               x 2047  x 1000
-//   64^2, 1 group     4.5     7.1    16.2     8.1         18.4
-//   64^2, 2 groups    5.1     7.1    13.5    16.7         29.3    62.4   105.2
-//   128^2, 4 stages   6.0     8.4    21.0     7.5         15.2    25.3    50.7
-//   128^2, 2 per CU   7.1    10.2    26.3     8.3         17.2    20.6    43.7        31.6*    43.8
-//   256 x 192                                                                         27.9*    45.7
-//   192 x 256                                                                                  40.6
-//   256^2                            45.4                 28.3    16.7    36.2        31.9*    46.4
-struct TilePlan {
-    int rows, cols, per_cu, terms;
-    double step, fixed;
-};
-constexpr TilePlan kTilePlans[] = {
-    {64, 64, 1, 256, 0.39, 1.2},    {64, 64, 2, 256, 0.55, 2.0},   {64, 64, 4, 256, 0.75, 3.3},
-    {64, 64, 1, 512, 0.53, 2.3},    {128, 128, 1, 256, 0.56, 3.3}, {128, 128, 2, 256, 0.95, 4.7},
-    {256, 192, 1, 256, 1.18, 10.5}, {192, 256, 1, 256, 1.12, 9.5}, {256, 256, 1, 256, 1.45, 10.0}};
-constexpr double kLaunchUs = 2.5;
-constexpr int kCus = 256;
-
-double tile_us(const TilePlan& t, const Mx4GemmArgs& a)
-{
-    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int64_t tiles = up(a.m, t.rows) * up(a.n, t.cols), rounds = up(tiles, t.per_cu * kCus);
-    if (tiles * 512 > kMaxThreads) return 1e30;  // more than a launch takes
-    return kLaunchUs + (double)rounds * (t.fixed + (double)up(a.k, t.terms) * t.step);
-}
-
 template <typename T>
 hipError_t launch(const Mx4GemmArgs& a, hipStream_t s)
 {
-    const int narrow = a.m < a.n ? a.m : a.n, wide = a.m < a.n ? a.n : a.m;
-    // One narrow block: the wide operand at the rate memory gives it.  Two blocks of it a
-    // workgroup where that leaves one for each CU (1 x 8192 x 8192: 9.2 against 9.5 us, 16 rows
-    // 10.3 against 11.7; the 64^2 tile 11.5 and 11.2).
-    if (narrow <= 16 && wide > 16 * kCus) return launch_skinny<T, 1, 2>(a, s);
-    double best = 1e30;
-    int pick = 0;
-    for (int i = 0; i < 9; ++i) {
-        const double t = tile_us(kTilePlans[i], a);
-        if (t < best) {
-            best = t;
-            pick = i;
-        }
-    }
-    if (best == 1e30 && narrow > 16) return hipErrorNotSupported;
-    // Small results over many terms (256^2 x 8192: 6.6 against 10.9 us on the 64^2 tile, 128 x 1024 x
-    // 8192 10.8 against 10.8): up to 2048 terms of a block, none among them, take its waves about 1 us.
-    const double blocks = ((narrow + 15) / 16) * (double)((wide + 15) / 16) / kCus;
-    const int steps = a.k > 0 ? (a.k + 2047) / 2048 : 1;
-    if (narrow <= 16 || 2.2 + steps * (blocks < 1 ? 1 : blocks) < best) return launch_skinny<T, 1, 1>(a, s);
-    switch (pick) {
-    case 0:
-    case 1:
-    case 2: return launch_tile<T, 2, 2, 1, 2, 2, 2>(a, s);
-    case 3: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
-    case 4: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
-    case 5: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
-    case 6: return launch_tile<T, 2, 4, 1, 8, 3, 2>(a, s);
-    case 7: return launch_tile<T, 2, 4, 1, 6, 4, 2>(a, s);
-    default: return launch_tile<T, 2, 4, 1, 8, 4, 2>(a, s);
+    switch (mx4_kernel(a.m, a.n, a.k)) {
+    case Mx4Kernel::Narrow2: return launch_skinny<T, 1, 2>(a, s);
+    case Mx4Kernel::Narrow: return launch_skinny<T, 1, 1>(a, s);
+    case Mx4Kernel::Tile64: return launch_tile<T, 2, 2, 1, 2, 2, 2>(a, s);
+    case Mx4Kernel::Tile64Groups: return launch_tile<T, 2, 2, 2, 2, 2, 4>(a, s);
+    case Mx4Kernel::Tile128Stages: return launch_tile<T, 2, 4, 1, 4, 2, 4>(a, s);
+    case Mx4Kernel::Tile128: return launch_tile<T, 2, 2, 1, 4, 4, 2>(a, s);
+    case Mx4Kernel::Tile256x192: return launch_tile<T, 2, 4, 1, 8, 3, 2>(a, s);
+    case Mx4Kernel::Tile192x256: return launch_tile<T, 2, 4, 1, 6, 4, 2>(a, s);
+    case Mx4Kernel::Tile256: return launch_tile<T, 2, 4, 1, 8, 4, 2>(a, s);
+    default: return hipErrorNotSupported;
     }
 }
 
