@@ -230,8 +230,9 @@ int sbx_dsyrk_strided_batched(void* stream, int layout, int upper, int trans, in
  * counter-based Philox4x32-10: 16 bits h per element -- word c % 8 / 2, half
  * c % 2, of the counter (c / 8, row, stream_id, 0x44524F50) under the key seed --
  * and an element stays if h >= t, t = floor(65536 p + 0.5).  The factor is
- * 65536 / (65536 - t) exactly, so the mean is kept whatever p rounds to; p = 1
- * drops everything.  The mask is never stored: the backward pass is the same
+ * 65536 / (65536 - t), rounded to the arithmetic's type (fp64 for F64, else fp32):
+ * that of the rate that p is rounded to, so the mean is kept.  From p = 1 - 2^-17
+ * on (t = 65536) everything is dropped.  The mask is never stored: the backward pass is the same
  * call on dY with the same p, seed and stream_id.
  * gate (may be NULL): values that pass only where gate > 0, else 0.  Backward:
  * the output of the ReLU that the dropout followed, so the call is the gradient
@@ -273,7 +274,7 @@ int sbx_mx4_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, cons
 /* C = epilogue(alpha * A * B^T + beta * C): A (m x k) and B (n x k) MXFP4
  * matrices (A, SA with lda, ldsa; B, SB with ldb, ldsb, as written by
  * sbx_mx4_quantize), C (m x n) of dtype F32, BF16 or F16 in `layout`.  Products
- * are exact, sums are held in 32 bits and rounded to dtype once.  What lies
+ * are exact (down to 2^-149), sums are held in 32 bits and rounded to dtype once.  What lies
  * past the k-th term's block is not used, nor are the codes there.  BLAS
  * semantics as for GEMM (beta == 0: C is not read; alpha == 0 or k == 0: A and
  * B are not).  A layer's three products are this one on the right quantisations:

@@ -22,7 +22,7 @@ struct Arith<double> {
 // of fp32 make it twice, of fp64 four times) by 256 / TX rows.
 //   Bound by HBM: 8192^2 bf16 43.7 us (268 MB, 6.1 TB/s), with a gate 65.3; fp32 91.5 (537 MB, 5.9
 // TB/s; a call of the generator for 8 values, which leaves a lane 32 bytes apart from the next,
-// 102), with a gate 132.6.  The generator makes 792 G calls/s: 8192^2 in 11 us, under the loads.
+// 102), with a gate 132.6; fp64 175-217 (1.07 GB, 4.9-6.1 TB/s), with a gate 254.  The generator makes 792 G calls/s: 8192^2 in 11 us, under the loads.
 // Small ones are a launch: fp32 512 x 1024 3.3 us, 5.5 a call.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, T* Y, int64_t ldy, int tx)

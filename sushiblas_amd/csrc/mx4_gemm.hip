@@ -157,9 +157,11 @@ __device__ inline void store(T* c, const Vec<T>& o, int left, const Mx4GemmArgs&
 //   B's block j holds the tile's rows 16 G (j / G) + 4 (j % G) + 4 G (i / 4) + i % 4 at
 // its index i (G: 2, or all 3 blocks), so that a lane's results of G blocks are 4 G
 // neighbouring columns.
-//   What bounds it.  8192^3 to bf16, 242-256 us (4.3-4.5 PFLOP/s; these products
-// straight from registers 8.66): power, at 1.9 GHz with the matrix units 56 % busy, and the
-// operands' way from the L2s (2.6 GB, 10 TB/s) beside; C's way out is not hidden.  A
+//   What bounds it.  8192^3 to bf16, 237-257 us (4.3-4.6 PFLOP/s; these products
+// straight from registers 8.66, which is 2.07 GHz): without loads and LDS reads 166 us, at 2.08 GHz
+// with the matrix units 76 % busy -- each round's first stage and C's way out are not hidden; with
+// them power holds 1.82-1.9 GHz and the units are 57 % busy, beside the operands' way from the L2s
+// (2.6 GB, 10 TB/s).  A
 // stage's loads asked for at once 290 us against 284 spread, results straight from the registers
 // 284 against 261, reads of a pass in a row 261 against 256; four waves of 128 x 128 527 against
 // 503 us at 16384 terms.
@@ -434,8 +436,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
     }
 }
 
-// Products with a narrow operand Y of up to 128 rows (tokens, or the columns of a narrow C) and
-// any number of rows of the wide one X (XA: A, else B), which is read from memory once: a
+// Products with a narrow operand Y (a few tokens, or the columns of a narrow C) and any number of
+// rows of the wide one X (XA: A, else B), or with a small C over many terms (mx4_plan.hpp): a
 // workgroup takes 16 XB rows of X and all of Y, its eight waves each an eighth of the terms, in
 // groups of 256 by turns, straight from memory to registers (a lane's 32 neighbouring bytes of a
 // row; the group after is under way meanwhile).  The waves' sums are added up in LDS, in order.

@@ -71,8 +71,8 @@ __device__ inline void load_rows(Eight<T> (&x)[RPT], const void* X, int64_t ld, 
 // generator.  A row's block lies in 4 neighbouring lanes, a column's in 8 lanes 8 apart, so one
 // pass over X makes both forms in registers.  They are gathered in LDS and leave 64 bytes of a
 // row at a time, past the L2s.
-//   Bound by HBM: 8192^2 bf16 37.4 us to both forms (205 MB, 5.5 TB/s), 27.1 to the rows' alone
-// (170 MB, 6.3 TB/s); stored through the L2s 45.9 and 33.7 us, straight from the lanes (4 bytes of
+//   Bound by HBM: 8192^2 bf16 33-37 us to both forms (205 MB, 5.5-6.2 TB/s), 25.5-27.1 to the rows'
+// alone (170 MB, 6.3-6.7 TB/s), 25.7-26.1 to the columns', fp32 53, 44 and 45; stored through the L2s 45.9 and 33.7 us, straight from the lanes (4 bytes of
 // P, 2 of PT each: the L2s take as long for a request of 16 bytes as for one of 64) 53.2 and 34.8.
 // With dropout and gate 57.3 us, the generator's and the selects' VALU work beside.
 template <typename T, bool DROP, bool GATE>
