@@ -62,8 +62,8 @@ typedef enum sbx_status {
     SBX_HIP_ERROR = 3         /* a HIP runtime call or kernel launch failed                */
 } sbx_status;
 
-/* SBX_BF16 and SBX_F16: the dropout and MXFP4 entry points only (the others
- * return SBX_UNSUPPORTED). */
+/* SBX_BF16 and SBX_F16: the dropout, norm, MXFP4 and MXFP8 entry points only (the
+ * others return SBX_UNSUPPORTED). */
 typedef enum sbx_dtype { SBX_F32 = 0, SBX_F64 = 1, SBX_BF16 = 2, SBX_F16 = 3 } sbx_dtype;
 
 /* Replaces oneapi::mkl::blas::row_major::gemm<float> (gemm.cpp:63) and
@@ -286,6 +286,86 @@ int sbx_mx4_gemm(void* stream, int dtype, int layout, int64_t m, int64_t n, int6
                  const void* A, int64_t lda, const void* SA, int64_t ldsa, const void* B,
                  int64_t ldb, const void* SB, int64_t ldsb, float beta, void* C, int64_t ldc,
                  int epilogue);
+
+/* ---- Norm, and MXFP4 weights for a few tokens -------------------------------
+ *
+ * None of these has a counterpart in the reference.  They are what stands around a
+ * dense layer: the norm before it, with the residual's addition, in training and
+ * serving, and products for a few tokens whose weights are MXFP4 matrices
+ * (sbx_mx4_quantize along rows) and whose activations keep their type, or 8 bits.
+ * dtype is F32, BF16 or F16, all dense matrices are row-major and of it.  Nothing is
+ * allocated: what needs memory of its own takes it from the caller, as many bytes
+ * as its _workspace function says (0: sizes that are refused), 16-byte aligned; its
+ * contents are nobody's business before or after, and calls that may run at the
+ * same time need one each. */
+
+/* H = X + R in dtype's precision (rounded to dtype; R NULL: H = X), and row by row
+ *   V = H * W / sqrt(mean(H^2) + eps)
+ * with W one value per column.  Sums and statistics are held in 64 bits, V in 32.
+ *   H, Y (NULL: not wanted): rows x cols, Y is V rounded to dtype.
+ *   P, S (NULL: not wanted): V as an MXFP8 matrix, blocks of 32 along its rows:
+ * element (r, c) is the e4m3 byte P[r*ldp + c], a row's last block filled with
+ * zeros; codes as MXFP4's (sbx_mx4_quantize).  code = max(floor(log2 max|v|) - 8,
+ * -127) + 127; elements are v / 2^(code - 127) rounded to nearest even and saturated
+ * at 448.  A block with an infinity or NaN has code 255: all of it is NaN.  P 16-byte
+ * aligned, ldp >= 32*ceil(cols/32) and a multiple of 16; S, lds as MXFP4's.
+ * One of H, Y, P at least.  H may be X or R; Y may be X or R too where H is neither
+ * (same leading dimension).  eps >= 0 and finite; with eps = 0 a row of zeros is NaN. */
+int sbx_rms_norm(void* stream, int dtype, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                 const void* R, int64_t ldr, const void* W, double eps, void* H, int64_t ldh, void* Y,
+                 int64_t ldy, void* P, int64_t ldp, void* S, int64_t lds);
+
+/* The gradient of Y = H * W / sqrt(mean(H^2) + eps): with s = 1 / sqrt(mean(H^2) + eps)
+ *   DX = s * DY * W - H * s^3 * mean(DY * W * H)  (+ DR, if there is one: a gradient that
+ *        reaches H along the residual), which is X's and R's of sbx_rms_norm alike
+ *   DW = the sum over rows of s * DY * H, in 32 bits (NULL: not wanted, and no workspace)
+ * s is computed again from H, so the forward call stores none.  DX may be DY or DR
+ * (same leading dimension).  The order of DW's sums depends on rows alone.  Without
+ * rows DW is zero. */
+int sbx_rms_norm_grad(void* stream, int dtype, int64_t rows, int64_t cols, const void* H, int64_t ldh,
+                      const void* W, double eps, const void* DY, int64_t lddy, const void* DR,
+                      int64_t lddr, void* DX, int64_t lddx, float* DW, void* workspace,
+                      size_t workspace_bytes);
+size_t sbx_rms_norm_grad_workspace(int64_t rows, int64_t cols);
+
+/* The values an MXFP8 matrix (P, S as above) stands for, rounded to dtype
+ * (F32: exact). */
+int sbx_mx8_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* P,
+                       int64_t ldp, const void* S, int64_t lds, void* Y, int64_t ldy);
+
+/* Y = epilogue(alpha * X * B^T + beta * Y) for a few rows: X (m x k) keeps its type
+ * (SX NULL) or is an MXFP8 matrix (X, SX), B (n x k) is an MXFP4 matrix, Y (m x n) of
+ * dtype.  X is not rounded; sums are held in 32 bits and rounded to dtype once.  What
+ * lies past the k-th term is not used.  BLAS semantics as for GEMM (beta == 0: Y is
+ * not read; alpha == 0 or k == 0: X and B are not).  Rows are computed apart: those of
+ * one call have the bits that they have alone.  m <= 1024, n <= 2^30, k <= 2^23, ldb <
+ * 2^23 - 15, with SX ldx < 2^24 - 31 (else SBX_UNSUPPORTED). */
+int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, float alpha,
+                   const void* X, int64_t ldx, const void* SX, int64_t ldsx, const void* B,
+                   int64_t ldb, const void* SB, int64_t ldsb, float beta, void* Y, int64_t ldy,
+                   int epilogue);
+
+/* A mixture-of-experts layer for a few tokens.  For each token x (a row of X, tokens x
+ * width): logits WR x (WR: experts x width, dense) in 64 bits; the topk experts with
+ * the highest ones, in that order, equal ones by index (NaN counts as the highest);
+ * p = softmax over the chosen ones' logits (normalize != 0) or over all (0); and
+ *   y = sum_j p_j * W2_e (silu(G_e x) * (U_e x)),  silu(z) = z / (1 + exp(-z)),  e the j-th expert
+ * W1, S1: an MXFP4 matrix of experts * 2 * hidden rows over width, expert e's G at rows
+ * e * 2 * hidden, its U hidden rows later.  W2, S2: of experts * width rows over hidden.
+ * Activations are not rounded before W1's product; before W2's they are held as the sum of
+ * two bf16 values (F32: three), 16 bits (24) where dtype has 8 or 11.  Sums are held in
+ * 32 bits and rounded to dtype once.
+ * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.
+ * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^20, ld1, ld2 <
+ * 2^23 - 15 (else SBX_UNSUPPORTED). */
+int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,
+                int64_t experts, int64_t topk, const void* X, int64_t ldx, const void* WR,
+                int64_t ldwr, int normalize, const void* W1, int64_t ld1, const void* S1,
+                int64_t lds1, const void* W2, int64_t ld2, const void* S2, int64_t lds2, void* Y,
+                int64_t ldy, int32_t* chosen, float* weights, void* workspace,
+                size_t workspace_bytes);
+size_t sbx_mx4_moe_workspace(int64_t tokens, int64_t width, int64_t hidden, int64_t experts,
+                             int64_t topk);
 
 /* Name of the plan (kernel tile and k-split) the dispatcher would launch for
  * this problem (tiling heuristics introspection for benchmarks).  A name is a

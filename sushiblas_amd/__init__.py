@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libsbx.so")
 # stamps for measurements; use_probe_library() selects it before first use.
 PROBE_LIB_PATH = os.path.join(_HERE, "lib", "libsbx_probe.so")
 
-F32, F64, BF16, F16 = 0, 1, 2, 3  # BF16, F16: dropout and MXFP4 calls only
+F32, F64, BF16, F16 = 0, 1, 2, 3  # BF16, F16: dropout, norm and MXFP4 calls only
 ALGO_AUTO, ALGO_GENERIC, ALGO_MFMA, ALGO_MFMA_TILE, ALGO_MFMA_SMALL = 0, 1, 2, 3, 4
 EPILOGUE_NONE, EPILOGUE_RELU = 0, 1
 STATUS = {0: "SBX_OK", 1: "SBX_INVALID_ARGUMENT", 2: "SBX_UNSUPPORTED", 3: "SBX_HIP_ERROR"}
@@ -144,6 +144,24 @@ def lib() -> ctypes.CDLL:
     L.sbx_mx4_gemm.restype = i32
     L.sbx_mx4_gemm.argtypes = [vp, i32, i32, i64, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp,
                                i64, vp, i64, ctypes.c_float, vp, i64, i32]
+    L.sbx_rms_norm.restype = i32
+    L.sbx_rms_norm.argtypes = [vp, i32, i64, i64, vp, i64, vp, i64, vp, ctypes.c_double, vp, i64,
+                               vp, i64, vp, i64, vp, i64]
+    L.sbx_rms_norm_grad.restype = i32
+    L.sbx_rms_norm_grad.argtypes = [vp, i32, i64, i64, vp, i64, vp, ctypes.c_double, vp, i64, vp,
+                                    i64, vp, i64, vp, vp, ctypes.c_size_t]
+    L.sbx_rms_norm_grad_workspace.restype = ctypes.c_size_t
+    L.sbx_rms_norm_grad_workspace.argtypes = [i64, i64]
+    L.sbx_mx8_dequantize.restype = i32
+    L.sbx_mx8_dequantize.argtypes = L.sbx_mx4_dequantize.argtypes
+    L.sbx_mx4_linear.restype = i32
+    L.sbx_mx4_linear.argtypes = [vp, i32, i64, i64, i64, ctypes.c_float, vp, i64, vp, i64, vp,
+                                 i64, vp, i64, ctypes.c_float, vp, i64, i32]
+    L.sbx_mx4_moe.restype = i32
+    L.sbx_mx4_moe.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, i64, i32, vp, i64,
+                              vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, ctypes.c_size_t]
+    L.sbx_mx4_moe_workspace.restype = ctypes.c_size_t
+    L.sbx_mx4_moe_workspace.argtypes = [i64] * 5
     L.sbx_version.restype = ctypes.c_char_p
     L.sbx_version.argtypes = []
     if LIB_PATH == PROBE_LIB_PATH:
@@ -375,6 +393,103 @@ def mx4_gemm(dtype, layout, m, n, k, alpha, A, lda, SA, ldsa, B, ldb, SB, ldsb, 
     _check(lib().sbx_mx4_gemm(_stream(stream), dtype, int(layout), m, n, k, alpha, _ptr(A), lda,
                               _ptr(SA), ldsa, _ptr(B), ldb, _ptr(SB), ldsb, beta, _ptr(C), ldc,
                               int(epilogue)), "sbx_mx4_gemm")
+
+
+def mx8_shapes(rows, cols):
+    """Shapes (uint8) of a rows x cols MXFP8 matrix without padding: elements (leading
+    dimension: the second) and scale codes (leading dimension: 8 * rows)."""
+    nb = -(-cols // 32)
+    return (rows, 32 * nb), (-(-nb // 8), rows, 8)
+
+
+def _mx8_lds(rows, cols, ldp, lds):
+    """_mx4_lds for an MXFP8 matrix."""
+    return (32 * (-(-cols // 32)) if rows == 1 else ldp), (8 * rows if cols <= 256 else lds)
+
+
+def rms_norm(dtype, rows, cols, X, ldx, W, eps, R=None, ldr=0, H=None, ldh=0, Y=None, ldy=0,
+             P=None, ldp=0, S=None, lds=0, stream=None) -> None:
+    """sbx_rms_norm: H = X + R, and H * W / sqrt(mean(H^2) + eps) along rows to Y, to
+    MXFP8 (P, S; mx8_shapes) or both."""
+    if rows == 1:
+        ldx = ldr = ldh = ldy = cols
+    ldp, lds = _mx8_lds(rows, cols, ldp, lds)
+    _check(lib().sbx_rms_norm(_stream(stream), dtype, rows, cols, _ptr(X), ldx, _ptr(R), ldr,
+                              _ptr(W), eps, _ptr(H), ldh, _ptr(Y), ldy, _ptr(P), ldp, _ptr(S),
+                              lds), "sbx_rms_norm")
+
+
+def _bytes(workspace, given) -> int:
+    """A workspace's size: as given, or the tensor's."""
+    if given is not None or workspace is None or isinstance(workspace, int):
+        return given or 0
+    return workspace.numel() * workspace.element_size()
+
+
+def rms_norm_grad_workspace(rows, cols) -> int:
+    """Bytes of rms_norm_grad's workspace."""
+    return int(lib().sbx_rms_norm_grad_workspace(rows, cols))
+
+
+def rms_norm_grad(dtype, rows, cols, H, ldh, W, eps, DY, lddy, DX, lddx, DW=None, DR=None, lddr=0,
+                  workspace=None, workspace_bytes=None, stream=None) -> None:
+    """sbx_rms_norm_grad: the norm's gradients with respect to its input H (plus DR) and, in
+    32 bits, to W.  With DW it needs a workspace (rms_norm_grad_workspace)."""
+    if rows == 1:
+        ldh = lddy = lddx = lddr = cols
+    _check(lib().sbx_rms_norm_grad(_stream(stream), dtype, rows, cols, _ptr(H), ldh, _ptr(W), eps,
+                                   _ptr(DY), lddy, _ptr(DR), lddr, _ptr(DX), lddx, _ptr(DW),
+                                   _ptr(workspace), _bytes(workspace, workspace_bytes)),
+           "sbx_rms_norm_grad")
+
+
+def mx8_dequantize(dtype, rows, cols, P, ldp, S, lds, Y, ldy, stream=None) -> None:
+    """sbx_mx8_dequantize: the values an MXFP8 matrix stands for."""
+    ldp, lds = _mx8_lds(rows, cols, ldp, lds)
+    if rows == 1:
+        ldy = cols
+    _check(lib().sbx_mx8_dequantize(_stream(stream), dtype, rows, cols, _ptr(P), ldp, _ptr(S),
+                                    lds, _ptr(Y), ldy), "sbx_mx8_dequantize")
+
+
+def mx4_linear(dtype, m, n, k, alpha, X, ldx, B, ldb, SB, ldsb, beta, Y, ldy, SX=None, ldsx=0,
+               epilogue=EPILOGUE_NONE, stream=None) -> None:
+    """sbx_mx4_linear: Y = epilogue(alpha * X * B^T + beta * Y) for a few rows of X, which
+    keep their type or (with SX) are MXFP8, and an MXFP4 matrix B."""
+    if SX is not None:
+        ldx, ldsx = _mx8_lds(m, k, ldx, ldsx)
+    elif m == 1:
+        ldx = k
+    ldb, ldsb = _mx4_lds(n, k, ldb, ldsb)
+    if m == 1:
+        ldy = n
+    _check(lib().sbx_mx4_linear(_stream(stream), dtype, m, n, k, alpha, _ptr(X), ldx, _ptr(SX),
+                                ldsx, _ptr(B), ldb, _ptr(SB), ldsb, beta, _ptr(Y), ldy,
+                                int(epilogue)), "sbx_mx4_linear")
+
+
+def mx4_moe_workspace(tokens, width, hidden, experts, topk) -> int:
+    """Bytes of mx4_moe's workspace."""
+    return int(lib().sbx_mx4_moe_workspace(tokens, width, hidden, experts, topk))
+
+
+def mx4_moe(dtype, tokens, width, hidden, experts, topk, X, ldx, WR, ldwr, W1, ld1, S1, lds1, W2,
+            ld2, S2, lds2, Y, ldy, normalize=True, chosen=None, weights=None, workspace=None,
+            workspace_bytes=None, stream=None) -> None:
+    """sbx_mx4_moe: a mixture-of-experts layer, router included, for a few tokens, its
+    experts' weights two MXFP4 matrices.  `chosen` (int32) and `weights` (float32), tokens x
+    topk, packed, receive the experts and their shares."""
+    if tokens == 1:
+        ldx = ldy = width
+    if experts == 1:
+        ldwr = width
+    ld1, lds1 = _mx4_lds(2 * experts * hidden, width, ld1, lds1)
+    ld2, lds2 = _mx4_lds(experts * width, hidden, ld2, lds2)
+    _check(lib().sbx_mx4_moe(_stream(stream), dtype, tokens, width, hidden, experts, topk, _ptr(X),
+                             ldx, _ptr(WR), ldwr, int(bool(normalize)), _ptr(W1), ld1, _ptr(S1),
+                             lds1, _ptr(W2), ld2, _ptr(S2), lds2, _ptr(Y), ldy, _ptr(chosen),
+                             _ptr(weights), _ptr(workspace), _bytes(workspace, workspace_bytes)),
+           "sbx_mx4_moe")
 
 
 def gemm_select(dtype, layout, transA, transB, m, n, k, lda, ldb, ldc, batch=1) -> str:

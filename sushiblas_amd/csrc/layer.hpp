@@ -1,0 +1,98 @@
+// layer.hpp -- what surrounds a layer with MXFP4 weights: the root-mean-square norm
+// and its gradient, the product for a few tokens, the mixture-of-experts layer.
+// Their arguments and launchers.
+//
+// An MXFP8 matrix is an MXFP4 one (mx4.hpp) with e4m3 elements, one a byte: 32 bytes
+// a block, codes in the same places, the largest element 448 = 1.75 * 2^8.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mx4.hpp"
+
+namespace sbx {
+
+struct NormArgs {
+    int64_t rows, cols;
+    const void *X, *R, *W;  // R: null, or what is added to X
+    int64_t ldx, ldr;
+    double eps;
+    void *H, *Y;  // the sum, its norm; null: not wanted
+    int64_t ldh, ldy;
+    Mx4Out q;  // the norm as MXFP8 (P null: not wanted)
+};
+
+struct NormGradArgs {
+    int64_t rows, cols;
+    const void *H, *W, *DY, *DR;  // DR: null, or a gradient that arrives at H beside the norm's
+    int64_t ldh, lddy, lddr;
+    double eps;
+    void* DX;
+    int64_t lddx;
+    float* DW;    // null: not wanted
+    float* part;  // with DW: norm_grad_parts(rows) x cols
+};
+
+// Groups of rows whose share of DW is summed apart.
+inline int norm_grad_parts(int64_t rows) { return rows < 256 ? (int)rows : 256; }
+
+struct Mx4LinearArgs {
+    int m, n, k;
+    const void* X;  // dense of the result's type; with SX e4m3 elements
+    int64_t ldx;
+    const uint8_t* SX;
+    int64_t ldsx;
+    const uint8_t *B, *SB;
+    int64_t ldb, ldsb;
+    void* Y;
+    int64_t ldy;
+    float alpha, beta;
+    int relu;
+};
+
+struct Mx4MoeArgs {
+    int tokens, width, hidden, experts, topk;
+    const void *X, *WR;
+    int64_t ldx, ldwr;
+    const uint8_t *W1, *S1, *W2, *S2;
+    int64_t ld1, lds1, ld2, lds2;
+    void* Y;
+    int64_t ldy;
+    int normalize;
+    int* chosen;     // null: not wanted
+    float* weights;  // the same
+    uint8_t* work;
+};
+
+// A mixture's workspace: offsets of its parts, each 256-byte aligned.
+struct Mx4MoeWork {
+    size_t logits, chosen, weights, act, bytes;
+};
+inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t hidden, int64_t experts, int64_t topk)
+{
+    Mx4MoeWork w;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t from = at;
+        at += (bytes + 255) / 256 * 256;
+        return from;
+    };
+    w.logits = take(8 * tokens * experts);
+    w.chosen = take(4 * tokens * topk);
+    w.weights = take(4 * tokens * topk);
+    w.act = take(4 * tokens * topk * hidden);
+    w.bytes = at;
+    return w;
+}
+
+// dtype: an sbx_dtype that the caller has checked.  hipErrorNotSupported: a grid of more than a
+// launch takes.
+hipError_t launch_rms_norm(int dtype, const NormArgs& a, hipStream_t s);
+hipError_t launch_rms_norm_grad(int dtype, const NormGradArgs& a, hipStream_t s);
+hipError_t launch_mx8_dequantize(int dtype, int64_t rows, int64_t cols, const uint8_t* P, int64_t ldp,
+                                 const uint8_t* S, int64_t lds, void* Y, int64_t ldy, hipStream_t s);
+hipError_t launch_mx4_linear(int dtype, const Mx4LinearArgs& a, hipStream_t s);
+hipError_t launch_mx4_moe(int dtype, const Mx4MoeArgs& a, hipStream_t s);
+
+}  // namespace sbx

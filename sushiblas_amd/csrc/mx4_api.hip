@@ -1,10 +1,11 @@
-// mx4_api.hip -- C entry points of the dropout and the MXFP4 operators
-// (include/sbx.h): argument checks, the column-major mapping, quick returns.
+// mx4_api.hip -- C entry points of the dropout, the norm and the operators on microscaled
+// matrices (include/sbx.h): argument checks, the column-major mapping, quick returns.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "../../include/sbx.h"
+#include "layer.hpp"
 #include "mx4.hpp"
 
 namespace sbx {
@@ -15,6 +16,10 @@ constexpr int64_t kMaxSide = (int64_t)1 << 30;  // rows, columns
 // kernel's 32-bit offsets
 constexpr int64_t kMaxTerms = (int64_t)1 << 23;
 constexpr int64_t kMaxRowBytes = ((int64_t)1 << 23) - 16;
+// what a mixture of experts takes: few tokens, and choices that fit its kernels' tables
+// (the rows of all experts together are within kMaxSide then)
+constexpr int64_t kMaxTokens = 256, kMaxExperts = 512, kMaxTopk = 16, kMaxLayer = (int64_t)1 << 20;
+constexpr int64_t kMaxLinearRows = 1024;
 
 int64_t blocks(int64_t k) { return (k + 31) / 32; }
 
@@ -31,11 +36,19 @@ bool bad_dense(const void* X, int64_t cols, int64_t ld, size_t elem)
     return !X || (uintptr_t)X % elem || ld < cols;
 }
 
-// The packed elements and codes of a rows x cols MXFP4 matrix.
-bool bad_mx4(const void* P, int64_t ldp, const void* S, int64_t lds, int64_t rows, int64_t cols)
+// The packed elements and codes of a rows x cols matrix of blocks of `bytes` bytes.
+bool bad_mx(const void* P, int64_t ldp, const void* S, int64_t lds, int64_t rows, int64_t cols, int bytes)
 {
     return !P || !S || (uintptr_t)P % 16 || (uintptr_t)S % 8 || ldp % 16 || lds % 8 ||
-           ldp < 16 * blocks(cols) || lds < 8 * rows;
+           ldp < bytes * blocks(cols) || lds < 8 * rows;
+}
+bool bad_mx4(const void* P, int64_t ldp, const void* S, int64_t lds, int64_t rows, int64_t cols)
+{
+    return bad_mx(P, ldp, S, lds, rows, cols, 16);
+}
+bool bad_mx8(const void* P, int64_t ldp, const void* S, int64_t lds, int64_t rows, int64_t cols)
+{
+    return bad_mx(P, ldp, S, lds, rows, cols, 32);
 }
 
 int dropout_args(DropoutArgs* a, const void* X, int64_t ldx, const void* gate, int64_t ldg,
@@ -53,6 +66,8 @@ int dropout_args(DropoutArgs* a, const void* X, int64_t ldx, const void* gate, i
     a->scale = a->threshold < 65536 ? 65536.0 / (65536 - a->threshold) : 0.0;
     return SBX_OK;
 }
+
+bool bad_eps(double eps) { return !(eps >= 0.0) || isinf(eps); }
 
 int status_of(hipError_t e)
 {
@@ -155,6 +170,156 @@ int sbx_mx4_gemm(void* stream, int dtype, int layout, int64_t m, int64_t n, int6
         a.m = (int)n; a.n = (int)m;
     }
     return sbx::status_of(sbx::launch_mx4_gemm(dtype, a, (hipStream_t)stream));
+}
+
+int sbx_rms_norm(void* stream, int dtype, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                 const void* R, int64_t ldr, const void* W, double eps, void* H, int64_t ldh, void* Y,
+                 int64_t ldy, void* P, int64_t ldp, void* S, int64_t lds)
+{
+    if (stream == (void*)-1) return SBX_INVALID_ARGUMENT;
+    if (!sbx::is_dtype(dtype, false)) return SBX_UNSUPPORTED;
+    if (rows < 0 || cols < 0) return SBX_INVALID_ARGUMENT;
+    if (rows > sbx::kMaxSide || cols > sbx::kMaxSide) return SBX_UNSUPPORTED;
+    if (rows == 0 || cols == 0) return SBX_OK;
+    const size_t elem = sbx::elem_size(dtype);
+    if (sbx::bad_eps(eps) || sbx::bad_dense(X, cols, ldx, elem) || sbx::bad_dense(W, cols, cols, elem))
+        return SBX_INVALID_ARGUMENT;
+    if (R && sbx::bad_dense(R, cols, ldr, elem)) return SBX_INVALID_ARGUMENT;
+    if (H && sbx::bad_dense(H, cols, ldh, elem)) return SBX_INVALID_ARGUMENT;
+    if (Y && sbx::bad_dense(Y, cols, ldy, elem)) return SBX_INVALID_ARGUMENT;
+    const bool mx = P || S;
+    if (mx && sbx::bad_mx8(P, ldp, S, lds, rows, cols)) return SBX_INVALID_ARGUMENT;
+    if (!H && !Y && !mx) return SBX_INVALID_ARGUMENT;
+    sbx::NormArgs a;
+    a.rows = rows; a.cols = cols;
+    a.X = X; a.ldx = ldx; a.R = R; a.ldr = ldr; a.W = W; a.eps = eps;
+    a.H = H; a.ldh = ldh; a.Y = Y; a.ldy = ldy;
+    a.q = sbx::Mx4Out{(uint8_t*)P, ldp, (uint8_t*)S, lds};
+    return sbx::status_of(sbx::launch_rms_norm(dtype, a, (hipStream_t)stream));
+}
+
+size_t sbx_rms_norm_grad_workspace(int64_t rows, int64_t cols)
+{
+    if (rows < 0 || cols < 0 || rows > sbx::kMaxSide || cols > sbx::kMaxSide) return 0;
+    return (size_t)sbx::norm_grad_parts(rows) * cols * sizeof(float);
+}
+
+int sbx_rms_norm_grad(void* stream, int dtype, int64_t rows, int64_t cols, const void* H, int64_t ldh,
+                      const void* W, double eps, const void* DY, int64_t lddy, const void* DR,
+                      int64_t lddr, void* DX, int64_t lddx, float* DW, void* workspace,
+                      size_t workspace_bytes)
+{
+    if (stream == (void*)-1) return SBX_INVALID_ARGUMENT;
+    if (!sbx::is_dtype(dtype, false)) return SBX_UNSUPPORTED;
+    if (rows < 0 || cols < 0) return SBX_INVALID_ARGUMENT;
+    if (rows > sbx::kMaxSide || cols > sbx::kMaxSide) return SBX_UNSUPPORTED;
+    if (cols == 0 || (rows == 0 && !DW)) return SBX_OK;
+    const size_t elem = sbx::elem_size(dtype);
+    if (rows > 0) {
+        if (sbx::bad_eps(eps) || sbx::bad_dense(H, cols, ldh, elem) || sbx::bad_dense(W, cols, cols, elem) ||
+            sbx::bad_dense(DY, cols, lddy, elem) || sbx::bad_dense(DX, cols, lddx, elem))
+            return SBX_INVALID_ARGUMENT;
+        if (DR && sbx::bad_dense(DR, cols, lddr, elem)) return SBX_INVALID_ARGUMENT;
+    }
+    if (DW) {
+        if ((uintptr_t)DW % 4) return SBX_INVALID_ARGUMENT;
+        if (rows > 0 && (!workspace || (uintptr_t)workspace % 16 ||
+                         workspace_bytes < sbx_rms_norm_grad_workspace(rows, cols)))
+            return SBX_INVALID_ARGUMENT;
+    }
+    sbx::NormGradArgs a;
+    a.rows = rows; a.cols = cols;
+    a.H = H; a.ldh = ldh; a.W = W; a.eps = eps; a.DY = DY; a.lddy = lddy; a.DR = DR; a.lddr = lddr;
+    a.DX = DX; a.lddx = lddx; a.DW = DW; a.part = (float*)workspace;
+    return sbx::status_of(sbx::launch_rms_norm_grad(dtype, a, (hipStream_t)stream));
+}
+
+int sbx_mx8_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* P,
+                       int64_t ldp, const void* S, int64_t lds, void* Y, int64_t ldy)
+{
+    if (stream == (void*)-1) return SBX_INVALID_ARGUMENT;
+    if (!sbx::is_dtype(dtype, false)) return SBX_UNSUPPORTED;
+    if (rows < 0 || cols < 0) return SBX_INVALID_ARGUMENT;
+    if (rows > sbx::kMaxSide || cols > sbx::kMaxSide) return SBX_UNSUPPORTED;
+    if (rows == 0 || cols == 0) return SBX_OK;
+    if (sbx::bad_mx8(P, ldp, S, lds, rows, cols)) return SBX_INVALID_ARGUMENT;
+    if (sbx::bad_dense(Y, cols, ldy, sbx::elem_size(dtype))) return SBX_INVALID_ARGUMENT;
+    return sbx::status_of(sbx::launch_mx8_dequantize(dtype, rows, cols, (const uint8_t*)P, ldp,
+                                                     (const uint8_t*)S, lds, Y, ldy,
+                                                     (hipStream_t)stream));
+}
+
+int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, float alpha,
+                   const void* X, int64_t ldx, const void* SX, int64_t ldsx, const void* B,
+                   int64_t ldb, const void* SB, int64_t ldsb, float beta, void* Y, int64_t ldy,
+                   int epilogue)
+{
+    if (stream == (void*)-1) return SBX_INVALID_ARGUMENT;
+    if (!sbx::is_dtype(dtype, false)) return SBX_UNSUPPORTED;
+    if (epilogue != SBX_EPILOGUE_NONE && epilogue != SBX_EPILOGUE_RELU) return SBX_INVALID_ARGUMENT;
+    if (m < 0 || n < 0 || k < 0) return SBX_INVALID_ARGUMENT;
+    if (m > sbx::kMaxLinearRows || n > sbx::kMaxSide || k > sbx::kMaxTerms) return SBX_UNSUPPORTED;
+    if (m == 0 || n == 0) return SBX_OK;
+    const size_t elem = sbx::elem_size(dtype);
+    if (sbx::bad_dense(Y, n, ldy, elem)) return SBX_INVALID_ARGUMENT;
+    if (alpha == 0.0f) k = 0;  // X and B are not read
+    if (k > 0) {
+        if (SX ? sbx::bad_mx8(X, ldx, SX, ldsx, m, k) : sbx::bad_dense(X, k, ldx, elem))
+            return SBX_INVALID_ARGUMENT;
+        if (sbx::bad_mx4(B, ldb, SB, ldsb, n, k)) return SBX_INVALID_ARGUMENT;
+        if (ldb > sbx::kMaxRowBytes || (SX && ldx > 2 * sbx::kMaxRowBytes)) return SBX_UNSUPPORTED;
+    }
+    sbx::Mx4LinearArgs a;
+    a.m = (int)m; a.n = (int)n; a.k = (int)k;
+    a.X = X; a.ldx = ldx; a.SX = (const uint8_t*)SX; a.ldsx = ldsx;
+    a.B = (const uint8_t*)B; a.ldb = ldb; a.SB = (const uint8_t*)SB; a.ldsb = ldsb;
+    a.Y = Y; a.ldy = ldy;
+    a.alpha = alpha; a.beta = beta;
+    a.relu = epilogue == SBX_EPILOGUE_RELU;
+    return sbx::status_of(sbx::launch_mx4_linear(dtype, a, (hipStream_t)stream));
+}
+
+size_t sbx_mx4_moe_workspace(int64_t tokens, int64_t width, int64_t hidden, int64_t experts, int64_t topk)
+{
+    if (tokens < 0 || width < 1 || hidden < 1 || experts < 1 || topk < 1 || topk > experts ||
+        tokens > sbx::kMaxTokens || width > sbx::kMaxLayer || hidden > sbx::kMaxLayer ||
+        experts > sbx::kMaxExperts || topk > sbx::kMaxTopk)
+        return 0;
+    return sbx::mx4_moe_work(tokens, hidden, experts, topk).bytes;
+}
+
+int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,
+                int64_t experts, int64_t topk, const void* X, int64_t ldx, const void* WR,
+                int64_t ldwr, int normalize, const void* W1, int64_t ld1, const void* S1,
+                int64_t lds1, const void* W2, int64_t ld2, const void* S2, int64_t lds2, void* Y,
+                int64_t ldy, int32_t* chosen, float* weights, void* workspace,
+                size_t workspace_bytes)
+{
+    if (stream == (void*)-1) return SBX_INVALID_ARGUMENT;
+    if (!sbx::is_dtype(dtype, false)) return SBX_UNSUPPORTED;
+    if (tokens < 0 || width < 1 || hidden < 1 || experts < 1 || topk < 1 || topk > experts)
+        return SBX_INVALID_ARGUMENT;
+    if (tokens > sbx::kMaxTokens || width > sbx::kMaxLayer || hidden > sbx::kMaxLayer ||
+        experts > sbx::kMaxExperts || topk > sbx::kMaxTopk)
+        return SBX_UNSUPPORTED;
+    if (tokens == 0) return SBX_OK;
+    const size_t elem = sbx::elem_size(dtype);
+    if (sbx::bad_dense(X, width, ldx, elem) || sbx::bad_dense(WR, width, ldwr, elem) ||
+        sbx::bad_dense(Y, width, ldy, elem) || sbx::bad_mx4(W1, ld1, S1, lds1, experts * 2 * hidden, width) ||
+        sbx::bad_mx4(W2, ld2, S2, lds2, experts * width, hidden))
+        return SBX_INVALID_ARGUMENT;
+    if ((uintptr_t)chosen % 4 || (uintptr_t)weights % 4 || !workspace || (uintptr_t)workspace % 16 ||
+        workspace_bytes < sbx_mx4_moe_workspace(tokens, width, hidden, experts, topk))
+        return SBX_INVALID_ARGUMENT;
+    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes) return SBX_UNSUPPORTED;
+    sbx::Mx4MoeArgs a;
+    a.tokens = (int)tokens; a.width = (int)width; a.hidden = (int)hidden;
+    a.experts = (int)experts; a.topk = (int)topk;
+    a.X = X; a.ldx = ldx; a.WR = WR; a.ldwr = ldwr; a.normalize = normalize != 0;
+    a.W1 = (const uint8_t*)W1; a.ld1 = ld1; a.S1 = (const uint8_t*)S1; a.lds1 = lds1;
+    a.W2 = (const uint8_t*)W2; a.ld2 = ld2; a.S2 = (const uint8_t*)S2; a.lds2 = lds2;
+    a.Y = Y; a.ldy = ldy; a.chosen = chosen; a.weights = weights; a.work = (uint8_t*)workspace;
+    return sbx::status_of(sbx::launch_mx4_moe(dtype, a, (hipStream_t)stream));
 }
 
 }  // extern "C"
