@@ -31,11 +31,12 @@ struct NormGradArgs {
     void* DX;
     int64_t lddx;
     float* DW;    // null: not wanted
-    float* part;  // with DW: norm_grad_parts(rows) x cols
+    float* part;  // with DW: up to norm_grad_parts(rows) x cols
 };
 
-// Groups of rows whose share of DW is summed apart.
-inline int norm_grad_parts(int64_t rows) { return rows < 256 ? (int)rows : 256; }
+// Groups of rows whose share of DW is summed apart: at most.
+constexpr int kNormGradParts = 256;
+inline int norm_grad_parts(int64_t rows) { return rows < kNormGradParts ? (int)rows : kNormGradParts; }
 
 struct Mx4LinearArgs {
     int m, n, k;
