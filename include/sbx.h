@@ -335,11 +335,12 @@ int sbx_mx8_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, cons
 
 /* Y = epilogue(alpha * X * B^T + beta * Y) for a few rows: X (m x k) keeps its type
  * (SX NULL) or is an MXFP8 matrix (X, SX), B (n x k) is an MXFP4 matrix, Y (m x n) of
- * dtype.  X is not rounded; sums are held in 32 bits and rounded to dtype once.  What
- * lies past the k-th term is not used.  BLAS semantics as for GEMM (beta == 0: Y is
+ * dtype.  X is not rounded (but for bits of fp32 values below 2^-133, which do not
+ * count); sums are held in 32 bits and rounded to dtype once.  What lies past the
+ * k-th term is not used.  BLAS semantics as for GEMM (beta == 0: Y is
  * not read; alpha == 0 or k == 0: X and B are not).  Rows are computed apart: those of
  * one call have the bits that they have alone.  m <= 1024, n <= 2^30, k <= 2^23, ldb <
- * 2^23 - 15, with SX ldx < 2^24 - 31 (else SBX_UNSUPPORTED). */
+ * 2^23 - 15, a row of X (ldx) at most 2^26 bytes (else SBX_UNSUPPORTED). */
 int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, float alpha,
                    const void* X, int64_t ldx, const void* SX, int64_t ldsx, const void* B,
                    int64_t ldb, const void* SB, int64_t ldsb, float beta, void* Y, int64_t ldy,
@@ -352,12 +353,13 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  *   y = sum_j p_j * W2_e (silu(G_e x) * (U_e x)),  silu(z) = z / (1 + exp(-z)),  e the j-th expert
  * W1, S1: an MXFP4 matrix of experts * 2 * hidden rows over width, expert e's G at rows
  * e * 2 * hidden, its U hidden rows later.  W2, S2: of experts * width rows over hidden.
- * Activations are not rounded before W1's product; before W2's they are held as the sum of
- * two bf16 values (F32: three), 16 bits (24) where dtype has 8 or 11.  Sums are held in
+ * Activations are not rounded before W1's product (but for bits of fp32 values below 2^-133);
+ * before W2's they are held as the sum of two bf16 values (F32: three), 16 bits (24) where
+ * dtype has 8 or 11.  Sums are held in
  * 32 bits and rounded to dtype once.
  * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.
- * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^20, ld1, ld2 <
- * 2^23 - 15 (else SBX_UNSUPPORTED). */
+ * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^20, ld1, ld2 < 2^23 -
+ * 15, a row of X (ldx) less than 2^23 - 15 bytes (else SBX_UNSUPPORTED). */
 int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,
                 int64_t experts, int64_t topk, const void* X, int64_t ldx, const void* WR,
                 int64_t ldwr, int normalize, const void* W1, int64_t ld1, const void* S1,

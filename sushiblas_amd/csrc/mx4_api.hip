@@ -19,7 +19,9 @@ constexpr int64_t kMaxRowBytes = ((int64_t)1 << 23) - 16;
 // what a mixture of experts takes: few tokens, and choices that fit its kernels' tables
 // (the rows of all experts together are within kMaxSide then)
 constexpr int64_t kMaxTokens = 256, kMaxExperts = 512, kMaxTopk = 16, kMaxLayer = (int64_t)1 << 20;
+constexpr int64_t kMaxMoeTokenBytes = ((int64_t)1 << 23) - 16;  // of a row of X: 256 rows stay within 32-bit offsets
 constexpr int64_t kMaxLinearRows = 1024;
+constexpr int64_t kMaxTokenBytes = (int64_t)1 << 26;  // of a row of X: 16 rows stay within 32-bit offsets
 
 int64_t blocks(int64_t k) { return (k + 31) / 32; }
 
@@ -267,7 +269,7 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
         if (SX ? sbx::bad_mx8(X, ldx, SX, ldsx, m, k) : sbx::bad_dense(X, k, ldx, elem))
             return SBX_INVALID_ARGUMENT;
         if (sbx::bad_mx4(B, ldb, SB, ldsb, n, k)) return SBX_INVALID_ARGUMENT;
-        if (ldb > sbx::kMaxRowBytes || (SX && ldx > 2 * sbx::kMaxRowBytes)) return SBX_UNSUPPORTED;
+        if (ldb > sbx::kMaxRowBytes || ldx * (SX ? 1 : (int64_t)elem) > sbx::kMaxTokenBytes) return SBX_UNSUPPORTED;
     }
     sbx::Mx4LinearArgs a;
     a.m = (int)m; a.n = (int)n; a.k = (int)k;
@@ -311,7 +313,8 @@ int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t 
     if ((uintptr_t)chosen % 4 || (uintptr_t)weights % 4 || !workspace || (uintptr_t)workspace % 16 ||
         workspace_bytes < sbx_mx4_moe_workspace(tokens, width, hidden, experts, topk))
         return SBX_INVALID_ARGUMENT;
-    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes) return SBX_UNSUPPORTED;
+    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes || ldx * (int64_t)elem > sbx::kMaxMoeTokenBytes)
+        return SBX_UNSUPPORTED;
     sbx::Mx4MoeArgs a;
     a.tokens = (int)tokens; a.width = (int)width; a.hidden = (int)hidden;
     a.experts = (int)experts; a.topk = (int)topk;

@@ -1,0 +1,343 @@
+// mx4_rows.hpp -- products of rows of an MXFP4 matrix with a few tokens whose values keep their
+// type or are MXFP8, a group of 256 terms at a time, by single waves.
+//
+// Both operands go to the bf16 matrix cores.  An MXFP4 or MXFP8 value is a bf16 one, its block's
+// code included, whatever the code (elements have 2 and 4 bits, and bf16 fp32's exponents); dense
+// values are exact sums of bf16 pieces: bf16 as they are, fp16 as 2 (8 and 3 bits), fp32 as 3 (8
+// each).  So products are exact (down to 2^-133 where bf16 ends), and sums are held in fp32.  The
+// scaled 4- and 8-bit instruction would take an eighth of the time, but it aligns the 128 terms of
+// a product to their largest, and drops what lies some 2^-14 below: blocks with small scales beside
+// one with a large one (1000 terms with codes 2^50 apart: off by 5e-5 of the result).
+//
+// v_mfma_f32_16x16x32_bf16: lane l holds terms 8 (l / 16) .. + 7 of row l % 16 of each operand; its
+// result has row 4 * (l / 16) + e of the first operand and row l % 16 of the second at register e.
+//
+// Neighbouring lanes of a fragment are different rows, and a CU's load unit takes a cycle for each
+// line that a quad of lanes meets: read straight from memory, fragments bound all of it (16 tokens x
+// 8192 x 8192: 17.4 us, of which the tokens' 7.4).  So a wave loads whole runs of rows, and turns
+// them round in LDS of its own; nothing there is shared, and no wave waits for another.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "layer.hpp"
+#include "mx4_group.hpp"
+#include "mx4_strip.hpp"
+#include "pieces.hpp"
+
+namespace sbx {
+
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* base, int bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, bytes, kRsrcWord3);
+}
+
+// The scale that a conversion takes for a code: its exponent field is what counts (0: 2^-127, 255: NaN).
+__device__ inline float scale_of_code(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
+
+// ---- rows of MXFP4 ----
+
+// 256 terms of 16 N rows.  In registers as loaded: 16 bytes (chunk lane % 8 of a row's 128) of rows
+// 8 i + lane / 8, and the 8 codes of rows 16 i + lane % 16.
+template <int N>
+struct Rows4 {
+    u32x4 v[2 * N];
+    u32x2 code[N];
+};
+
+template <int N>
+struct Source4 {
+    const uint8_t *rows, *codes;
+    int64_t lds;
+    int bytes, count, ld, at[2 * N], lane;
+
+    // Rows first .. (n in all), of nb blocks.
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int64_t first, int64_t n,
+                                int nb, int lane_)
+    {
+        count = (int)min(n - first, (int64_t)(16 * N));
+        ld = (int)ld_;
+        lds = lds_;
+        lane = lane_;
+        rows = P + first * ld_;
+        bytes = strip_bytes(count, ld, nb);
+        codes = S + 8 * first;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) {
+            const int row = 8 * i + lane / 8;
+            at[i] = row < count ? row * ld + lane % 8 * 16 : kOutside;
+        }
+    }
+
+    // Group g, `left` blocks up to the last: zeros, not from memory, past it and past the last row
+    // (a range check is certain to test the vector offset: mx4_strip.hpp).
+    __device__ inline void load(Rows4<N>& d, int g, int left) const
+    {
+        const __amdgpu_buffer_rsrc_t v = buffer_of(rows, bytes);
+        const __amdgpu_buffer_rsrc_t c = buffer_of(codes + g * lds, left > 0 ? 8 * count : 0);
+        const int from = left > 0 ? 128 * g : 0;
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i)
+            d.v[i] = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, lane % 8 < left ? at[i] : kOutside, from, 0));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            d.code[i] = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_raw_buffer_load_b64(c, lane % 16 * 8 + 128 * i, 0, 0));
+    }
+};
+
+// The codes of the first `left` blocks, 0 for the others (whose elements are zeros, and whose
+// codes may be NaN's).
+__device__ inline u32x2 first_codes(u32x2 code, int left)
+{
+    const uint32_t lo = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
+    const uint32_t hi = left >= 8 ? ~0u : left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
+    return u32x2{code[0] & lo, code[1] & hi};
+}
+
+// Four lanes' blocks for the matrix cores: word b of lane group q becomes word q of block b.
+__device__ inline u32x4 by_blocks(u32x4 v)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
+    auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    return u32x4{c[0], c[1], d[0], d[1]};
+}
+
+__device__ inline bf16x8 values4(uint32_t word, float scale)
+{
+    const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0),
+                 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1),
+                 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2),
+                 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+    return bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+
+// A wave's LDS for rows: 2 KiB for each 16.  Chunk c of row x lies at place c ^ (x / 2 % 8) of its
+// 128 bytes: LDS serves 16 bytes a lane to lanes 0-3, 12-15 and 20-27, then to the others of 0-31,
+// then to 32-63 likewise, and no two of such 16 meet in a bank.
+constexpr int rows4_bytes(int n) { return 2048 * n; }
+
+// The rows' values as fragments, a block of 32 terms each, through the wave's LDS.
+template <int N>
+__device__ inline void fragments(const Rows4<N>& d, char* lds, int lane, bf16x8 (&to)[N][8])
+{
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+        const int row = 8 * i + lane / 8;
+        *(u32x4*)(lds + row * 128 + (lane % 8 ^ row / 2 % 8) * 16) = d.v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row = 16 * i + lane % 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 w = by_blocks(*(const u32x4*)(lds + row * 128 + (4 * h + lane / 16 ^ row / 2 % 8) * 16));
+#pragma unroll
+            for (int b = 0; b < 4; ++b) to[i][4 * h + b] = values4(w[b], scale_of_code(d.code[i][h] >> 8 * b & 255));
+        }
+    }
+}
+
+// ---- tokens ----
+
+template <typename T>
+constexpr int kBf16Pieces = sizeof(T) == 4 ? 3 : std::is_same<T, f16_t>::value ? 2 : 1;
+
+// Eight values as bf16 pieces, the largest first.  An infinity's lower pieces are zeros.
+template <int N>
+__device__ inline void split(const float (&x)[8], bf16x8 (&to)[N])
+{
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        u32x4 w;  // the upper halves of two words
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, rest[2 * i + 1]),
+                                         __builtin_bit_cast(uint32_t, rest[2 * i]), 0x07060302);
+        to[n] = __builtin_bit_cast(bf16x8, w);
+        if (n + 1 == N) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float top = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xffff0000);
+            const float left = rest[i] - top;
+            rest[i] = n == 0 && __builtin_isinf(x[i]) ? 0.0f : left;
+        }
+    }
+}
+
+// 256 terms of a tile of TOKENS (2, 8 or 16) tokens: a lane loads 8 terms, 8 (lane % 32) .., of tokens
+// 2 i + lane / 32, makes their pieces, and writes them to the wave's LDS.  Chunk c (8 terms) of
+// token t lies at place c ^ t of its 512 bytes, for the same reason as above.
+constexpr int tokens_bytes(int pieces, int tokens) { return 512 * pieces * tokens; }
+
+template <int PIECES, int TOKENS>
+__device__ inline void put_tokens(char* lds, int i, int lane, const bf16x8 (&x)[PIECES])
+{
+    const int t = 2 * i + lane / 32;
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+        *(bf16x8*)(lds + (n * TOKENS + t) * 512 + (lane % 32 ^ t) * 16) = x[n];
+}
+
+// A block's fragment: token lane % 16 of the tile (those past a smaller tile: again from its first).
+template <int PIECES, int TOKENS>
+__device__ inline void get_tokens(const char* lds, int b, int lane, bf16x8 (&x)[PIECES])
+{
+    const int t = lane % TOKENS;
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+        x[n] = *(const bf16x8*)(lds + (n * TOKENS + t) * 512 + (4 * b + lane / 16 ^ t) * 16);
+}
+
+// Tokens of type T: rows anywhere within 2 GiB.
+template <typename T, int TOKENS>
+struct DenseTokens {
+    static constexpr int PIECES = kBf16Pieces<T>, PER = 8 * sizeof(T) / 16, LOADS = TOKENS / 2;
+    struct Values {
+        Piece<T> v[LOADS][PER];
+    };
+    const T* base;
+    int bytes, at[LOADS];
+
+    // Token t of the tile lies offset_of(t) bytes from base, or is not there (kOutside); `bytes` to the last one's end.
+    template <typename F>
+    __device__ inline void init(const T* base_, int bytes_, F&& offset_of, int lane)
+    {
+        base = base_;
+        bytes = bytes_;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int from = offset_of(2 * i + lane / 32);
+            at[i] = from == kOutside ? kOutside : from + lane % 32 * (int)(8 * sizeof(T));
+        }
+    }
+    // Group g, all of it before the rows' end.
+    __device__ inline void load(Values& d, int g) const
+    {
+        const __amdgpu_buffer_rsrc_t v = buffer_of((const uint8_t*)base, bytes);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+            for (int p = 0; p < PER; ++p)
+                d.v[i][p] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(
+                                                             v, at[i] + 16 * p, g * (int)(256 * sizeof(T)), 0));
+    }
+    // The group with the rows' end, at term k: zeros from there on (a token that is not there: any).
+    template <Cut CUT>
+    __device__ inline void load_end(Values& d, int g, int k, int lane) const
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int c0 = lane % 32 * 8, from = at[i] == kOutside ? 0 : at[i] - c0 * (int)sizeof(T);
+            const T* row = (const T*)((const char*)base + from);
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                const int c = 256 * g + c0 + Piece<T>::N * p;
+                d.v[i][p] = load_piece<CUT>(row, c, k);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+            for (int p = 0; p < PER; ++p) trim_piece<CUT>(d.v[i][p], 256 * g + lane % 32 * 8 + Piece<T>::N * p, k);
+    }
+    __device__ inline void put(const Values& d, char* lds, int lane) const
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            bf16x8 x[PIECES];
+            if constexpr (PIECES == 1)
+                x[0] = __builtin_bit_cast(bf16x8, d.v[i][0]);
+            else {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = (float)d.v[i][e / Piece<T>::N].v[e % Piece<T>::N];
+                split(f, x);
+            }
+            put_tokens<PIECES, TOKENS>(lds, i, lane, x);
+        }
+    }
+};
+
+// Tokens that are rows of an MXFP8 matrix.
+template <int TOKENS>
+struct Mx8Tokens {
+    static constexpr int PIECES = 1, LOADS = TOKENS / 2;
+    struct Values {
+        u32x2 v[LOADS];
+        uint32_t code[LOADS];
+    };
+    const uint8_t *rows, *codes;
+    int64_t lds;
+    int bytes, count, ld;
+
+    // Rows first .. (n in all) of nb blocks.
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n, int nb)
+    {
+        count = min(n - first, TOKENS);
+        ld = (int)ld_;
+        lds = lds_;
+        rows = P + first * ld_;
+        bytes = (count - 1) * ld + 32 * nb;
+        codes = S + 8 * (int64_t)first;
+    }
+    // Group g, `left` blocks up to the last: zeros past it and past the last row.
+    __device__ inline void load(Values& d, int g, int left, int lane) const
+    {
+        const __amdgpu_buffer_rsrc_t v = buffer_of(rows, bytes);
+        const __amdgpu_buffer_rsrc_t c = buffer_of(codes + g * lds, left > 0 ? 8 * count : 0);
+        const int from = left > 0 ? 256 * g : 0, block = lane % 32 / 4;  // (counts inside alone: mx4_strip.hpp)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int t = 2 * i + lane / 32;
+            const bool inside = t < count && block < left;
+            d.v[i] = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_raw_buffer_load_b64(v, inside ? t * ld + lane % 32 * 8 : kOutside, from, 0));
+            d.code[i] = __builtin_amdgcn_raw_buffer_load_b8(c, inside ? 8 * t + block : kOutside, 0, 0);
+        }
+    }
+    __device__ inline void put(const Values& d, char* lds_, int lane) const
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const float scale = scale_of_code(d.code[i] & 255);
+            const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d.v[i][0], scale, false),
+                         v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d.v[i][0], scale, true),
+                         v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d.v[i][1], scale, false),
+                         v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d.v[i][1], scale, true);
+            const bf16x8 x[1] = {bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]}};
+            put_tokens<1, TOKENS>(lds_, i, lane, x);
+        }
+    }
+};
+
+// acc[i]: rows 4 (lane / 16) + e of block i of w, token lane % 16 of the tile in the wave's LDS.
+template <int PIECES, int TOKENS, int N>
+__device__ inline void multiply(f32x4 (&acc)[N], const bf16x8 (&w)[N][8], const char* lds, int lane)
+{
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        bf16x8 x[PIECES];
+        get_tokens<PIECES, TOKENS>(lds, b, lane, x);
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][b], x[n], acc[i], 0, 0, 0);
+    }
+}
+
+}  // namespace sbx

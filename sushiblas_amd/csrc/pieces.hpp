@@ -25,10 +25,16 @@ __device__ inline Piece<T> load_piece(const T* row, int c, int cols)
 {
     constexpr int N = Piece<T>::N;
     if constexpr (CUT == Cut::Short) {
-        Piece<T> y;
+        u32x4 y = {};
 #pragma unroll
-        for (int i = 0; i < N; ++i) y.v[i] = c + i < cols ? row[c + i] : (T)0;
-        return y;
+        for (int i = 0; i < N; ++i)
+            if (c + i < cols) {
+                if constexpr (sizeof(T) == 2)
+                    y[i / 2] |= (uint32_t)((const uint16_t*)row)[c + i] << i % 2 * 16;
+                else
+                    y[i] = ((const uint32_t*)row)[c + i];
+            }
+        return __builtin_bit_cast(Piece<T>, y);
     }
     return *(const Piece<T>*)(row + (c + N <= cols ? c : cols - N));
 }

@@ -3,7 +3,8 @@
 Where x are small whole numbers and codes lie within 2 of each other, terms are multiples of one
 quantum and fewer than 2^24 of it in sum, so results are equal after the one rounding to their
 type whatever the order of the sums.  Elsewhere a sum of k terms in 32 bits is off by at most
-(k + 4) 2^-24 of its terms' magnitudes, and rounded to its type once."""
+(k + 4) 2^-24 of its terms' magnitudes, and rounded to its type once.  fp32 values lose what lies
+below 2^-133, less than 2^-133 of each, which counts times the weight's magnitude."""
 import numpy as np
 import pytest
 
@@ -53,6 +54,8 @@ def _run(cuda, name, m, n, k, alpha=1.0, beta=0.0, relu=False, mx8=False, pads=(
     with np.errstate(invalid="ignore", over="ignore"):
         want = alpha * (x @ w.T) + (beta * y0 if beta != 0 else 0.0)
         bound = (k + 4) * 2.0 ** -24 * (abs(alpha) * (np.abs(x) @ np.abs(w).T) + np.abs(beta * y0))
+        if name == "f32" and not mx8:
+            bound = bound + abs(alpha) * 2.0 ** -133 * np.abs(w).sum(1)
     if relu:
         want = np.where(want > 0, want, 0.0)
     got = ref.f64(Y)
