@@ -9,8 +9,6 @@
 namespace sbx {
 namespace {
 
-constexpr int kWaves = 8;
-
 template <typename T>
 __device__ inline T result(float acc, float y, const Mx4LinearArgs& p)
 {
@@ -18,22 +16,28 @@ __device__ inline T result(float acc, float y, const Mx4LinearArgs& p)
     return (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
 }
 
-// A workgroup takes 16 XB rows of B and YB tiles of TOKENS rows of X, its eight waves each an eighth
-// of the terms, in groups of 256 by turns: two groups of B are under way beside the one at work, and
-// a tile of X.  The waves' sums are added up in LDS, in order.  Which wave has a term does not
-// depend on m, so a row's bits do not either.
-template <typename T, bool MX8, int TOKENS, int YB, int XB>
-__global__ void __launch_bounds__(64 * kWaves, 2) linear_kernel(Mx4LinearArgs p)
+// A workgroup takes 16 XB rows of B and YB tiles of TOKENS rows of X, its waves a share each of the
+// terms, in groups of 256 by turns; AHEAD groups of B are under way, and of X (of a larger tile than
+// 2 rows the next one alone, for want of registers).  The waves' sums are added up in LDS, in order.
+// Which wave has a term does not depend on m, so a row's bits do not either.
+//   One token is bound by memory: bf16 1 x 28672 x 8192 26.5 us (125 MB, 4.7 TB/s; the product of
+// MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 10.7 (36 MB: 2.6 of it are any kernel's, then the first
+// loads' way, and there is one round).  Four groups ahead in place of two 11.4, blocks that follow one
+// another to a wave in place of turns 11.2 against 11.4.  More tokens are bound by X's way from the
+// L2s, as each workgroup reads all of it: 16 x 28672 x 8192 38 us, loads alone as long (64 rows of B a
+// workgroup take too many registers: 79).
+template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 {
     typedef typename std::conditional<MX8, Mx8Tokens<TOKENS>, DenseTokens<T, TOKENS>>::type tokens_t;
-    constexpr int PIECES = tokens_t::PIECES, PITCH = 16 * YB + 4;
+    constexpr int PIECES = tokens_t::PIECES, PITCH = 16 * YB + 4, AHEAD = 2, AHEAD_X = TOKENS == 2 ? AHEAD : 1;
     constexpr int OWN = rows4_bytes(XB) + tokens_bytes(PIECES, TOKENS), PART = 16 * PITCH * 4;
-    __shared__ __align__(16) char lds[kWaves * (OWN > PART ? OWN : PART)];
+    __shared__ __align__(16) char lds[WAVES * (OWN > PART ? OWN : PART)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int x0 = block_x() * (16 * XB), y0 = blockIdx.y * (TOKENS * YB);
     if (x0 >= p.n) return;
     char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(XB);
-    const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8, whole = MX8 ? groups : p.k / 256;
+    const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
     Source4<XB> sw;
     sw.init(p.B, p.ldb, p.SB, p.ldsb, x0, p.n, nb, lane);
     tokens_t sa[YB];
@@ -44,54 +48,39 @@ __global__ void __launch_bounds__(64 * kWaves, 2) linear_kernel(Mx4LinearArgs p)
             sa[j].init((const uint8_t*)p.X, p.ldx, p.SX, p.ldsx, first, p.m, nb);
         else {
             const int ld = (int)(p.ldx * sizeof(T)), count = min(p.m - first, TOKENS);
-            sa[j].init((const T*)p.X + first * p.ldx, (count - 1) * ld + p.k * (int)sizeof(T),
+            sa[j].init((const T*)p.X + first * p.ldx, (count - 1) * ld + p.k * (int)sizeof(T), p.k,
                        [&](int t) { return t < count ? t * ld : kOutside; }, lane);
         }
     }
 
     f32x4 acc[YB][XB] = {};
-    Rows4<XB> w0, w1;
-    typename tokens_t::Values a;
-    auto load_tokens = [&](int j, int g) {  // (a group past the last: the last whole one, not used)
-        if constexpr (MX8)
-            sa[j].load(a, g, nb - 8 * g, lane);
-        else
-            sa[j].load(a, min(g, whole - 1));
-    };
-    auto use = [&](Rows4<XB>& w, int g, bool end) {
-        if (nb - 8 * g < 8)
+    Rows4<XB> w[AHEAD];
+    typename tokens_t::Values a[AHEAD_X];
+    // (no branch around a load, and one past the last group reads zeros or the last group again: the
+    // compiler would wait for all of them where paths meet)
 #pragma unroll
-            for (int i = 0; i < XB; ++i) w.code[i] = first_codes(w.code[i], nb - 8 * g);
-        bf16x8 v[XB][8];
-        fragments(w, own, lane, v);
-        sw.load(w, g + 2 * kWaves, nb - 8 * (g + 2 * kWaves));
-#pragma unroll
-        for (int j = 0; j < YB; ++j) {
-            if (end)
-                if constexpr (!MX8) {
-                    if (p.k >= Piece<T>::N)
-                        sa[j].template load_end<Cut::Ragged>(a, g, p.k, lane);
-                    else
-                        sa[j].template load_end<Cut::Short>(a, g, p.k, lane);
-                }
-            sa[j].put(a, tokens_at, lane);
-            if (!end) load_tokens(j + 1 < YB ? j + 1 : 0, j + 1 < YB ? g : g + kWaves);
-            multiply<PIECES, TOKENS>(acc[j], v, tokens_at, lane);
-        }
-    };
-    sw.load(w0, wave, nb - 8 * wave);
-    sw.load(w1, wave + kWaves, nb - 8 * (wave + kWaves));
-    int g = wave;
-    if (g < whole) {
-        load_tokens(0, g);
-        for (; g < whole; g += 2 * kWaves) {
-            use(w0, g, false);
-            if (g + kWaves < whole) use(w1, g + kWaves, false);
-        }
+    for (int d = 0; d < AHEAD; ++d) {
+        sw.load(w[d], wave + d * WAVES, nb - 8 * (wave + d * WAVES));
+        if (d < AHEAD_X) sa[0].load(a[d], wave + d * WAVES, lane);
     }
-    if (!MX8 && p.k % 256 && whole % kWaves == wave) {
-        Rows4<XB> w = whole / kWaves % 2 ? w1 : w0;
-        use(w, whole, true);
+    for (int g = wave; g < groups;) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+            bf16x8 v[XB][8];
+            if (nb - 8 * g < 8)
+#pragma unroll
+                for (int i = 0; i < XB; ++i) w[d].code[i] = first_codes(w[d].code[i], nb - 8 * g);
+            fragments(w[d], own, lane, v);
+            sw.load(w[d], g + AHEAD * WAVES, nb - 8 * (g + AHEAD * WAVES));
+#pragma unroll
+            for (int j = 0; j < YB; ++j) {
+                sa[j].put(a[d % AHEAD_X], tokens_at, g, lane);
+                sa[j + 1 < YB ? j + 1 : 0].load(a[d % AHEAD_X], j + 1 < YB ? g : g + AHEAD_X * WAVES, lane);
+                multiply<PIECES, TOKENS>(acc[j], v, tokens_at, lane);
+            }
+            g += WAVES;
+            if (g >= groups) break;
+        }
     }
 
     __syncthreads();
@@ -106,12 +95,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) linear_kernel(Mx4LinearArgs p)
 #pragma unroll
             for (int e = 0; e < 4; ++e) part[(wave * 16 + 4 * q + e) * PITCH + 16 * j + r] = acc[j][i][e];
         __syncthreads();
-        for (int t = threadIdx.x; t < 16 * TOKENS * YB; t += 64 * kWaves) {
+        for (int t = threadIdx.x; t < 16 * TOKENS * YB; t += 64 * WAVES) {
             const int dm = t / 16, n = x0 + 16 * i + t % 16, m = y0 + dm;
             if (n >= p.n || m >= p.m) continue;
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w)
+            for (int w = 0; w < WAVES; ++w)
                 v += part[(w * 16 + t % 16) * PITCH + dm / TOKENS * 16 + dm % TOKENS];
             T* y = Y + (int64_t)m * p.ldy + n;
             *y = result<T>(v, p.beta != 0.0f ? (float)*y : 0.0f, p);
@@ -119,15 +108,39 @@ __global__ void __launch_bounds__(64 * kWaves, 2) linear_kernel(Mx4LinearArgs p)
     }
 }
 
+// Fewer terms than a piece has, or none.  A thread to a result.
+template <typename T>
+__global__ void __launch_bounds__(256) few_terms_kernel(Mx4LinearArgs p)
+{
+    const int64_t n = (int64_t)block_x() * 256 + threadIdx.x;
+    if (n >= p.n) return;
+    const int m = blockIdx.y;
+    float sum = 0.0f;
+    if (p.k > 0) {
+        const float scale = scale_of_code(p.SB[8 * n]);
+        for (int c = 0; c < p.k; ++c)
+            sum += (float)((const T*)p.X)[m * p.ldx + c] *
+                   __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(p.B[n * p.ldb + c / 2] >> c % 2 * 4, scale, 0)[0];
+    }
+    T* y = (T*)p.Y + (int64_t)m * p.ldy + n;
+    *y = result<T>(sum, p.beta != 0.0f ? (float)*y : 0.0f, p);
+}
+
 template <typename T, bool MX8, int TOKENS, int YB>
 hipError_t launch_form(const Mx4LinearArgs& a, hipStream_t s)
 {
     const unsigned gy = (unsigned)((a.m + TOKENS * YB - 1) / (TOKENS * YB));
-    // two blocks of B's rows a workgroup, where that leaves one for each CU
-    if (a.n > 16 * 256)
-        linear_kernel<T, MX8, TOKENS, YB, 2><<<grid_of((a.n + 31) / 32, gy), 64 * kWaves, 0, s>>>(a);
-    else
-        linear_kernel<T, MX8, TOKENS, YB, 1><<<grid_of((a.n + 15) / 16, gy), 64 * kWaves, 0, s>>>(a);
+    if (a.n <= 16 * 256) {
+        // one block of B's rows a workgroup, of which a CU has one: eight waves (1 x 4096 x 16384 9.8 us, by
+        // four 12.2)
+        linear_kernel<T, MX8, TOKENS, YB, 1, 8><<<grid_of((a.n + 15) / 16, gy), 512, 0, s>>>(a);
+    } else {
+        // several workgroups to a CU, of four waves: one's loads go on while another adds up (1 x 28672
+        // x 8192 26.5 us, by eight 28.9).  Two blocks each (16 x 28672 x 8192 38 us, one 45), but for one
+        // token of one piece (28.7 against 26.5)
+        constexpr int XB = TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1) ? 1 : 2;
+        linear_kernel<T, MX8, TOKENS, YB, XB, 4><<<grid_of((a.n + 16 * XB - 1) / (16 * XB), gy), 256, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 
@@ -135,6 +148,10 @@ template <typename T, bool MX8>
 hipError_t launch(const Mx4LinearArgs& a, hipStream_t s)
 {
     constexpr int TOKENS = MX8 || kBf16Pieces<T> == 1 ? 16 : 8;  // (pieces of 16 would not fit the LDS)
+    if (a.k == 0 || (!MX8 && a.k < 8)) {
+        few_terms_kernel<T><<<grid_of((a.n + 255) / 256, (unsigned)a.m), 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
     if (a.m <= 2) return launch_form<T, MX8, 2, 1>(a, s);
     if (a.m <= TOKENS) return launch_form<T, MX8, TOKENS, 1>(a, s);
     if (a.m <= 2 * TOKENS) return launch_form<T, MX8, TOKENS, 2>(a, s);

@@ -210,52 +210,41 @@ struct DenseTokens {
         Piece<T> v[LOADS][PER];
     };
     const T* base;
-    int bytes, at[LOADS];
+    int bytes, k, at[LOADS];
 
-    // Token t of the tile lies offset_of(t) bytes from base, or is not there (kOutside); `bytes` to the last one's end.
+    // Token t of the tile lies offset_of(t) bytes from base, or is not there (kOutside); `bytes` to the
+    // last one's end.  k >= 8 terms.
     template <typename F>
-    __device__ inline void init(const T* base_, int bytes_, F&& offset_of, int lane)
+    __device__ inline void init(const T* base_, int bytes_, int k_, F&& offset_of, int lane)
     {
         base = base_;
         bytes = bytes_;
+        k = k_;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int from = offset_of(2 * i + lane / 32);
-            at[i] = from == kOutside ? kOutside : from + lane % 32 * (int)(8 * sizeof(T));
-        }
+        for (int i = 0; i < LOADS; ++i) at[i] = offset_of(2 * i + lane / 32);
     }
-    // Group g, all of it before the rows' end.
-    __device__ inline void load(Values& d, int g) const
+    // Group g.  A piece that reaches past the rows' end is read that much earlier (put moves it).
+    __device__ inline void load(Values& d, int g, int lane) const
     {
         const __amdgpu_buffer_rsrc_t v = buffer_of((const uint8_t*)base, bytes);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
+        for (int p = 0; p < PER; ++p) {
+            const int c = min(256 * g + lane % 32 * 8 + Piece<T>::N * p, k - Piece<T>::N) * (int)sizeof(T);
 #pragma unroll
-            for (int p = 0; p < PER; ++p)
-                d.v[i][p] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(
-                                                             v, at[i] + 16 * p, g * (int)(256 * sizeof(T)), 0));
-    }
-    // The group with the rows' end, at term k: zeros from there on (a token that is not there: any).
-    template <Cut CUT>
-    __device__ inline void load_end(Values& d, int g, int k, int lane) const
-    {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int c0 = lane % 32 * 8, from = at[i] == kOutside ? 0 : at[i] - c0 * (int)sizeof(T);
-            const T* row = (const T*)((const char*)base + from);
-#pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                const int c = 256 * g + c0 + Piece<T>::N * p;
-                d.v[i][p] = load_piece<CUT>(row, c, k);
-            }
+            for (int i = 0; i < LOADS; ++i)
+                d.v[i][p] = __builtin_bit_cast(
+                    Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(v, at[i] == kOutside ? kOutside : at[i] + c, 0, 0));
         }
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-            for (int p = 0; p < PER; ++p) trim_piece<CUT>(d.v[i][p], 256 * g + lane % 32 * 8 + Piece<T>::N * p, k);
     }
-    __device__ inline void put(const Values& d, char* lds, int lane) const
+    // To LDS.
+    __device__ inline void put(Values& d, char* lds, int g, int lane) const
     {
+        if (256 * g + 256 > k)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+                for (int p = 0; p < PER; ++p)
+                    trim_piece<Cut::Ragged>(d.v[i][p], 256 * g + lane % 32 * 8 + Piece<T>::N * p, k);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             bf16x8 x[PIECES];
@@ -282,11 +271,12 @@ struct Mx8Tokens {
     };
     const uint8_t *rows, *codes;
     int64_t lds;
-    int bytes, count, ld;
+    int bytes, count, ld, nb;
 
     // Rows first .. (n in all) of nb blocks.
-    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n, int nb)
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n, int nb_)
     {
+        nb = nb_;
         count = min(n - first, TOKENS);
         ld = (int)ld_;
         lds = lds_;
@@ -294,9 +284,10 @@ struct Mx8Tokens {
         bytes = (count - 1) * ld + 32 * nb;
         codes = S + 8 * (int64_t)first;
     }
-    // Group g, `left` blocks up to the last: zeros past it and past the last row.
-    __device__ inline void load(Values& d, int g, int left, int lane) const
+    // Group g: zeros past the last block and the last row.
+    __device__ inline void load(Values& d, int g, int lane) const
     {
+        const int left = nb - 8 * g;
         const __amdgpu_buffer_rsrc_t v = buffer_of(rows, bytes);
         const __amdgpu_buffer_rsrc_t c = buffer_of(codes + g * lds, left > 0 ? 8 * count : 0);
         const int from = left > 0 ? 256 * g : 0, block = lane % 32 / 4;  // (counts inside alone: mx4_strip.hpp)
@@ -309,7 +300,7 @@ struct Mx8Tokens {
             d.code[i] = __builtin_amdgcn_raw_buffer_load_b8(c, inside ? 8 * t + block : kOutside, 0, 0);
         }
     }
-    __device__ inline void put(const Values& d, char* lds_, int lane) const
+    __device__ inline void put(const Values& d, char* lds_, int, int lane) const
     {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
