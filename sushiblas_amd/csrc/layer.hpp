@@ -66,11 +66,25 @@ struct Mx4MoeArgs {
     uint8_t* work;
 };
 
+// A mixture is computed for 64 tokens at a time (kernels' z): tokens of other chunks share no tile.
+constexpr int kMoeChunk = 64;
+
 // A mixture's workspace: offsets of its parts, each 256-byte aligned.
 struct Mx4MoeWork {
-    size_t logits, chosen, weights, act, bytes;
+    size_t logits;           // tokens x experts, 64 bits
+    size_t chosen, weights;  // tokens x topk
+    size_t x, x_stride;      // tokens as bf16 pieces (up to 3, x_stride bytes apart), zeros to x_ld bytes
+    size_t act, act_stride;  // the hidden layer times its share, one row a choice, likewise
+    size_t tiles;            // of each chunk, tiles_bytes apart: what is below, in 32-bit words
+    size_t tiles_bytes, bytes;
+    int x_ld, act_ld;
 };
-inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t hidden, int64_t experts, int64_t topk)
+// A chunk's tiles: their numbers, of the first product and of the second; then their experts, first
+// places and counts; then the choices by place.
+constexpr int kMoeChoices = kMoeChunk * 16, kMoeTiles = kMoeChoices;
+constexpr int kMoeTileWords = 2 + 2 * 3 * kMoeTiles + kMoeChoices;
+
+inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t width, int64_t hidden, int64_t experts, int64_t topk)
 {
     Mx4MoeWork w;
     size_t at = 0;
@@ -79,10 +93,17 @@ inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t hidden, int64_t experts, 
         at += (bytes + 255) / 256 * 256;
         return from;
     };
+    w.x_ld = (int)((width + 255) / 256 * 512);
+    w.act_ld = (int)((hidden + 255) / 256 * 512);
     w.logits = take(8 * tokens * experts);
     w.chosen = take(4 * tokens * topk);
     w.weights = take(4 * tokens * topk);
-    w.act = take(4 * tokens * topk * hidden);
+    w.x_stride = (size_t)w.x_ld * tokens;
+    w.x = take(3 * w.x_stride);
+    w.act_stride = (size_t)w.act_ld * tokens * topk;
+    w.act = take(3 * w.act_stride);
+    w.tiles_bytes = 4 * kMoeTileWords;
+    w.tiles = take((tokens + kMoeChunk - 1) / kMoeChunk * w.tiles_bytes);
     w.bytes = at;
     return w;
 }

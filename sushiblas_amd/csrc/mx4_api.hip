@@ -18,7 +18,7 @@ constexpr int64_t kMaxTerms = (int64_t)1 << 23;
 constexpr int64_t kMaxRowBytes = ((int64_t)1 << 23) - 16;
 // what a mixture of experts takes: few tokens, and choices that fit its kernels' tables
 // (the rows of all experts together are within kMaxSide then)
-constexpr int64_t kMaxTokens = 256, kMaxExperts = 512, kMaxTopk = 16, kMaxLayer = (int64_t)1 << 20;
+constexpr int64_t kMaxTokens = 256, kMaxExperts = 512, kMaxTopk = 16, kMaxLayer = (int64_t)1 << 18;
 constexpr int64_t kMaxMoeTokenBytes = ((int64_t)1 << 23) - 16;  // of a row of X: 256 rows stay within 32-bit offsets
 constexpr int64_t kMaxLinearRows = 1024;
 constexpr int64_t kMaxTokenBytes = (int64_t)1 << 26;  // of a row of X: 16 rows stay within 32-bit offsets
@@ -287,7 +287,7 @@ size_t sbx_mx4_moe_workspace(int64_t tokens, int64_t width, int64_t hidden, int6
         tokens > sbx::kMaxTokens || width > sbx::kMaxLayer || hidden > sbx::kMaxLayer ||
         experts > sbx::kMaxExperts || topk > sbx::kMaxTopk)
         return 0;
-    return sbx::mx4_moe_work(tokens, hidden, experts, topk).bytes;
+    return sbx::mx4_moe_work(tokens, width, hidden, experts, topk).bytes;
 }
 
 int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,

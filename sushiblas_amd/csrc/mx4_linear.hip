@@ -39,7 +39,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
     char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(XB);
     const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8;
     Source4<XB> sw;
-    sw.init(p.B, p.ldb, p.SB, p.ldsb, x0, p.n, nb, lane);
+    sw.init(p.ldb, p.ldsb, p.n - x0, nb, lane);
+    sw.move(p.B, p.SB, x0);
     tokens_t sa[YB];
 #pragma unroll
     for (int j = 0; j < YB; ++j) {

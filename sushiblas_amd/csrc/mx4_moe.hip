@@ -1,112 +1,465 @@
 // mx4_moe.hip -- a mixture-of-experts layer for a few tokens, its experts' weights MXFP4
 // (layer.hpp).
+//
+// Kernels, each on what the one before wrote to the workspace:
+//   prepare  the router's logits, and the tokens as bf16 pieces
+//   choose   (more than one token) each token's experts and shares, the choices sorted by expert,
+//            in tiles of a few tokens of one expert
+//   up       a tile by 16 units of the hidden layer: share * silu(G x) * (U x), as bf16 pieces; of
+//            one token it chooses itself, which costs less than a launch
+//   down     16 results of all of a chunk's tokens: the sum over its tiles, which the waves share
+// Products and pieces: mx4_rows.hpp.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "layer.hpp"
+#include "mx4_rows.hpp"
 
 namespace sbx {
 namespace {
 
-__device__ inline double* logits_of(const Mx4MoeArgs& a, const Mx4MoeWork& w) { return (double*)(a.work + w.logits); }
-__device__ inline int* chosen_of(const Mx4MoeArgs& a, const Mx4MoeWork& w) { return (int*)(a.work + w.chosen); }
-__device__ inline float* weights_of(const Mx4MoeArgs& a, const Mx4MoeWork& w) { return (float*)(a.work + w.weights); }
-__device__ inline float* act_of(const Mx4MoeArgs& a, const Mx4MoeWork& w) { return (float*)(a.work + w.act); }
+// ---- the router ----
 
-// Logits in 64 bits, so that which experts are chosen does not depend on the order of the sums.
+// Pieces that an activation is held in before the second product: of fp32 all of its bits, else 16.
 template <typename T>
-__global__ void __launch_bounds__(64) logits_kernel(Mx4MoeArgs a, Mx4MoeWork w)
-{
-    const int e = blockIdx.x, t = blockIdx.y;
-    double sum = 0.0;
-    for (int c = threadIdx.x; c < a.width; c += 64)
-        sum += (double)(float)((const T*)a.X)[t * a.ldx + c] * (double)(float)((const T*)a.WR)[e * a.ldwr + c];
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-    if (threadIdx.x == 0) logits_of(a, w)[(int64_t)t * a.experts + e] = sum;
-}
+constexpr int kActPieces = sizeof(T) == 4 ? 3 : 2;
 
-// Whether logit x of expert i comes before y of j: the higher one, NaN highest, ties by index.
-__device__ inline bool before(double x, int i, double y, int j)
-{
-    const bool nx = x != x, ny = y != y;
-    if (nx != ny) return nx;
-    return !nx && x != y ? x > y : i < j;
-}
-
-__global__ void __launch_bounds__(64) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w)
-{
-    const int t = blockIdx.x * 64 + threadIdx.x;
-    if (t >= a.tokens) return;
-    const double* l = logits_of(a, w) + (int64_t)t * a.experts;
-    int* chosen = chosen_of(a, w) + t * a.topk;
-    double top = 0.0, last = 0.0, sum = 0.0;
-    int last_e = -1;
-    for (int j = 0; j < a.topk; ++j) {
-        int best = -1;
-        for (int e = 0; e < a.experts; ++e)
-            if ((last_e < 0 || before(last, last_e, l[e], e)) && (best < 0 || before(l[e], e, l[best], best))) best = e;
-        chosen[j] = last_e = best;
-        last = l[best];
-        if (j == 0) top = last;
-        if (a.normalize) sum += exp(last - top);
-    }
-    if (!a.normalize)
-        for (int e = 0; e < a.experts; ++e) sum += exp(l[e] - top);
-    for (int j = 0; j < a.topk; ++j) {
-        const float p = (float)(exp(l[chosen[j]] - top) / sum);
-        weights_of(a, w)[t * a.topk + j] = p;
-        if (a.weights) a.weights[t * a.topk + j] = p;
-        if (a.chosen) a.chosen[t * a.topk + j] = chosen[j];
-    }
-}
-
-// A wave's product of a row of an MXFP4 matrix.
+// Four waves; a wave takes an expert and up to 4 tokens.  Logits in 64 bits, so that which experts are
+// chosen does not depend on the order of the sums.  Workgroups past the experts' make pieces.
 template <typename T>
-__device__ inline float dot(const T* x, const uint8_t* P, const uint8_t* S, int64_t lds, int k)
+__global__ void __launch_bounds__(256) prepare_kernel(Mx4MoeArgs a, Mx4MoeWork w, int expert_groups)
 {
-    float sum = 0.0f;
-    for (int b = threadIdx.x % 64; b < (k + 31) / 32; b += 64) {
-        const float s = __builtin_bit_cast(float, (uint32_t)S[b / 8 * lds + b % 8] << 23);
-        for (int i = 0; i < 32 && 32 * b + i < k; ++i)
-            sum += (float)x[32 * b + i] *
-                   __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(P[16 * b + i / 2] >> i % 2 * 4, s, 0)[0];
+    constexpr int N = Piece<T>::N, PIECES = kBf16Pieces<T>;
+    if ((int)blockIdx.x >= expert_groups) {  // 8 terms a thread
+        const int per_row = w.x_ld / 16, i = (blockIdx.x - expert_groups) * 256 + threadIdx.x;
+        if (blockIdx.y > 0 || i >= per_row * a.tokens) return;
+        const int t = i / per_row, c = i % per_row * 8;
+        const T* row = (const T*)a.X + t * a.ldx;
+        float x[8];
+#pragma unroll
+        for (int p = 0; p < 8 / N; ++p) {
+            const Piece<T> v = a.width > N ? whole_piece<Cut::Ragged>(row, c + N * p, a.width)
+                                           : whole_piece<Cut::Short>(row, c + N * p, a.width);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[N * p + e] = (float)v.v[e];
+        }
+        bf16x8 to[PIECES];
+        split(x, to);
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) *(bf16x8*)(a.work + w.x + n * w.x_stride + (size_t)i * 16) = to[n];
+        return;
     }
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-    return sum;
+    const int e = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64, t0 = blockIdx.y * 4;
+    if (e >= a.experts) return;
+    const T* wr = (const T*)a.WR + e * a.ldwr;
+    const T* x[4];
+    double sum[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (const T*)a.X + min(t0 + j, a.tokens - 1) * a.ldx;
+    auto add = [&](double& s, T xv, T wv) {
+        if constexpr (sizeof(T) == 2)  // (the product is exact in 32 bits)
+            s += (double)((float)xv * (float)wv);
+        else
+            s += (double)xv * (double)wv;
+    };
+    const int whole = a.width / N * N;
+#pragma unroll 4
+    for (int c = lane * N; c < whole; c += 64 * N) {
+        const Piece<T> wv = *(const Piece<T>*)(wr + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > 0 && t0 + j >= a.tokens) break;
+            const Piece<T> xv = *(const Piece<T>*)(x[j] + c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) add(sum[j], xv.v[i], wv.v[i]);
+        }
+    }
+    if (whole + lane < a.width)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add(sum[j], x[j][whole + lane], wr[whole + lane]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double s = sum64(sum[j]);
+        if (lane == 0 && t0 + j < a.tokens) ((double*)(a.work + w.logits))[(int64_t)(t0 + j) * a.experts + e] = s;
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(64) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+// The highest of a wave's words.
+__device__ inline uint32_t highest(uint32_t x)
 {
-    const int64_t j = blockIdx.x, c = blockIdx.y;  // unit of the hidden layer, choice
-    const int64_t g = (int64_t)chosen_of(a, w)[c] * 2 * a.hidden + j, u = g + a.hidden;
-    const T* x = (const T*)a.X + c / a.topk * a.ldx;
-    const float gate = dot(x, a.W1 + g * a.ld1, a.S1 + 8 * g, a.lds1, a.width);
-    const float up = dot(x, a.W1 + u * a.ld1, a.S1 + 8 * u, a.lds1, a.width);
-    if (threadIdx.x == 0) act_of(a, w)[c * a.hidden + j] = gate / (1.0f + expf(-gate)) * up;
+    auto dpp = [&](auto ctrl) {
+        x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    dpp(std::integral_constant<int, kDppXor1>{});
+    dpp(std::integral_constant<int, kDppXor2>{});
+    dpp(std::integral_constant<int, kDppHalfMirror>{});
+    dpp(std::integral_constant<int, kDppMirror>{});
+    const uint32_t a = __builtin_amdgcn_readlane((int)x, 0), b = __builtin_amdgcn_readlane((int)x, 16),
+                   c = __builtin_amdgcn_readlane((int)x, 32), d = __builtin_amdgcn_readlane((int)x, 48);
+    return max(max(a, b), max(c, d));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(64) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+// A wave's choice for one token: take(j, e) for the j-th expert, the same in all lanes, up to `count`.
+// Returns the lane's share: of its choice in lanes below topk.
+constexpr int kMaxExperts = 512;
+template <typename F>
+__device__ inline float choose(const double* logits, int experts, int topk, int count, int normalize, int lane, F&& take)
 {
-    const int64_t n = blockIdx.x, t = blockIdx.y;
-    float y = 0.0f;
-    for (int j = 0; j < a.topk; ++j) {
-        const int64_t c = t * a.topk + j, r = (int64_t)chosen_of(a, w)[c] * a.width + n;
-        y += weights_of(a, w)[c] * dot(act_of(a, w) + c * a.hidden, a.W2 + r * a.ld2, a.S2 + 8 * r, a.lds2, a.hidden);
+    constexpr int EACH = kMaxExperts / 64;
+    double l[EACH];
+    uint64_t key[EACH];  // in the logits' order; 0: none, or taken already
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        key[i] = 0;
+        l[i] = 0.0;
+        if (i * 64 + lane < experts) {
+            l[i] = logits[i * 64 + lane] + 0.0;  // (no negative zero)
+            const uint64_t b = __builtin_bit_cast(uint64_t, l[i]);
+            key[i] = l[i] != l[i] ? ~0ull : b >> 63 ? ~b : b | 1ull << 63;
+        }
     }
-    if (threadIdx.x == 0) ((T*)a.Y)[t * a.ldy + n] = (T)y;
+    double mine = 0.0, top = 0.0;
+    for (int j = 0; j < count; ++j) {
+        uint64_t best = key[0];
+        int at = 0;
+        double value = l[0];
+#pragma unroll
+        for (int i = 1; i < EACH; ++i)
+            if (i * 64 < experts && key[i] > best) {
+                best = key[i];
+                at = i;
+                value = l[i];
+            }
+        const uint32_t hi = highest((uint32_t)(best >> 32));
+        uint64_t with = __builtin_amdgcn_ballot_w64((uint32_t)(best >> 32) == hi);
+        if (with & (with - 1)) {  // several: by the lower words, then the lowest index
+            const bool in = with >> lane & 1;
+            const uint32_t lo = highest(in ? (uint32_t)best : 0u);
+            const bool equal = in && (uint32_t)best == lo;
+            const uint32_t first = ~highest(equal ? ~(uint32_t)(at * 64 + lane) : 0u);
+            with = __builtin_amdgcn_ballot_w64(equal && (uint32_t)(at * 64 + lane) == first);
+        }
+        const int winner = __builtin_ctzll(with);
+        const int e = __builtin_amdgcn_readlane(at, winner) * 64 + winner;
+        const double x = lane_value(value, winner);
+        if (j == 0) top = x;
+        if (lane == j) mine = x;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (lane == winner && i == at) key[i] = 0;
+        take(j, e);
+    }
+    double all = 0.0;
+    if (normalize) {
+        all = lane < topk ? exp(mine - top) : 0.0;
+    } else {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (i * 64 + lane < experts) all += exp(l[i] - top);
+    }
+    return (float)(exp(mine - top) / sum64(all));
+}
+
+// A chunk's choices, by expert, in tiles of `up_size` and of `down_size` tokens.
+__global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w, int up_size, int down_size)
+{
+    __shared__ uint64_t tokens_of[kMaxExperts];  // as bits
+    __shared__ int expert_of[kMoeChoices], place[kMaxExperts], scan[3][16];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, t0 = blockIdx.x * kMoeChunk;
+    const int count = min(a.tokens - t0, kMoeChunk);
+    if (threadIdx.x < kMaxExperts) tokens_of[threadIdx.x] = 0;
+    __syncthreads();
+    for (int t = wave; t < count; t += 16) {
+        const int c0 = (t0 + t) * a.topk;
+        int mine = 0;
+        const float p = choose((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts, a.topk,
+                               a.topk, a.normalize, lane, [&](int j, int e) {
+                                   if (lane == j) mine = e;
+                               });
+        if (lane < a.topk) {
+            expert_of[t * a.topk + lane] = mine;
+            atomicOr((unsigned long long*)&tokens_of[mine], 1ull << t);
+            ((float*)(a.work + w.weights))[c0 + lane] = p;
+            if (a.weights) a.weights[c0 + lane] = p;
+            if (a.chosen) a.chosen[c0 + lane] = mine;
+        }
+    }
+    __syncthreads();
+    // sums over the experts before: choices, and tiles of either size
+    const int e = threadIdx.x, n = e < kMaxExperts ? __popcll(tokens_of[e]) : 0;
+    const int own[3] = {n, (n + up_size - 1) / up_size, (n + down_size - 1) / down_size};
+    int at[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        at[i] = own[i];
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(at[i], d);
+            if (lane >= d) at[i] += v;
+        }
+        if (lane == 63) scan[i][wave] = at[i];
+    }
+    __syncthreads();
+    int total[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        total[i] = 0;
+        for (int v = 0; v < 16; ++v) {
+            if (v < wave) at[i] += scan[i][v];
+            total[i] += scan[i][v];
+        }
+        at[i] -= own[i];
+    }
+    if (e < kMaxExperts) place[e] = at[0];
+    int* out = (int*)(a.work + w.tiles + blockIdx.x * w.tiles_bytes);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int size = k ? down_size : up_size;
+        int* to = out + 2 + k * 3 * kMoeTiles;
+        for (int i = 0; i < own[1 + k]; ++i) {
+            to[at[1 + k] + i] = e;
+            to[kMoeTiles + at[1 + k] + i] = at[0] + i * size;
+            to[2 * kMoeTiles + at[1 + k] + i] = min(n - i * size, size);
+        }
+        if (threadIdx.x == 0) out[k] = total[1 + k];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < count * a.topk; c += 1024) {
+        const int x = expert_of[c], before = __popcll(tokens_of[x] & ((1ull << c / a.topk) - 1));
+        out[2 + 6 * kMoeTiles + place[x] + before] = t0 * a.topk + c;
+    }
+}
+
+// ---- the experts ----
+
+// A tile's product with 16 rows each of G and U; ONE: the only token's, tile j of its j-th choice.
+template <typename T, int TOKENS, int WAVES, bool ONE>
+__global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    constexpr int PIECES = kBf16Pieces<T>, PITCH = 20;
+    constexpr int OWN = rows4_bytes(2) + tokens_bytes(PIECES, TOKENS), PART = 2 * 16 * PITCH * 4;
+    __shared__ __align__(16) char lds[WAVES * (OWN > PART ? OWN : PART)];
+    __shared__ int choice_of[TOKENS];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int j0 = blockIdx.x * 16, tile = blockIdx.y;
+    int expert, count = 1;
+    float share = 0.0f;  // ONE: of the tile's choice
+    if constexpr (ONE) {
+        expert = 0;
+        int mine = 0;
+        // (the tile's own first, which its weights wait for; all of them for the shares)
+        const float p = choose((const double*)(a.work + w.logits), a.experts, a.topk, a.topk, a.normalize, lane,
+                               [&](int j, int e) {
+                                   if (j == tile) expert = e;
+                                   if (lane == j) mine = e;
+                               });
+        share = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), tile));
+        if (blockIdx.x == 0 && tile == 0 && wave == 0 && lane < a.topk) {
+            ((int*)(a.work + w.chosen))[lane] = mine;
+            if (a.weights) a.weights[lane] = p;
+            if (a.chosen) a.chosen[lane] = mine;
+        }
+    } else {
+        const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
+        if (tile >= tiles[0]) return;
+        expert = __builtin_amdgcn_readfirstlane(tiles[2 + tile]);
+        const int from = tiles[2 + kMoeTiles + tile];
+        count = __builtin_amdgcn_readfirstlane(tiles[2 + 2 * kMoeTiles + tile]);
+        if (threadIdx.x < TOKENS)
+            choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
+        __syncthreads();
+    }
+    char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(2);
+    const int nb = (a.width + 31) / 32, groups = (nb + 7) / 8, rows = min(a.hidden - j0, 16);
+    f32x4 acc[2] = {};
+    if (rows > 0) {
+        Source4<1> sg, su;
+        sg.init(a.ld1, a.lds1, rows, nb, lane);
+        sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + j0);
+        su = sg;
+        su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + j0);
+        PieceTokens<PIECES, TOKENS> sa;
+        sa.base = a.work + w.x;
+        sa.stride = w.x_stride;
+        sa.move([&](int t) { return ONE ? 0 : choice_of[t] / a.topk * w.x_ld; }, lane);
+        Rows4<1> wg[2], wu[2];
+        typename PieceTokens<PIECES, TOKENS>::Values x;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const int g = wave + d * WAVES;
+            sg.load(wg[d], g, nb - 8 * g);
+            su.load(wu[d], g, nb - 8 * g);
+        }
+        sa.load(x, min(wave, groups - 1));
+        for (int g = wave; g < groups;) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                bf16x8 v[2][8];
+                if (nb - 8 * g < 8) {
+                    wg[d].code[0] = first_codes(wg[d].code[0], nb - 8 * g);
+                    wu[d].code[0] = first_codes(wu[d].code[0], nb - 8 * g);
+                }
+                const Rows4<2> both = {{wg[d].v[0], wg[d].v[1], wu[d].v[0], wu[d].v[1]}, {wg[d].code[0], wu[d].code[0]}};
+                fragments(both, own, lane, v);
+                sg.load(wg[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
+                su.load(wu[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
+                sa.put(x, tokens_at, lane);
+                sa.load(x, min(g + WAVES, groups - 1));
+                multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
+                g += WAVES;
+                if (g >= groups) break;
+            }
+        }
+    }
+    __syncthreads();
+    float* part = (float*)lds;
+    const int r = lane % 16, q = lane / 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[((wave * 2 + i) * 16 + 4 * q + e) * PITCH + r] = acc[i][e];
+    __syncthreads();
+    // 8 units a thread, and zeros past the last one, to the row's end
+    for (int t = threadIdx.x; t < 2 * TOKENS; t += 64 * WAVES) {
+        const int token = t / 2, u0 = t % 2 * 8;
+        if (token >= count) continue;
+        const int choice = ONE ? tile : choice_of[token];
+        const float p = ONE ? share : ((const float*)(a.work + w.weights))[choice];
+        float h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float g = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+                g += part[((v * 2) * 16 + u0 + i) * PITCH + token];
+                u += part[((v * 2 + 1) * 16 + u0 + i) * PITCH + token];
+            }
+            h[i] = u0 + i < rows ? p * (g / (1.0f + expf(-g)) * u) : 0.0f;
+        }
+        bf16x8 to[kActPieces<T>];
+        split(h, to);
+#pragma unroll
+        for (int n = 0; n < kActPieces<T>; ++n)
+            *(bf16x8*)(a.work + w.act + n * w.act_stride + (size_t)choice * w.act_ld + 2 * (j0 + u0)) = to[n];
+    }
+}
+
+// 16 results of a chunk's tokens.  Its tiles times their groups of terms are cut into one run for each
+// wave; a wave adds a tile's sums to its tokens' in LDS when it leaves it, and the waves' are added up at
+// the end, in order.  ONE: the only token's.
+template <typename T, int TOKENS, int WAVES, bool ONE>
+__global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    constexpr int PIECES = kActPieces<T>, OWN = rows4_bytes(1) + tokens_bytes(PIECES, TOKENS);
+    constexpr int MOST = ONE ? 1 : kMoeChunk, PITCH = 17;
+    __shared__ __align__(16) char lds[WAVES * OWN];
+    __shared__ float part[WAVES][MOST * PITCH];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n0 = blockIdx.x * 16, t0 = blockIdx.y * kMoeChunk, count = min(a.tokens - t0, MOST);
+    const int* tiles = (const int*)(a.work + w.tiles + blockIdx.y * w.tiles_bytes);
+    const int *experts = ONE ? (const int*)(a.work + w.chosen) : tiles + 2 + 3 * kMoeTiles, *choices = tiles + 2 + 6 * kMoeTiles;
+    const int tile_count = ONE ? a.topk : tiles[1];
+    char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(1);
+    const int nb = (a.hidden + 31) / 32, groups = (nb + 7) / 8;
+    for (int i = lane; i < MOST * PITCH; i += 64) part[wave][i] = 0.0f;
+
+    const int units = tile_count * groups, from = (int)((int64_t)units * wave / WAVES),
+              to = (int)((int64_t)units * (wave + 1) / WAVES);
+    if (from < to) {
+        struct Place {  // a tile and a group of its terms
+            int tile, g;
+        };
+        auto after = [&](Place p) { return p.g + 1 < groups ? Place{p.tile, p.g + 1} : Place{p.tile + 1, 0}; };
+        Source4<1> sw;
+        sw.init(a.ld2, a.lds2, a.width - n0, nb, lane);
+        PieceTokens<PIECES, TOKENS> sa;
+        sa.base = a.work + w.act;
+        sa.stride = w.act_stride;
+        auto load_rows = [&](Rows4<1>& d, Place p) {  // (past the last tile: the last one again)
+            const int e = __builtin_amdgcn_readfirstlane(experts[min(p.tile, tile_count - 1)]);
+            sw.move(a.W2, a.S2, (int64_t)e * a.width + n0);
+            sw.load(d, p.g, nb - 8 * p.g);
+        };
+        typename PieceTokens<PIECES, TOKENS>::Values x;
+        auto load_tokens = [&](Place p) {
+            if constexpr (ONE) {
+                const int row = min(p.tile, tile_count - 1) * w.act_ld;
+                sa.move([&](int) { return row; }, lane);
+            } else {
+                const int tile = min(p.tile, tile_count - 1), first = experts[kMoeTiles + tile],
+                          n = experts[2 * kMoeTiles + tile];
+                sa.move([&](int t) { return choices[first + min(t, n - 1)] * w.act_ld; }, lane);
+            }
+            sa.load(x, p.g);
+        };
+        Rows4<1> rows[2];
+        f32x4 acc[1] = {};
+        Place now{from / groups, from % groups}, next = after(now);
+        load_rows(rows[0], now);
+        load_rows(rows[1], next);
+        load_tokens(now);
+        for (int u = from; u < to;) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const Place then = after(next);
+                bf16x8 v[1][8];
+                if (nb - 8 * now.g < 8) rows[d].code[0] = first_codes(rows[d].code[0], nb - 8 * now.g);
+                fragments(rows[d], own, lane, v);
+                load_rows(rows[d], then);
+                sa.put(x, tokens_at, lane);
+                load_tokens(next);
+                multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
+                ++u;
+                if (u == to || next.tile != now.tile) {
+                    const int r = lane % 16, q = lane / 16;
+                    int token = r < 1 ? 0 : -1;
+                    if constexpr (!ONE) {
+                        const int first = experts[kMoeTiles + now.tile], n = experts[2 * kMoeTiles + now.tile];
+                        token = r < n ? choices[first + r] / a.topk - t0 : -1;
+                    }
+                    if (token >= 0)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) part[wave][token * PITCH + 4 * q + e] += acc[0][e];
+                    acc[0] = f32x4{};
+                }
+                now = next;
+                next = then;
+                if (u == to) break;
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * 16; i += 64 * WAVES) {
+        const int t = i / 16, n = n0 + i % 16;
+        if (n >= a.width) continue;
+        float y = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) y += part[v][t * PITCH + i % 16];
+        ((T*)a.Y)[(t0 + t) * a.ldy + n] = (T)y;
+    }
 }
 
 template <typename T>
 hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
 {
-    const Mx4MoeWork w = mx4_moe_work(a.tokens, a.hidden, a.experts, a.topk);
-    const unsigned choices = (unsigned)(a.tokens * a.topk);
-    logits_kernel<T><<<dim3((unsigned)a.experts, (unsigned)a.tokens), 64, 0, s>>>(a, w);
-    choose_kernel<<<(unsigned)(a.tokens + 63) / 64, 64, 0, s>>>(a, w);
-    up_kernel<T><<<dim3((unsigned)a.hidden, choices), 64, 0, s>>>(a, w);
-    down_kernel<T><<<dim3((unsigned)a.width, (unsigned)a.tokens), 64, 0, s>>>(a, w);
+    const Mx4MoeWork w = mx4_moe_work(a.tokens, a.width, a.hidden, a.experts, a.topk);
+    constexpr int UP = kBf16Pieces<T> == 1 ? 16 : 8, DOWN = 8;  // tokens of a tile (what fits the LDS)
+    const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
+    const int expert_groups = (a.experts + 3) / 4, pieces = (w.x_ld / 16 * a.tokens + 255) / 256;
+    prepare_kernel<T><<<dim3((unsigned)(expert_groups + pieces), (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(
+        a, w, expert_groups);
+    const unsigned up_x = (unsigned)(w.act_ld / 32), down_x = (unsigned)((a.width + 15) / 16);
+    if (a.tokens == 1) {
+        up_kernel<T, 2, 8, true><<<dim3(up_x, (unsigned)a.topk), 512, 0, s>>>(a, w);
+        down_kernel<T, 2, 16, true><<<down_x, 1024, 0, s>>>(a, w);
+    } else {
+        choose_kernel<<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
+        const int most = a.experts + choices / UP < choices ? a.experts + choices / UP : choices;
+        up_kernel<T, UP, 4, false><<<dim3(up_x, (unsigned)most, chunks), 256, 0, s>>>(a, w);
+        down_kernel<T, DOWN, 8, false><<<dim3(down_x, chunks), 512, 0, s>>>(a, w);
+    }
     return hipGetLastError();
 }
 

@@ -58,22 +58,25 @@ struct Source4 {
     int64_t lds;
     int bytes, count, ld, at[2 * N], lane;
 
-    // Rows first .. (n in all), of nb blocks.
-    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int64_t first, int64_t n,
-                                int nb, int lane_)
+    // `count_` rows of nb blocks (or 16 N of more), the first of them in `rows` and `codes`.
+    __device__ inline void init(int64_t ld_, int64_t lds_, int count_, int nb, int lane_)
     {
-        count = (int)min(n - first, (int64_t)(16 * N));
+        count = min(count_, 16 * N);
         ld = (int)ld_;
         lds = lds_;
         lane = lane_;
-        rows = P + first * ld_;
         bytes = strip_bytes(count, ld, nb);
-        codes = S + 8 * first;
 #pragma unroll
         for (int i = 0; i < 2 * N; ++i) {
             const int row = 8 * i + lane / 8;
             at[i] = row < count ? row * ld + lane % 8 * 16 : kOutside;
         }
+    }
+
+    __device__ inline void move(const uint8_t* P, const uint8_t* S, int64_t first)
+    {
+        rows = P + first * ld;
+        codes = S + 8 * first;
     }
 
     // Group g, `left` blocks up to the last: zeros, not from memory, past it and past the last row
@@ -122,6 +125,10 @@ __device__ inline bf16x8 values4(uint32_t word, float scale)
     return bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 }
 
+// Between a wave's writes to its LDS and the reads of other lanes' (and those and the next writes):
+// LDS serves a wave in order, so only the compiler has to keep it.
+__device__ inline void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // A wave's LDS for rows: 2 KiB for each 16.  Chunk c of row x lies at place c ^ (x / 2 % 8) of its
 // 128 bytes: LDS serves 16 bytes a lane to lanes 0-3, 12-15 and 20-27, then to the others of 0-31,
 // then to 32-63 likewise, and no two of such 16 meet in a bank.
@@ -136,6 +143,7 @@ __device__ inline void fragments(const Rows4<N>& d, char* lds, int lane, bf16x8 
         const int row = 8 * i + lane / 8;
         *(u32x4*)(lds + row * 128 + (lane % 8 ^ row / 2 % 8) * 16) = d.v[i];
     }
+    in_order();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int row = 16 * i + lane % 16;
@@ -146,6 +154,7 @@ __device__ inline void fragments(const Rows4<N>& d, char* lds, int lane, bf16x8 
             for (int b = 0; b < 4; ++b) to[i][4 * h + b] = values4(w[b], scale_of_code(d.code[i][h] >> 8 * b & 255));
         }
     }
+    in_order();
 }
 
 // ---- tokens ----
@@ -153,7 +162,8 @@ __device__ inline void fragments(const Rows4<N>& d, char* lds, int lane, bf16x8 
 template <typename T>
 constexpr int kBf16Pieces = sizeof(T) == 4 ? 3 : std::is_same<T, f16_t>::value ? 2 : 1;
 
-// Eight values as bf16 pieces, the largest first.  An infinity's lower pieces are zeros.
+// Eight values as bf16 pieces, the largest first; what is left for the last one is rounded to it (of
+// 2 pieces for fp16 and 3 for fp32 nothing is lost).  An infinity's lower pieces are zeros.
 template <int N>
 __device__ inline void split(const float (&x)[8], bf16x8 (&to)[N])
 {
@@ -161,14 +171,13 @@ __device__ inline void split(const float (&x)[8], bf16x8 (&to)[N])
 #pragma unroll
     for (int i = 0; i < 8; ++i) rest[i] = x[i];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+    for (int n = 0; n + 1 < N; ++n) {
         u32x4 w;  // the upper halves of two words
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, rest[2 * i + 1]),
                                          __builtin_bit_cast(uint32_t, rest[2 * i]), 0x07060302);
         to[n] = __builtin_bit_cast(bf16x8, w);
-        if (n + 1 == N) break;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float top = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xffff0000);
@@ -176,6 +185,8 @@ __device__ inline void split(const float (&x)[8], bf16x8 (&to)[N])
             rest[i] = n == 0 && __builtin_isinf(x[i]) ? 0.0f : left;
         }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to[N - 1][i] = (bf16_t)rest[i];
 }
 
 // 256 terms of a tile of TOKENS (2, 8 or 16) tokens: a lane loads 8 terms, 8 (lane % 32) .., of tokens
@@ -315,10 +326,48 @@ struct Mx8Tokens {
     }
 };
 
+// Tokens that lie as bf16 pieces already: row t of piece n at `at` + n * stride, zeros to a whole group.
+template <int PIECES_, int TOKENS>
+struct PieceTokens {
+    static constexpr int PIECES = PIECES_, LOADS = TOKENS / 2;
+    struct Values {
+        u32x4 v[LOADS][PIECES];
+    };
+    const uint8_t* base;
+    int64_t stride;
+    int at[LOADS];
+
+    // Token t of the tile lies offset_of(t) bytes from a piece's base; of one that is not there, another.
+    template <typename F>
+    __device__ inline void move(F&& offset_of, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) at[i] = offset_of(2 * i + lane / 32) + lane % 32 * 16;
+    }
+    __device__ inline void load(Values& d, int g) const
+    {
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) d.v[i][n] = *(const u32x4*)(base + n * stride + g * 512 + (int64_t)at[i]);
+    }
+    __device__ inline void put(const Values& d, char* lds, int lane) const
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            bf16x8 x[PIECES];
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) x[n] = __builtin_bit_cast(bf16x8, d.v[i][n]);
+            put_tokens<PIECES, TOKENS>(lds, i, lane, x);
+        }
+    }
+};
+
 // acc[i]: rows 4 (lane / 16) + e of block i of w, token lane % 16 of the tile in the wave's LDS.
 template <int PIECES, int TOKENS, int N>
 __device__ inline void multiply(f32x4 (&acc)[N], const bf16x8 (&w)[N][8], const char* lds, int lane)
 {
+    in_order();
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
         bf16x8 x[PIECES];
@@ -329,6 +378,7 @@ __device__ inline void multiply(f32x4 (&acc)[N], const bf16x8 (&w)[N][8], const 
             for (int i = 0; i < N; ++i)
                 acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][b], x[n], acc[i], 0, 0, 0);
     }
+    in_order();
 }
 
 }  // namespace sbx

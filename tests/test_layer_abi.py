@@ -80,7 +80,7 @@ def test_linear_refusals(kw, status):
 
 @pytest.mark.parametrize("kw,status", ANY + [
     (dict(tokens=-1), 1), (dict(width=0), 1), (dict(hidden=0), 1), (dict(experts=0), 1), (dict(topk=0), 1),
-    (dict(topk=6), 1), (dict(tokens=257), 2), (dict(width=(1 << 20) + 1), 2), (dict(hidden=(1 << 20) + 1), 2),
+    (dict(topk=6), 1), (dict(tokens=257), 2), (dict(width=(1 << 18) + 1), 2), (dict(hidden=(1 << 18) + 1), 2),
     (dict(experts=513), 2), (dict(experts=40, topk=17), 2),
     (dict(X=0), 1), (dict(X=66), 1), (dict(ldx=39), 1), (dict(WR=0), 1), (dict(WR=66), 1), (dict(ldwr=39), 1),
     (dict(W1=0), 1), (dict(W1=72), 1), (dict(ld1=16), 1), (dict(ld1=40), 1), (dict(S1=0), 1), (dict(S1=68), 1),
