@@ -26,9 +26,10 @@ namespace {
 template <typename T>
 constexpr int kActPieces = sizeof(T) == 4 ? 3 : 2;
 
-// Four waves; a wave takes an expert and up to 4 tokens.  Logits in 64 bits, so that which experts are
-// chosen does not depend on the order of the sums.  Workgroups past the experts' make pieces.
-template <typename T>
+// Four experts and TOKENS (1 or 4) tokens a workgroup, whose four waves take a quarter of the terms each.
+// Logits in 64 bits, so that which experts are chosen does not depend on the order of the sums.
+// Workgroups past the experts' make pieces.
+template <typename T, int TOKENS>
 __global__ void __launch_bounds__(256) prepare_kernel(Mx4MoeArgs a, Mx4MoeWork w, int expert_groups)
 {
     constexpr int N = Piece<T>::N, PIECES = kBf16Pieces<T>;
@@ -51,39 +52,63 @@ __global__ void __launch_bounds__(256) prepare_kernel(Mx4MoeArgs a, Mx4MoeWork w
         for (int n = 0; n < PIECES; ++n) *(bf16x8*)(a.work + w.x + n * w.x_stride + (size_t)i * 16) = to[n];
         return;
     }
-    const int e = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64, t0 = blockIdx.y * 4;
-    if (e >= a.experts) return;
-    const T* wr = (const T*)a.WR + e * a.ldwr;
-    const T* x[4];
-    double sum[4] = {};
+    __shared__ double part[4][4 * TOKENS];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, e0 = blockIdx.x * 4, t0 = blockIdx.y * TOKENS;
+    const T *wr[4], *x[TOKENS];  // (past the last expert or token: the last one again)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (const T*)a.X + min(t0 + j, a.tokens - 1) * a.ldx;
-    auto add = [&](double& s, T xv, T wv) {
-        if constexpr (sizeof(T) == 2)  // (the product is exact in 32 bits)
-            s += (double)((float)xv * (float)wv);
-        else
-            s += (double)xv * (double)wv;
+    for (int i = 0; i < 4; ++i) wr[i] = (const T*)a.WR + min(e0 + i, a.experts - 1) * a.ldwr;
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) x[j] = (const T*)a.X + min(t0 + j, a.tokens - 1) * a.ldx;
+    double sum[4][TOKENS] = {};
+    auto add = [&](const T(&wv)[4], const T(&xv)[TOKENS]) {
+        double wd[4], xd[TOKENS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wd[i] = (double)(float)wv[i];
+#pragma unroll
+        for (int j = 0; j < TOKENS; ++j) xd[j] = (double)(float)xv[j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < TOKENS; ++j) sum[i][j] += wd[i] * xd[j];
     };
     const int whole = a.width / N * N;
-#pragma unroll 4
-    for (int c = lane * N; c < whole; c += 64 * N) {
-        const Piece<T> wv = *(const Piece<T>*)(wr + c);
+#pragma unroll 2
+    for (int c = threadIdx.x * N; c < whole; c += 256 * N) {
+        Piece<T> wv[4], xv[TOKENS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > 0 && t0 + j >= a.tokens) break;
-            const Piece<T> xv = *(const Piece<T>*)(x[j] + c);
+        for (int i = 0; i < 4; ++i) wv[i] = *(const Piece<T>*)(wr[i] + c);
 #pragma unroll
-            for (int i = 0; i < N; ++i) add(sum[j], xv.v[i], wv.v[i]);
+        for (int j = 0; j < TOKENS; ++j) xv[j] = *(const Piece<T>*)(x[j] + c);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            T we[4], xe[TOKENS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) we[i] = wv[i].v[n];
+#pragma unroll
+            for (int j = 0; j < TOKENS; ++j) xe[j] = xv[j].v[n];
+            add(we, xe);
         }
     }
-    if (whole + lane < a.width)
+    if (whole + (int)threadIdx.x < a.width) {
+        T we[4], xe[TOKENS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) add(sum[j], x[j][whole + lane], wr[whole + lane]);
+        for (int i = 0; i < 4; ++i) we[i] = wr[i][whole + threadIdx.x];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const double s = sum64(sum[j]);
-        if (lane == 0 && t0 + j < a.tokens) ((double*)(a.work + w.logits))[(int64_t)(t0 + j) * a.experts + e] = s;
+        for (int j = 0; j < TOKENS; ++j) xe[j] = x[j][whole + threadIdx.x];
+        add(we, xe);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < TOKENS; ++j) {
+            const double s = sum64(sum[i][j]);
+            if (lane == 0) part[wave][i * TOKENS + j] = s;
+        }
+    __syncthreads();
+    const int i = threadIdx.x / TOKENS, j = threadIdx.x % TOKENS;
+    if (i < 4 && e0 + i < a.experts && t0 + j < a.tokens)
+        ((double*)(a.work + w.logits))[(int64_t)(t0 + j) * a.experts + e0 + i] =
+            part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
 }
 
 // The highest of a wave's words.
@@ -101,13 +126,13 @@ __device__ inline uint32_t highest(uint32_t x)
     return max(max(a, b), max(c, d));
 }
 
-// A wave's choice for one token: take(j, e) for the j-th expert, the same in all lanes, up to `count`.
-// Returns the lane's share: of its choice in lanes below topk.
+// A wave's choice for one token: take(j, e) for the j-th expert, the same in all lanes.
+// Returns the lane's share: of its choice in lanes below topk.  EACH: logits a lane has, 64 * EACH >=
+// experts.
 constexpr int kMaxExperts = 512;
-template <typename F>
-__device__ inline float choose(const double* logits, int experts, int topk, int count, int normalize, int lane, F&& take)
+template <int EACH, typename F>
+__device__ inline float choose(const double* logits, int experts, int topk, int normalize, int lane, F&& take)
 {
-    constexpr int EACH = kMaxExperts / 64;
     double l[EACH];
     uint64_t key[EACH];  // in the logits' order; 0: none, or taken already
 #pragma unroll
@@ -121,7 +146,7 @@ __device__ inline float choose(const double* logits, int experts, int topk, int 
         }
     }
     double mine = 0.0, top = 0.0;
-    for (int j = 0; j < count; ++j) {
+    for (int j = 0; j < topk; ++j) {
         uint64_t best = key[0];
         int at = 0;
         double value = l[0];
@@ -163,6 +188,7 @@ __device__ inline float choose(const double* logits, int experts, int topk, int 
 }
 
 // A chunk's choices, by expert, in tiles of `up_size` and of `down_size` tokens.
+template <int EACH>
 __global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w, int up_size, int down_size)
 {
     __shared__ uint64_t tokens_of[kMaxExperts];  // as bits
@@ -174,10 +200,10 @@ __global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w
     for (int t = wave; t < count; t += 16) {
         const int c0 = (t0 + t) * a.topk;
         int mine = 0;
-        const float p = choose((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts, a.topk,
-                               a.topk, a.normalize, lane, [&](int j, int e) {
-                                   if (lane == j) mine = e;
-                               });
+        const float p = choose<EACH>((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts,
+                                     a.topk, a.normalize, lane, [&](int j, int e) {
+                                         if (lane == j) mine = e;
+                                     });
         if (lane < a.topk) {
             expert_of[t * a.topk + lane] = mine;
             atomicOr((unsigned long long*)&tokens_of[mine], 1ull << t);
@@ -233,8 +259,9 @@ __global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w
 
 // ---- the experts ----
 
-// A tile's product with 16 rows each of G and U; ONE: the only token's, tile j of its j-th choice.
-template <typename T, int TOKENS, int WAVES, bool ONE>
+// A tile's product with 16 rows each of G and U.  ONE (EACH of choose, or 0): the only token's, tile j of
+// its j-th choice.
+template <typename T, int TOKENS, int WAVES, int ONE>
 __global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kBf16Pieces<T>, PITCH = 20;
@@ -248,12 +275,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeW
     if constexpr (ONE) {
         expert = 0;
         int mine = 0;
-        // (the tile's own first, which its weights wait for; all of them for the shares)
-        const float p = choose((const double*)(a.work + w.logits), a.experts, a.topk, a.topk, a.normalize, lane,
-                               [&](int j, int e) {
-                                   if (j == tile) expert = e;
-                                   if (lane == j) mine = e;
-                               });
+        const float p = choose<ONE>((const double*)(a.work + w.logits), a.experts, a.topk, a.normalize, lane,
+                                    [&](int j, int e) {
+                                        if (j == tile) expert = e;
+                                        if (lane == j) mine = e;
+                                    });
         share = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), tile));
         if (blockIdx.x == 0 && tile == 0 && wave == 0 && lane < a.topk) {
             ((int*)(a.work + w.chosen))[lane] = mine;
@@ -282,7 +308,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeW
         PieceTokens<PIECES, TOKENS> sa;
         sa.base = a.work + w.x;
         sa.stride = w.x_stride;
-        sa.move([&](int t) { return ONE ? 0 : choice_of[t] / a.topk * w.x_ld; }, lane);
+        sa.move([&](int t) { return t >= count ? kOutside : ONE ? 0 : choice_of[t] / a.topk * w.x_ld; }, lane);
         Rows4<1> wg[2], wu[2];
         typename PieceTokens<PIECES, TOKENS>::Values x;
 #pragma unroll
@@ -374,7 +400,7 @@ __global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWo
         Source4<1> sw;
         sw.init(a.ld2, a.lds2, a.width - n0, nb, lane);
         PieceTokens<PIECES, TOKENS> sa;
-        sa.base = a.work + w.act;
+        sa.base = a.work + w.act + (size_t)(t0 * a.topk) * w.act_ld;
         sa.stride = w.act_stride;
         auto load_rows = [&](Rows4<1>& d, Place p) {  // (past the last tile: the last one again)
             const int e = __builtin_amdgcn_readfirstlane(experts[min(p.tile, tile_count - 1)]);
@@ -385,11 +411,11 @@ __global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWo
         auto load_tokens = [&](Place p) {
             if constexpr (ONE) {
                 const int row = min(p.tile, tile_count - 1) * w.act_ld;
-                sa.move([&](int) { return row; }, lane);
+                sa.move([&](int t) { return t > 0 ? kOutside : row; }, lane);
             } else {
                 const int tile = min(p.tile, tile_count - 1), first = experts[kMoeTiles + tile],
                           n = experts[2 * kMoeTiles + tile];
-                sa.move([&](int t) { return choices[first + min(t, n - 1)] * w.act_ld; }, lane);
+                sa.move([&](int t) { return t < n ? (choices[first + t] - t0 * a.topk) * w.act_ld : kOutside; }, lane);
             }
             sa.load(x, p.g);
         };
@@ -447,17 +473,29 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
     constexpr int UP = kBf16Pieces<T> == 1 ? 16 : 8, DOWN = 8;  // tokens of a tile (what fits the LDS)
     const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
     const int expert_groups = (a.experts + 3) / 4, pieces = (w.x_ld / 16 * a.tokens + 255) / 256;
-    prepare_kernel<T><<<dim3((unsigned)(expert_groups + pieces), (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(
-        a, w, expert_groups);
+    const unsigned prepare_x = (unsigned)(expert_groups + pieces);
     const unsigned up_x = (unsigned)(w.act_ld / 32), down_x = (unsigned)((a.width + 15) / 16);
     if (a.tokens == 1) {
-        up_kernel<T, 2, 8, true><<<dim3(up_x, (unsigned)a.topk), 512, 0, s>>>(a, w);
+        prepare_kernel<T, 1><<<prepare_x, 256, 0, s>>>(a, w, expert_groups);
+        const dim3 up(up_x, (unsigned)a.topk);
+        if (a.experts <= 64)
+            up_kernel<T, 2, 8, 1><<<up, 512, 0, s>>>(a, w);
+        else if (a.experts <= 128)
+            up_kernel<T, 2, 8, 2><<<up, 512, 0, s>>>(a, w);
+        else
+            up_kernel<T, 2, 8, 8><<<up, 512, 0, s>>>(a, w);
         down_kernel<T, 2, 16, true><<<down_x, 1024, 0, s>>>(a, w);
     } else {
-        choose_kernel<<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
+        if (a.experts <= 64)
+            choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        else if (a.experts <= 128)
+            choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        else
+            choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
         const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
         const int most = a.experts + choices / UP < choices ? a.experts + choices / UP : choices;
-        up_kernel<T, UP, 4, false><<<dim3(up_x, (unsigned)most, chunks), 256, 0, s>>>(a, w);
+        up_kernel<T, UP, 4, 0><<<dim3(up_x, (unsigned)most, chunks), 256, 0, s>>>(a, w);
         down_kernel<T, DOWN, 8, false><<<dim3(down_x, chunks), 512, 0, s>>>(a, w);
     }
     return hipGetLastError();

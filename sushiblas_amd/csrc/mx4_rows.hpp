@@ -326,7 +326,8 @@ struct Mx8Tokens {
     }
 };
 
-// Tokens that lie as bf16 pieces already: row t of piece n at `at` + n * stride, zeros to a whole group.
+// Tokens that lie as bf16 pieces already: a piece of token t offset_of(t) bytes from its base, zeros to
+// a whole group; the pieces' bases are `stride` apart.
 template <int PIECES_, int TOKENS>
 struct PieceTokens {
     static constexpr int PIECES = PIECES_, LOADS = TOKENS / 2;
@@ -337,19 +338,25 @@ struct PieceTokens {
     int64_t stride;
     int at[LOADS];
 
-    // Token t of the tile lies offset_of(t) bytes from a piece's base; of one that is not there, another.
+    // A token that is not there (kOutside) is not read.
     template <typename F>
     __device__ inline void move(F&& offset_of, int lane)
     {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) at[i] = offset_of(2 * i + lane / 32) + lane % 32 * 16;
+        for (int i = 0; i < LOADS; ++i) {
+            const int from = offset_of(2 * i + lane / 32);
+            at[i] = from == kOutside ? kOutside : from + lane % 32 * 16;
+        }
     }
     __device__ inline void load(Values& d, int g) const
     {
 #pragma unroll
-        for (int n = 0; n < PIECES; ++n)
+        for (int n = 0; n < PIECES; ++n) {
+            const __amdgpu_buffer_rsrc_t v = buffer_of(base + n * stride, 0x7fffffff);
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) d.v[i][n] = *(const u32x4*)(base + n * stride + g * 512 + (int64_t)at[i]);
+            for (int i = 0; i < LOADS; ++i)
+                d.v[i][n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], g * 512, 0));
+        }
     }
     __device__ inline void put(const Values& d, char* lds, int lane) const
     {
