@@ -30,7 +30,7 @@ template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 {
     typedef typename std::conditional<MX8, Mx8Tokens<TOKENS>, DenseTokens<T, TOKENS>>::type tokens_t;
-    constexpr int PIECES = tokens_t::PIECES, PITCH = 16 * YB + 4, AHEAD = 2, AHEAD_X = TOKENS == 2 ? AHEAD : 1;
+    constexpr int PIECES = tokens_t::PIECES, FRAGMENTS = fragments_of(PIECES, TOKENS), PITCH = 16 * FRAGMENTS * YB + 4, AHEAD = 2, AHEAD_X = TOKENS == 2 ? AHEAD : 1;
     constexpr int OWN = rows4_bytes(XB) + tokens_bytes(PIECES, TOKENS), PART = 16 * PITCH * 4;
     __shared__ __align__(16) char lds[WAVES * (OWN > PART ? OWN : PART)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
         }
     }
 
-    f32x4 acc[YB][XB] = {};
+    f32x4 acc[YB][FRAGMENTS][XB] = {};
     Rows4<XB> w[AHEAD];
     typename tokens_t::Values a[AHEAD_X];
     // (no branch around a load, and one past the last group reads zeros or the last group again: the
@@ -94,7 +94,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 #pragma unroll
         for (int j = 0; j < YB; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[(wave * 16 + 4 * q + e) * PITCH + 16 * j + r] = acc[j][i][e];
+            for (int f = 0; f < FRAGMENTS; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    part[(wave * 16 + 4 * q + e) * PITCH + 16 * (FRAGMENTS * j + f) + r] = acc[j][f][i][e];
         __syncthreads();
         for (int t = threadIdx.x; t < 16 * TOKENS * YB; t += 64 * WAVES) {
             const int dm = t / 16, n = x0 + 16 * i + t % 16, m = y0 + dm;
@@ -102,7 +105,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w)
-                v += part[(w * 16 + t % 16) * PITCH + dm / TOKENS * 16 + dm % TOKENS];
+#pragma unroll
+                for (int x = 0; x < PIECES; ++x)
+                    v += part[(w * 16 + t % 16) * PITCH + 16 * FRAGMENTS * (dm / TOKENS) + x * TOKENS + dm % TOKENS];
             T* y = Y + (int64_t)m * p.ldy + n;
             *y = result<T>(v, p.beta != 0.0f ? (float)*y : 0.0f, p);
         }
@@ -155,8 +160,11 @@ hipError_t launch(const Mx4LinearArgs& a, hipStream_t s)
     }
     if (a.m <= 2) return launch_form<T, MX8, 2, 1>(a, s);
     if (a.m <= TOKENS) return launch_form<T, MX8, TOKENS, 1>(a, s);
-    if (a.m <= 2 * TOKENS) return launch_form<T, MX8, TOKENS, 2>(a, s);
-    return launch_form<T, MX8, TOKENS, 4>(a, s);
+    // (four tiles of fp32 would not fit the registers)
+    if (a.m <= 2 * TOKENS || (!MX8 && sizeof(T) == 4))
+        return launch_form<T, MX8, TOKENS, 2>(a, s);
+    else if constexpr (MX8 || sizeof(T) < 4)
+        return launch_form<T, MX8, TOKENS, 4>(a, s);
 }
 
 }  // namespace

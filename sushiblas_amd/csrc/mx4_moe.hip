@@ -126,33 +126,36 @@ __device__ inline uint32_t highest(uint32_t x)
     return max(max(a, b), max(c, d));
 }
 
-// A wave's choice for one token: take(j, e) for the j-th expert, the same in all lanes.
-// Returns the lane's share: of its choice in lanes below topk.  EACH: logits a lane has, 64 * EACH >=
-// experts.
+// A wave's choices for one token, one after another.  EACH: logits a lane has, 64 * EACH >= experts.
 constexpr int kMaxExperts = 512;
-template <int EACH, typename F>
-__device__ inline float choose(const double* logits, int experts, int topk, int normalize, int lane, F&& take)
-{
-    double l[EACH];
+template <int EACH>
+struct Chooser {
+    double l[EACH], mine, top;
     uint64_t key[EACH];  // in the logits' order; 0: none, or taken already
+
+    __device__ __forceinline__ void init(const double* logits, int experts, int lane)
+    {
+        mine = top = 0.0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        key[i] = 0;
-        l[i] = 0.0;
-        if (i * 64 + lane < experts) {
-            l[i] = logits[i * 64 + lane] + 0.0;  // (no negative zero)
-            const uint64_t b = __builtin_bit_cast(uint64_t, l[i]);
-            key[i] = l[i] != l[i] ? ~0ull : b >> 63 ? ~b : b | 1ull << 63;
+        for (int i = 0; i < EACH; ++i) {
+            key[i] = 0;
+            l[i] = 0.0;
+            if (i * 64 + lane < experts) {
+                l[i] = logits[i * 64 + lane] + 0.0;  // (no negative zero)
+                const uint64_t b = __builtin_bit_cast(uint64_t, l[i]);
+                key[i] = l[i] != l[i] ? ~0ull : b >> 63 ? ~b : b | 1ull << 63;
+            }
         }
     }
-    double mine = 0.0, top = 0.0;
-    for (int j = 0; j < topk; ++j) {
+    // The j-th expert, the same in all lanes.
+    __device__ __forceinline__ int next(int j, int lane)
+    {
         uint64_t best = key[0];
         int at = 0;
         double value = l[0];
 #pragma unroll
         for (int i = 1; i < EACH; ++i)
-            if (i * 64 < experts && key[i] > best) {
+            if (key[i] > best) {
                 best = key[i];
                 at = i;
                 value = l[i];
@@ -174,18 +177,23 @@ __device__ inline float choose(const double* logits, int experts, int topk, int 
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
             if (lane == winner && i == at) key[i] = 0;
-        take(j, e);
+        return e;
     }
-    double all = 0.0;
-    if (normalize) {
-        all = lane < topk ? exp(mine - top) : 0.0;
-    } else {
+    // After all: the share of a lane's choice, in lanes below topk.
+    __device__ __forceinline__ float share(int experts, int topk, int normalize, int lane) const
+    {
+        const double own = exp(mine - top);
+        double all = 0.0;
+        if (normalize) {
+            all = lane < topk ? own : 0.0;
+        } else {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i)
-            if (i * 64 + lane < experts) all += exp(l[i] - top);
+            for (int i = 0; i < EACH; ++i)
+                if (i * 64 + lane < experts) all += exp(l[i] - top);
+        }
+        return (float)(own / sum64(all));
     }
-    return (float)(exp(mine - top) / sum64(all));
-}
+};
 
 // A chunk's choices, by expert, in tiles of `up_size` and of `down_size` tokens.
 template <int EACH>
@@ -199,11 +207,14 @@ __global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w
     __syncthreads();
     for (int t = wave; t < count; t += 16) {
         const int c0 = (t0 + t) * a.topk;
+        Chooser<EACH> from;
+        from.init((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts, lane);
         int mine = 0;
-        const float p = choose<EACH>((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts,
-                                     a.topk, a.normalize, lane, [&](int j, int e) {
-                                         if (lane == j) mine = e;
-                                     });
+        for (int k = 0; k < a.topk; ++k) {
+            const int e = from.next(k, lane);
+            if (lane == k) mine = e;
+        }
+        const float p = from.share(a.experts, a.topk, a.normalize, lane);
         if (lane < a.topk) {
             expert_of[t * a.topk + lane] = mine;
             atomicOr((unsigned long long*)&tokens_of[mine], 1ull << t);
@@ -259,83 +270,91 @@ __global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w
 
 // ---- the experts ----
 
-// A tile's product with 16 rows each of G and U.  ONE (EACH of choose, or 0): the only token's, tile j of
-// its j-th choice.
-template <typename T, int TOKENS, int WAVES, int ONE>
-__global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+// The hidden layer's values, times their shares, as pieces.
+template <typename T, int N>
+__device__ inline void store_act(const Mx4MoeArgs& a, const Mx4MoeWork& w, int choice, int unit, const float (&h)[8])
 {
-    constexpr int PIECES = kBf16Pieces<T>, PITCH = 20;
+    bf16x8 to[kActPieces<T>];
+    split(h, to);
+#pragma unroll
+    for (int n = 0; n < kActPieces<T>; ++n) {
+        uint8_t* at = a.work + w.act + n * w.act_stride + (size_t)choice * w.act_ld + 2 * unit;
+        const u32x4 v = __builtin_bit_cast(u32x4, to[n]);
+        if constexpr (N == 8)
+            *(u32x4*)at = v;
+        else
+            *(u32x2*)at = u32x2{v[0], v[1]};
+    }
+}
+__device__ inline float act_of(float gate, float up, float share) { return share * (gate / (1.0f + expf(-gate)) * up); }
+
+// The only token's: 16 units of the expert that is its choice blockIdx.y, by eight waves that share the terms.
+template <typename T, int EACH>
+__global__ void __launch_bounds__(512, 2) up_one_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    constexpr int WAVES = 8, TOKENS = 2, PIECES = kBf16Pieces<T>, PITCH = 20;
     constexpr int OWN = rows4_bytes(2) + tokens_bytes(PIECES, TOKENS), PART = 2 * 16 * PITCH * 4;
     __shared__ __align__(16) char lds[WAVES * (OWN > PART ? OWN : PART)];
-    __shared__ int choice_of[TOKENS];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int j0 = blockIdx.x * 16, tile = blockIdx.y;
-    int expert, count = 1;
-    float share = 0.0f;  // ONE: of the tile's choice
-    if constexpr (ONE) {
-        expert = 0;
-        int mine = 0;
-        const float p = choose<ONE>((const double*)(a.work + w.logits), a.experts, a.topk, a.normalize, lane,
-                                    [&](int j, int e) {
-                                        if (j == tile) expert = e;
-                                        if (lane == j) mine = e;
-                                    });
-        share = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), tile));
-        if (blockIdx.x == 0 && tile == 0 && wave == 0 && lane < a.topk) {
-            ((int*)(a.work + w.chosen))[lane] = mine;
-            if (a.weights) a.weights[lane] = p;
-            if (a.chosen) a.chosen[lane] = mine;
-        }
-    } else {
-        const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
-        if (tile >= tiles[0]) return;
-        expert = __builtin_amdgcn_readfirstlane(tiles[2 + tile]);
-        const int from = tiles[2 + kMoeTiles + tile];
-        count = __builtin_amdgcn_readfirstlane(tiles[2 + 2 * kMoeTiles + tile]);
-        if (threadIdx.x < TOKENS)
-            choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
-        __syncthreads();
+    const int j0 = blockIdx.x * 16, choice = blockIdx.y;
+    const int nb = (a.width + 31) / 32, groups = (nb + 7) / 8, rows = min(a.hidden - j0, 16);
+    PieceTokens<PIECES, TOKENS> sa;
+    sa.base = a.work + w.x;
+    sa.stride = w.x_stride;
+    sa.move([&](int t) { return t > 0 ? kOutside : 0; }, lane);
+    typename PieceTokens<PIECES, TOKENS>::Values x;
+    sa.load(x, min(wave, groups - 1));
+    Chooser<EACH> from;
+    from.init((const double*)(a.work + w.logits), a.experts, lane);
+    int expert = 0, mine = 0;
+    for (int k = 0; k <= choice; ++k) {
+        expert = from.next(k, lane);
+        if (lane == k) mine = expert;
     }
     char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(2);
-    const int nb = (a.width + 31) / 32, groups = (nb + 7) / 8, rows = min(a.hidden - j0, 16);
-    f32x4 acc[2] = {};
-    if (rows > 0) {
-        Source4<1> sg, su;
-        sg.init(a.ld1, a.lds1, rows, nb, lane);
-        sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + j0);
-        su = sg;
-        su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + j0);
-        PieceTokens<PIECES, TOKENS> sa;
-        sa.base = a.work + w.x;
-        sa.stride = w.x_stride;
-        sa.move([&](int t) { return t >= count ? kOutside : ONE ? 0 : choice_of[t] / a.topk * w.x_ld; }, lane);
-        Rows4<1> wg[2], wu[2];
-        typename PieceTokens<PIECES, TOKENS>::Values x;
+    f32x4 acc[1][2] = {};
+    Source4<1> sg, su;
+    sg.init(a.ld1, a.lds1, rows > 0 ? rows : 1, nb, lane);
+    su = sg;
+    // (past the last unit: the last one's rows, not used)
+    sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + min(j0, a.hidden - 1));
+    su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
+    Rows4<1> wg[2], wu[2];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        const int g = wave + d * WAVES;
+        sg.load(wg[d], g, nb - 8 * g);
+        su.load(wu[d], g, nb - 8 * g);
+    }
+    // the other choices, and the shares, while the weights are under way
+    for (int k = choice + 1; k < a.topk; ++k) {
+        const int e = from.next(k, lane);
+        if (lane == k) mine = e;
+    }
+    const float shares = from.share(a.experts, a.topk, a.normalize, lane);
+    const float share = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, shares), choice));
+    if (blockIdx.x == 0 && choice == 0 && wave == 0 && lane < a.topk) {
+        ((int*)(a.work + w.chosen))[lane] = mine;
+        if (a.weights) a.weights[lane] = shares;
+        if (a.chosen) a.chosen[lane] = mine;
+    }
+    for (int g = wave; g < groups;) {
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
-            const int g = wave + d * WAVES;
-            sg.load(wg[d], g, nb - 8 * g);
-            su.load(wu[d], g, nb - 8 * g);
-        }
-        sa.load(x, min(wave, groups - 1));
-        for (int g = wave; g < groups;) {
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                bf16x8 v[2][8];
-                if (nb - 8 * g < 8) {
-                    wg[d].code[0] = first_codes(wg[d].code[0], nb - 8 * g);
-                    wu[d].code[0] = first_codes(wu[d].code[0], nb - 8 * g);
-                }
-                const Rows4<2> both = {{wg[d].v[0], wg[d].v[1], wu[d].v[0], wu[d].v[1]}, {wg[d].code[0], wu[d].code[0]}};
-                fragments(both, own, lane, v);
-                sg.load(wg[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
-                su.load(wu[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
-                sa.put(x, tokens_at, lane);
-                sa.load(x, min(g + WAVES, groups - 1));
-                multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
-                g += WAVES;
-                if (g >= groups) break;
+            bf16x8 v[2][8];
+            if (nb - 8 * g < 8) {
+                wg[d].code[0] = first_codes(wg[d].code[0], nb - 8 * g);
+                wu[d].code[0] = first_codes(wu[d].code[0], nb - 8 * g);
             }
+            const Rows4<2> both = {{wg[d].v[0], wg[d].v[1], wu[d].v[0], wu[d].v[1]}, {wg[d].code[0], wu[d].code[0]}};
+            fragments(both, own, lane, v);
+            sg.load(wg[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
+            su.load(wu[d], g + 2 * WAVES, nb - 8 * (g + 2 * WAVES));
+            sa.put(x, tokens_at, lane);
+            sa.load(x, min(g + WAVES, groups - 1));
+            multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
+            g += WAVES;
+            if (g >= groups) break;
         }
     }
     __syncthreads();
@@ -344,31 +363,131 @@ __global__ void __launch_bounds__(64 * WAVES, 2) up_kernel(Mx4MoeArgs a, Mx4MoeW
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part[((wave * 2 + i) * 16 + 4 * q + e) * PITCH + r] = acc[i][e];
+        for (int e = 0; e < 4; ++e) part[((wave * 2 + i) * 16 + 4 * q + e) * PITCH + r] = acc[0][i][e];
     __syncthreads();
-    // 8 units a thread, and zeros past the last one, to the row's end
-    for (int t = threadIdx.x; t < 2 * TOKENS; t += 64 * WAVES) {
-        const int token = t / 2, u0 = t % 2 * 8;
-        if (token >= count) continue;
-        const int choice = ONE ? tile : choice_of[token];
-        const float p = ONE ? share : ((const float*)(a.work + w.weights))[choice];
-        float h[8];
+    if (threadIdx.x >= 16) return;
+    // a unit a thread, and zeros past the last one, to the row's end
+    float g = 0.0f, u = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float g = 0.0f, u = 0.0f;
+    for (int v = 0; v < WAVES; ++v)
 #pragma unroll
-            for (int v = 0; v < WAVES; ++v) {
-                g += part[((v * 2) * 16 + u0 + i) * PITCH + token];
-                u += part[((v * 2 + 1) * 16 + u0 + i) * PITCH + token];
-            }
-            h[i] = u0 + i < rows ? p * (g / (1.0f + expf(-g)) * u) : 0.0f;
+        for (int n = 0; n < PIECES; ++n) {
+            g += part[((v * 2) * 16 + threadIdx.x) * PITCH + n * TOKENS];
+            u += part[((v * 2 + 1) * 16 + threadIdx.x) * PITCH + n * TOKENS];
         }
-        bf16x8 to[kActPieces<T>];
-        split(h, to);
+    const float h = (int)threadIdx.x < rows ? act_of(g, u, share) : 0.0f;
+    float all[8];
 #pragma unroll
-        for (int n = 0; n < kActPieces<T>; ++n)
-            *(bf16x8*)(a.work + w.act + n * w.act_stride + (size_t)choice * w.act_ld + 2 * (j0 + u0)) = to[n];
+    for (int i = 0; i < 8; ++i) all[i] = __shfl(h, (int)(threadIdx.x * 8 + i) % 16);
+    if (threadIdx.x < 2) store_act<T, 8>(a, w, choice, j0 + 8 * threadIdx.x, all);
+}
+
+// A wave's sums of a tile (PIECES of a token in as many columns), of tokens lane % TOKENS.
+template <int PIECES, int TOKENS, int N>
+__device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKENS)][N], int i)
+{
+    f32x4 v = acc[0][i];
+    if constexpr (TOKENS == 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], 8);  // (the same in either order)
+        if constexpr (PIECES == 3) v += acc[1][i];
     }
+    return v;
+}
+
+// A tile's tokens by 16 units of each of four waves; the tokens' terms are in LDS for all of them, a group
+// after another.
+constexpr int kUpWaves = 4;
+template <typename T, int TOKENS>
+__global__ void __launch_bounds__(64 * kUpWaves) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    constexpr int PIECES = kBf16Pieces<T>, STAGE = tokens_bytes(PIECES, TOKENS);
+    constexpr int LOADS = TOKENS * 32 / (64 * kUpWaves) ? TOKENS * 32 / (64 * kUpWaves) : 1;  // a thread's, of a piece
+    __shared__ __align__(16) char lds[2 * STAGE + kUpWaves * rows4_bytes(2)];
+    __shared__ int choice_of[TOKENS];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), tile = blockIdx.y;
+    const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
+    if (tile >= tiles[0]) return;
+    const int expert = __builtin_amdgcn_readfirstlane(tiles[2 + tile]), from = tiles[2 + kMoeTiles + tile];
+    const int count = __builtin_amdgcn_readfirstlane(tiles[2 + 2 * kMoeTiles + tile]);
+    const int j0 = (blockIdx.x * kUpWaves + wave) * 16, nb = (a.width + 31) / 32, groups = (nb + 7) / 8;
+    const int rows = min(a.hidden - j0, 16);
+    char* own = lds + 2 * STAGE + wave * rows4_bytes(2);
+    Source4<1> sg, su;
+    sg.init(a.ld1, a.lds1, rows > 0 ? rows : 1, nb, lane);
+    su = sg;
+    // (past the last unit: the last one's rows, not used)
+    sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + min(j0, a.hidden - 1));
+    su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
+    Rows4<1> wg[2], wu[2];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        sg.load(wg[d], d, nb - 8 * d);
+        su.load(wu[d], d, nb - 8 * d);
+    }
+    if (threadIdx.x < TOKENS)
+        choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
+    __syncthreads();
+    // a thread's chunks of the tile: token (threadIdx.x + 256 i) / 32
+    int at[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int t = (threadIdx.x + 64 * kUpWaves * i) / 32;
+        at[i] = t < count ? choice_of[t] / a.topk * w.x_ld + lane % 32 * 16 : kOutside;
+    }
+    u32x4 x[LOADS][PIECES];
+    auto load_tokens = [&](int g) {
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const __amdgpu_buffer_rsrc_t v = buffer_of(a.work + w.x + n * w.x_stride, 0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                x[i][n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], g * 512, 0));
+        }
+    };
+    auto put_tokens = [&](char* to) {
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int row = n * TOKENS + (threadIdx.x + 64 * kUpWaves * i) / 32;
+                *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
+            }
+    };
+    auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (loads go on)
+    f32x4 acc[fragments_of(PIECES, TOKENS)][2] = {};
+    load_tokens(0);
+    put_tokens(lds);
+    load_tokens(min(1, groups - 1));
+    barrier();
+    for (int g = 0; g < groups;) {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {  // (stage g % 2)
+            bf16x8 v[2][8];
+            if (nb - 8 * g < 8) {
+                wg[d].code[0] = first_codes(wg[d].code[0], nb - 8 * g);
+                wu[d].code[0] = first_codes(wu[d].code[0], nb - 8 * g);
+            }
+            const Rows4<2> both = {{wg[d].v[0], wg[d].v[1], wu[d].v[0], wu[d].v[1]}, {wg[d].code[0], wu[d].code[0]}};
+            fragments(both, own, lane, v);
+            sg.load(wg[d], g + 2, nb - 8 * (g + 2));
+            su.load(wu[d], g + 2, nb - 8 * (g + 2));
+            // the next stage: its last readers passed the barrier before
+            put_tokens(lds + (1 - d) * STAGE);
+            load_tokens(min(g + 2, groups - 1));
+            multiply<PIECES, TOKENS>(acc, v, lds + d * STAGE, lane);
+            barrier();
+            if (++g >= groups) break;
+        }
+    }
+    const int t = lane % TOKENS, q = lane / 16;
+    const f32x4 gate = token_sums<PIECES, TOKENS>(acc, 0), up = token_sums<PIECES, TOKENS>(acc, 1);
+    if (lane % 16 >= count || lane % 16 >= TOKENS) return;
+    const float share = ((const float*)(a.work + w.weights))[choice_of[t]];
+    float h[8] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = 4 * q + e < rows ? act_of(gate[e], up[e], share) : 0.0f;
+    store_act<T, 4>(a, w, choice_of[t], j0 + 4 * q, h);
 }
 
 // 16 results of a chunk's tokens.  Its tiles times their groups of terms are cut into one run for each
@@ -420,7 +539,7 @@ __global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWo
             sa.load(x, p.g);
         };
         Rows4<1> rows[2];
-        f32x4 acc[1] = {};
+        f32x4 acc[fragments_of(PIECES, TOKENS)][1] = {};
         Place now{from / groups, from % groups}, next = after(now);
         load_rows(rows[0], now);
         load_rows(rows[1], next);
@@ -439,15 +558,25 @@ __global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWo
                 ++u;
                 if (u == to || next.tile != now.tile) {
                     const int r = lane % 16, q = lane / 16;
-                    int token = r < 1 ? 0 : -1;
-                    if constexpr (!ONE) {
+                    f32x4 v4;
+                    int token;
+                    if constexpr (ONE) {  // pieces in columns 0, 2 and 4
+                        v4 = acc[0][0];
+#pragma unroll
+                        for (int n = 1; n < PIECES; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v4[e] += __shfl_down(acc[0][0][e], 2 * n);
+                        token = r == 0 ? 0 : -1;
+                    } else {
+                        v4 = token_sums<PIECES, TOKENS>(acc, 0);
                         const int first = experts[kMoeTiles + now.tile], n = experts[2 * kMoeTiles + now.tile];
                         token = r < n ? choices[first + r] / a.topk - t0 : -1;
                     }
                     if (token >= 0)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) part[wave][token * PITCH + 4 * q + e] += acc[0][e];
-                    acc[0] = f32x4{};
+                        for (int e = 0; e < 4; ++e) part[wave][token * PITCH + 4 * q + e] += v4[e];
+#pragma unroll
+                    for (int f = 0; f < fragments_of(PIECES, TOKENS); ++f) acc[f][0] = f32x4{};
                 }
                 now = next;
                 next = then;
@@ -479,11 +608,11 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
         prepare_kernel<T, 1><<<prepare_x, 256, 0, s>>>(a, w, expert_groups);
         const dim3 up(up_x, (unsigned)a.topk);
         if (a.experts <= 64)
-            up_kernel<T, 2, 8, 1><<<up, 512, 0, s>>>(a, w);
+            up_one_kernel<T, 1><<<up, 512, 0, s>>>(a, w);
         else if (a.experts <= 128)
-            up_kernel<T, 2, 8, 2><<<up, 512, 0, s>>>(a, w);
+            up_one_kernel<T, 2><<<up, 512, 0, s>>>(a, w);
         else
-            up_kernel<T, 2, 8, 8><<<up, 512, 0, s>>>(a, w);
+            up_one_kernel<T, 8><<<up, 512, 0, s>>>(a, w);
         down_kernel<T, 2, 16, true><<<down_x, 1024, 0, s>>>(a, w);
     } else {
         prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
@@ -495,7 +624,7 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
             choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
         const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
         const int most = a.experts + choices / UP < choices ? a.experts + choices / UP : choices;
-        up_kernel<T, UP, 4, 0><<<dim3(up_x, (unsigned)most, chunks), 256, 0, s>>>(a, w);
+        up_kernel<T, UP><<<dim3(up_x / kUpWaves, (unsigned)most, chunks), 64 * kUpWaves, 0, s>>>(a, w);
         down_kernel<T, DOWN, 8, false><<<dim3(down_x, chunks), 512, 0, s>>>(a, w);
     }
     return hipGetLastError();

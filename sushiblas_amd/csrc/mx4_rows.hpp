@@ -190,27 +190,31 @@ __device__ inline void split(const float (&x)[8], bf16x8 (&to)[N])
 }
 
 // 256 terms of a tile of TOKENS (2, 8 or 16) tokens: a lane loads 8 terms, 8 (lane % 32) .., of tokens
-// 2 i + lane / 32, makes their pieces, and writes them to the wave's LDS.  Chunk c (8 terms) of
-// token t lies at place c ^ t of its 512 bytes, for the same reason as above.
+// 2 i + lane / 32, makes their pieces, and writes them to LDS.  Piece n of token t is row x = n TOKENS + t
+// there, of 512 bytes, its chunk c (8 terms) at place c ^ (x % 16), for the same reason as above.
+//   A fragment's 16 rows are 16 of these, pieces of a token among them: so that fp16's two of 8 tokens take
+// one instruction a block, as bf16's 16 tokens do, and three of two tokens one.  Each piece has sums of its
+// own, added at the end, the largest piece's first.
 constexpr int tokens_bytes(int pieces, int tokens) { return 512 * pieces * tokens; }
+constexpr int fragments_of(int pieces, int tokens) { return (pieces * tokens + 15) / 16; }
 
 template <int PIECES, int TOKENS>
 __device__ inline void put_tokens(char* lds, int i, int lane, const bf16x8 (&x)[PIECES])
 {
-    const int t = 2 * i + lane / 32;
 #pragma unroll
-    for (int n = 0; n < PIECES; ++n)
-        *(bf16x8*)(lds + (n * TOKENS + t) * 512 + (lane % 32 ^ t) * 16) = x[n];
+    for (int n = 0; n < PIECES; ++n) {
+        const int row = n * TOKENS + 2 * i + lane / 32;
+        *(bf16x8*)(lds + row * 512 + (lane % 32 ^ row % 16) * 16) = x[n];
+    }
 }
 
-// A block's fragment: token lane % 16 of the tile (those past a smaller tile: again from its first).
+// A block's fragment f: rows 16 f + lane % 16 (past the last: again the first ones, whose sums nobody takes).
 template <int PIECES, int TOKENS>
-__device__ inline void get_tokens(const char* lds, int b, int lane, bf16x8 (&x)[PIECES])
+__device__ inline bf16x8 get_tokens(const char* lds, int b, int f, int lane)
 {
-    const int t = lane % TOKENS;
-#pragma unroll
-    for (int n = 0; n < PIECES; ++n)
-        x[n] = *(const bf16x8*)(lds + (n * TOKENS + t) * 512 + (4 * b + lane / 16 ^ t) * 16);
+    constexpr int ROWS = PIECES * TOKENS;
+    const int row = ROWS >= 16 * f + 16 ? 16 * f + lane % 16 : 16 * f + lane % 16 % (ROWS - 16 * f);
+    return *(const bf16x8*)(lds + row * 512 + (4 * b + lane / 16 ^ row % 16) * 16);
 }
 
 // Tokens of type T: rows anywhere within 2 GiB.
@@ -370,21 +374,21 @@ struct PieceTokens {
     }
 };
 
-// acc[i]: rows 4 (lane / 16) + e of block i of w, token lane % 16 of the tile in the wave's LDS.
+// acc[f][i]: rows 4 (lane / 16) + e of block i of w, row 16 f + lane % 16 of the tile in LDS.
 template <int PIECES, int TOKENS, int N>
-__device__ inline void multiply(f32x4 (&acc)[N], const bf16x8 (&w)[N][8], const char* lds, int lane)
+__device__ inline void multiply(f32x4 (&acc)[fragments_of(PIECES, TOKENS)][N], const bf16x8 (&w)[N][8], const char* lds,
+                                int lane)
 {
     in_order();
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-        bf16x8 x[PIECES];
-        get_tokens<PIECES, TOKENS>(lds, b, lane, x);
+    for (int b = 0; b < 8; ++b)
 #pragma unroll
-        for (int n = 0; n < PIECES; ++n)
+        for (int f = 0; f < fragments_of(PIECES, TOKENS); ++f) {
+            const bf16x8 x = get_tokens<PIECES, TOKENS>(lds, b, f, lane);
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][b], x[n], acc[i], 0, 0, 0);
-    }
+                acc[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][b], x, acc[f][i], 0, 0, 0);
+        }
     in_order();
 }
 
