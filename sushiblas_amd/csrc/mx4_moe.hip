@@ -5,9 +5,10 @@
 //   prepare  the router's logits, and the tokens as bf16 pieces
 //   choose   (more than one token) each token's experts and shares, the choices sorted by expert,
 //            in tiles of a few tokens of one expert
-//   up       a tile by 16 units of the hidden layer: share * silu(G x) * (U x), as bf16 pieces; of
-//            one token it chooses itself, which costs less than a launch
-//   down     16 results of all of a chunk's tokens: the sum over its tiles, which the waves share
+//   up       a tile by 16 units of the hidden layer a wave: share * silu(G x) * (U x), as bf16 pieces;
+//            of one token it chooses itself, which costs less than a launch
+//   down     a tile by 32 results; of one token, 16 results over all of its choices, which the waves share
+//   combine  (more than one token) the sum over a token's choices
 // Products and pieces: mx4_rows.hpp.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -395,94 +396,127 @@ __device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKEN
     return v;
 }
 
-// A tile's tokens by 16 units of each of four waves; the tokens' terms are in LDS for all of them, a group
-// after another.
-constexpr int kUpWaves = 4;
+// A tile's tokens times two blocks of 16 rows of each of four waves.  The tokens' terms are in LDS for
+// all of them, a group after another, the next one on its way; rows stay within a wave (mx4_rows.hpp).
+constexpr int kTileWaves = 4;
+template <int PIECES, int TOKENS>
+struct TileProduct {
+    static constexpr int STAGE = tokens_bytes(PIECES, TOKENS), BYTES = 2 * STAGE + kTileWaves * rows4_bytes(2);
+    // a thread's chunks of a piece: of tokens (threadIdx.x + 256 i) / 32
+    static constexpr int LOADS = TOKENS * 32 / (64 * kTileWaves);
+    f32x4 acc[fragments_of(PIECES, TOKENS)][2];
+
+    // s0, s1: the rows, at least one of each; x: the tokens' pieces, `stride` apart, token t's offset_of(t)
+    // bytes from there or not there (kOutside).
+    template <typename F>
+    __device__ inline void run(const Source4<1>& s0, const Source4<1>& s1, int nb, const uint8_t* tokens, int64_t stride,
+                               F&& offset_of, char* lds, int lane, int wave)
+    {
+        const int groups = (nb + 7) / 8;
+        char* own = lds + 2 * STAGE + wave * rows4_bytes(2);
+        int at[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int from = offset_of((threadIdx.x + 64 * kTileWaves * i) / 32);
+            at[i] = from == kOutside ? kOutside : from + lane % 32 * 16;
+        }
+        u32x4 x[LOADS][PIECES];
+        auto load_tokens = [&](int g) {
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) {
+                const __amdgpu_buffer_rsrc_t v = buffer_of(tokens + n * stride, 0x7fffffff);
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i)
+                    x[i][n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], g * 512, 0));
+            }
+        };
+        auto put_tokens = [&](char* to) {
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int row = n * TOKENS + (threadIdx.x + 64 * kTileWaves * i) / 32;
+                    *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
+                }
+        };
+        auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (loads go on)
+        Rows4<1> w0[2], w1[2];
+        load_tokens(0);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            s0.load(w0[d], d, nb - 8 * d);
+            s1.load(w1[d], d, nb - 8 * d);
+        }
+        put_tokens(lds);
+        load_tokens(min(1, groups - 1));
+        barrier();
+#pragma unroll
+        for (int f = 0; f < fragments_of(PIECES, TOKENS); ++f) acc[f][0] = acc[f][1] = f32x4{};
+        for (int g = 0; g < groups;) {
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {  // (stage g % 2)
+                bf16x8 v[2][8];
+                if (nb - 8 * g < 8) {
+                    w0[d].code[0] = first_codes(w0[d].code[0], nb - 8 * g);
+                    w1[d].code[0] = first_codes(w1[d].code[0], nb - 8 * g);
+                }
+                const Rows4<2> both = {{w0[d].v[0], w0[d].v[1], w1[d].v[0], w1[d].v[1]}, {w0[d].code[0], w1[d].code[0]}};
+                fragments(both, own, lane, v);
+                s0.load(w0[d], g + 2, nb - 8 * (g + 2));
+                s1.load(w1[d], g + 2, nb - 8 * (g + 2));
+                put_tokens(lds + (1 - d) * STAGE);  // its last readers passed the barrier before
+                load_tokens(min(g + 2, groups - 1));
+                multiply<PIECES, TOKENS>(acc, v, lds + d * STAGE, lane);
+                barrier();
+                if (++g >= groups) break;
+            }
+        }
+    }
+};
+
+// What a tile's kernel finds in the list of tiles.
+template <int TOKENS>
+struct Tile {
+    int expert, count;
+    __device__ inline bool find(const Mx4MoeArgs& a, const Mx4MoeWork& w, int list, int (&choice_of)[TOKENS])
+    {
+        const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
+        const int* own = tiles + 2 + list * 3 * kMoeTiles + blockIdx.y;
+        if ((int)blockIdx.y >= tiles[list]) return false;
+        expert = __builtin_amdgcn_readfirstlane(own[0]);
+        count = __builtin_amdgcn_readfirstlane(own[2 * kMoeTiles]);
+        const int from = own[kMoeTiles];
+        if (threadIdx.x < TOKENS)
+            choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
+        __syncthreads();
+        return true;
+    }
+};
+
+// 16 units a wave: its rows of G and of U.
 template <typename T, int TOKENS>
-__global__ void __launch_bounds__(64 * kUpWaves) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+__global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
-    constexpr int PIECES = kBf16Pieces<T>, STAGE = tokens_bytes(PIECES, TOKENS);
-    constexpr int LOADS = TOKENS * 32 / (64 * kUpWaves) ? TOKENS * 32 / (64 * kUpWaves) : 1;  // a thread's, of a piece
-    __shared__ __align__(16) char lds[2 * STAGE + kUpWaves * rows4_bytes(2)];
+    constexpr int PIECES = kBf16Pieces<T>;
+    typedef TileProduct<PIECES, TOKENS> product_t;
+    __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ int choice_of[TOKENS];
-    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), tile = blockIdx.y;
-    const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
-    if (tile >= tiles[0]) return;
-    const int expert = __builtin_amdgcn_readfirstlane(tiles[2 + tile]), from = tiles[2 + kMoeTiles + tile];
-    const int count = __builtin_amdgcn_readfirstlane(tiles[2 + 2 * kMoeTiles + tile]);
-    const int j0 = (blockIdx.x * kUpWaves + wave) * 16, nb = (a.width + 31) / 32, groups = (nb + 7) / 8;
-    const int rows = min(a.hidden - j0, 16);
-    char* own = lds + 2 * STAGE + wave * rows4_bytes(2);
+    Tile<TOKENS> tile;
+    if (!tile.find(a, w, 0, choice_of)) return;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int j0 = (blockIdx.x * kTileWaves + wave) * 16, nb = (a.width + 31) / 32, rows = min(a.hidden - j0, 16);
     Source4<1> sg, su;
     sg.init(a.ld1, a.lds1, rows > 0 ? rows : 1, nb, lane);
     su = sg;
     // (past the last unit: the last one's rows, not used)
-    sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + min(j0, a.hidden - 1));
-    su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
-    Rows4<1> wg[2], wu[2];
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-        sg.load(wg[d], d, nb - 8 * d);
-        su.load(wu[d], d, nb - 8 * d);
-    }
-    if (threadIdx.x < TOKENS)
-        choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
-    __syncthreads();
-    // a thread's chunks of the tile: token (threadIdx.x + 256 i) / 32
-    int at[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int t = (threadIdx.x + 64 * kUpWaves * i) / 32;
-        at[i] = t < count ? choice_of[t] / a.topk * w.x_ld + lane % 32 * 16 : kOutside;
-    }
-    u32x4 x[LOADS][PIECES];
-    auto load_tokens = [&](int g) {
-#pragma unroll
-        for (int n = 0; n < PIECES; ++n) {
-            const __amdgpu_buffer_rsrc_t v = buffer_of(a.work + w.x + n * w.x_stride, 0x7fffffff);
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i)
-                x[i][n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], g * 512, 0));
-        }
-    };
-    auto put_tokens = [&](char* to) {
-#pragma unroll
-        for (int n = 0; n < PIECES; ++n)
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int row = n * TOKENS + (threadIdx.x + 64 * kUpWaves * i) / 32;
-                *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
-            }
-    };
-    auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (loads go on)
-    f32x4 acc[fragments_of(PIECES, TOKENS)][2] = {};
-    load_tokens(0);
-    put_tokens(lds);
-    load_tokens(min(1, groups - 1));
-    barrier();
-    for (int g = 0; g < groups;) {
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {  // (stage g % 2)
-            bf16x8 v[2][8];
-            if (nb - 8 * g < 8) {
-                wg[d].code[0] = first_codes(wg[d].code[0], nb - 8 * g);
-                wu[d].code[0] = first_codes(wu[d].code[0], nb - 8 * g);
-            }
-            const Rows4<2> both = {{wg[d].v[0], wg[d].v[1], wu[d].v[0], wu[d].v[1]}, {wg[d].code[0], wu[d].code[0]}};
-            fragments(both, own, lane, v);
-            sg.load(wg[d], g + 2, nb - 8 * (g + 2));
-            su.load(wu[d], g + 2, nb - 8 * (g + 2));
-            // the next stage: its last readers passed the barrier before
-            put_tokens(lds + (1 - d) * STAGE);
-            load_tokens(min(g + 2, groups - 1));
-            multiply<PIECES, TOKENS>(acc, v, lds + d * STAGE, lane);
-            barrier();
-            if (++g >= groups) break;
-        }
-    }
-    const int t = lane % TOKENS, q = lane / 16;
-    const f32x4 gate = token_sums<PIECES, TOKENS>(acc, 0), up = token_sums<PIECES, TOKENS>(acc, 1);
-    if (lane % 16 >= count || lane % 16 >= TOKENS) return;
+    sg.move(a.W1, a.S1, (int64_t)tile.expert * 2 * a.hidden + min(j0, a.hidden - 1));
+    su.move(a.W1, a.S1, (int64_t)tile.expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
+    product_t product;
+    product.run(sg, su, nb, a.work + w.x, w.x_stride,
+                [&](int t) { return t < tile.count ? choice_of[t] / a.topk * w.x_ld : kOutside; }, lds, lane, wave);
+    const int t = lane % 16, q = lane / 16;
+    const f32x4 gate = token_sums<PIECES, TOKENS>(product.acc, 0), up = token_sums<PIECES, TOKENS>(product.acc, 1);
+    if (t >= tile.count || t >= TOKENS) return;
     const float share = ((const float*)(a.work + w.weights))[choice_of[t]];
     float h[8] = {};
 #pragma unroll
@@ -490,56 +524,92 @@ __global__ void __launch_bounds__(64 * kUpWaves) up_kernel(Mx4MoeArgs a, Mx4MoeW
     store_act<T, 4>(a, w, choice_of[t], j0 + 4 * q, h);
 }
 
-// 16 results of a chunk's tokens.  Its tiles times their groups of terms are cut into one run for each
-// wave; a wave adds a tile's sums to its tokens' in LDS when it leaves it, and the waves' are added up at
-// the end, in order.  ONE: the only token's.
-template <typename T, int TOKENS, int WAVES, bool ONE>
-__global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+// 32 results a wave, of each choice apart.
+template <typename T, int TOKENS>
+__global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
-    constexpr int PIECES = kActPieces<T>, OWN = rows4_bytes(1) + tokens_bytes(PIECES, TOKENS);
-    constexpr int MOST = ONE ? 1 : kMoeChunk, PITCH = 17;
-    __shared__ __align__(16) char lds[WAVES * OWN];
-    __shared__ float part[WAVES][MOST * PITCH];
+    constexpr int PIECES = kActPieces<T>;
+    typedef TileProduct<PIECES, TOKENS> product_t;
+    __shared__ __align__(16) char lds[product_t::BYTES];
+    __shared__ int choice_of[TOKENS];
+    Tile<TOKENS> tile;
+    if (!tile.find(a, w, 1, choice_of)) return;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int n0 = blockIdx.x * 16, t0 = blockIdx.y * kMoeChunk, count = min(a.tokens - t0, MOST);
-    const int* tiles = (const int*)(a.work + w.tiles + blockIdx.y * w.tiles_bytes);
-    const int *experts = ONE ? (const int*)(a.work + w.chosen) : tiles + 2 + 3 * kMoeTiles, *choices = tiles + 2 + 6 * kMoeTiles;
-    const int tile_count = ONE ? a.topk : tiles[1];
+    const int n0 = (blockIdx.x * kTileWaves + wave) * 32, nb = (a.hidden + 31) / 32;
+    Source4<1> s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // (past the last row: that one, not used)
+        const int at = min(n0 + 16 * i, a.width - 1);
+        s[i].init(a.ld2, a.lds2, a.width - at, nb, lane);
+        s[i].move(a.W2, a.S2, (int64_t)tile.expert * a.width + at);
+    }
+    const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
+    product_t product;
+    product.run(s[0], s[1], nb, a.work + w.act + (size_t)first * w.act_ld, w.act_stride,
+                [&](int t) { return t < tile.count ? (choice_of[t] - first) * w.act_ld : kOutside; }, lds, lane, wave);
+    const int t = lane % 16, q = lane / 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x4 v = token_sums<PIECES, TOKENS>(product.acc, i);
+        const int n = n0 + 16 * i + 4 * q;
+        // (rows of `out` are whole 16 bytes)
+        if (t < tile.count && t < TOKENS && n < a.width)
+            *(f32x4*)(a.work + w.out + ((size_t)choice_of[t] * w.out_ld + n) * 4) = v;
+    }
+}
+
+// A token's sum over its choices, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 4, t = blockIdx.y;
+    if (n >= a.width) return;
+    const float* from = (const float*)(a.work + w.out) + (size_t)t * a.topk * w.out_ld + n;
+    f32x4 v = *(const f32x4*)from;
+#pragma unroll 4
+    for (int j = 1; j < a.topk; ++j) v += *(const f32x4*)(from + (size_t)j * w.out_ld);
+    T* y = (T*)a.Y + t * a.ldy + n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < a.width) y[e] = (T)v[e];
+}
+
+// The only token's: 16 results a workgroup.  Its choices times their groups of terms are cut into one run
+// for each of 16 waves, whose sums are added up in LDS, in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+{
+    constexpr int WAVES = 16, TOKENS = 2, PIECES = kActPieces<T>, OWN = rows4_bytes(1) + tokens_bytes(PIECES, TOKENS);
+    __shared__ __align__(16) char lds[WAVES * OWN];
+    __shared__ float part[WAVES][16];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n0 = blockIdx.x * 16, *experts = (const int*)(a.work + w.chosen);
     char *own = lds + wave * OWN, *tokens_at = own + rows4_bytes(1);
     const int nb = (a.hidden + 31) / 32, groups = (nb + 7) / 8;
-    for (int i = lane; i < MOST * PITCH; i += 64) part[wave][i] = 0.0f;
-
-    const int units = tile_count * groups, from = (int)((int64_t)units * wave / WAVES),
-              to = (int)((int64_t)units * (wave + 1) / WAVES);
+    const int units = a.topk * groups, from = units * wave / WAVES, to = units * (wave + 1) / WAVES;
+    f32x4 acc[1][1] = {};
     if (from < to) {
-        struct Place {  // a tile and a group of its terms
-            int tile, g;
+        struct Place {  // a choice and a group of its terms
+            int choice, g;
         };
-        auto after = [&](Place p) { return p.g + 1 < groups ? Place{p.tile, p.g + 1} : Place{p.tile + 1, 0}; };
+        auto after = [&](Place p) { return p.g + 1 < groups ? Place{p.choice, p.g + 1} : Place{p.choice + 1, 0}; };
         Source4<1> sw;
         sw.init(a.ld2, a.lds2, a.width - n0, nb, lane);
         PieceTokens<PIECES, TOKENS> sa;
-        sa.base = a.work + w.act + (size_t)(t0 * a.topk) * w.act_ld;
+        sa.base = a.work + w.act;
         sa.stride = w.act_stride;
-        auto load_rows = [&](Rows4<1>& d, Place p) {  // (past the last tile: the last one again)
-            const int e = __builtin_amdgcn_readfirstlane(experts[min(p.tile, tile_count - 1)]);
+        auto load_rows = [&](Rows4<1>& d, Place p) {  // (past the last choice: the last one again)
+            const int e = __builtin_amdgcn_readfirstlane(experts[min(p.choice, a.topk - 1)]);
             sw.move(a.W2, a.S2, (int64_t)e * a.width + n0);
             sw.load(d, p.g, nb - 8 * p.g);
         };
         typename PieceTokens<PIECES, TOKENS>::Values x;
         auto load_tokens = [&](Place p) {
-            if constexpr (ONE) {
-                const int row = min(p.tile, tile_count - 1) * w.act_ld;
-                sa.move([&](int t) { return t > 0 ? kOutside : row; }, lane);
-            } else {
-                const int tile = min(p.tile, tile_count - 1), first = experts[kMoeTiles + tile],
-                          n = experts[2 * kMoeTiles + tile];
-                sa.move([&](int t) { return t < n ? (choices[first + t] - t0 * a.topk) * w.act_ld : kOutside; }, lane);
-            }
+            const int row = min(p.choice, a.topk - 1) * w.act_ld;
+            sa.move([&](int t) { return t > 0 ? kOutside : row; }, lane);
             sa.load(x, p.g);
         };
         Rows4<1> rows[2];
-        f32x4 acc[fragments_of(PIECES, TOKENS)][1] = {};
         Place now{from / groups, from % groups}, next = after(now);
         load_rows(rows[0], now);
         load_rows(rows[1], next);
@@ -555,44 +625,28 @@ __global__ void __launch_bounds__(64 * WAVES) down_kernel(Mx4MoeArgs a, Mx4MoeWo
                 sa.put(x, tokens_at, lane);
                 load_tokens(next);
                 multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
-                ++u;
-                if (u == to || next.tile != now.tile) {
-                    const int r = lane % 16, q = lane / 16;
-                    f32x4 v4;
-                    int token;
-                    if constexpr (ONE) {  // pieces in columns 0, 2 and 4
-                        v4 = acc[0][0];
-#pragma unroll
-                        for (int n = 1; n < PIECES; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v4[e] += __shfl_down(acc[0][0][e], 2 * n);
-                        token = r == 0 ? 0 : -1;
-                    } else {
-                        v4 = token_sums<PIECES, TOKENS>(acc, 0);
-                        const int first = experts[kMoeTiles + now.tile], n = experts[2 * kMoeTiles + now.tile];
-                        token = r < n ? choices[first + r] / a.topk - t0 : -1;
-                    }
-                    if (token >= 0)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) part[wave][token * PITCH + 4 * q + e] += v4[e];
-#pragma unroll
-                    for (int f = 0; f < fragments_of(PIECES, TOKENS); ++f) acc[f][0] = f32x4{};
-                }
                 now = next;
                 next = then;
-                if (u == to) break;
+                if (++u == to) break;
             }
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < count * 16; i += 64 * WAVES) {
-        const int t = i / 16, n = n0 + i % 16;
-        if (n >= a.width) continue;
-        float y = 0.0f;
+    // pieces are in columns 0, 2 and 4
+    f32x4 sum = acc[0][0];
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) y += part[v][t * PITCH + i % 16];
-        ((T*)a.Y)[(t0 + t) * a.ldy + n] = (T)y;
-    }
+    for (int n = 1; n < PIECES; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_down(acc[0][0][e], 2 * n);
+    if (lane % 16 == 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[wave][lane / 4 + e] = sum[e];
+    __syncthreads();
+    const int n = n0 + (int)threadIdx.x;
+    if (threadIdx.x >= 16 || n >= a.width) return;
+    float y = 0.0f;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) y += part[v][threadIdx.x];
+    ((T*)a.Y)[n] = (T)y;
 }
 
 template <typename T>
@@ -603,7 +657,7 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
     const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
     const int expert_groups = (a.experts + 3) / 4, pieces = (w.x_ld / 16 * a.tokens + 255) / 256;
     const unsigned prepare_x = (unsigned)(expert_groups + pieces);
-    const unsigned up_x = (unsigned)(w.act_ld / 32), down_x = (unsigned)((a.width + 15) / 16);
+    const unsigned up_x = (unsigned)(w.act_ld / 32);  // 16 units each, to the end of a row of the workspace
     if (a.tokens == 1) {
         prepare_kernel<T, 1><<<prepare_x, 256, 0, s>>>(a, w, expert_groups);
         const dim3 up(up_x, (unsigned)a.topk);
@@ -613,7 +667,7 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
             up_one_kernel<T, 2><<<up, 512, 0, s>>>(a, w);
         else
             up_one_kernel<T, 8><<<up, 512, 0, s>>>(a, w);
-        down_kernel<T, 2, 16, true><<<down_x, 1024, 0, s>>>(a, w);
+        down_one_kernel<T><<<(unsigned)((a.width + 15) / 16), 1024, 0, s>>>(a, w);
     } else {
         prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
         if (a.experts <= 64)
@@ -623,9 +677,14 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
         else
             choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
         const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
-        const int most = a.experts + choices / UP < choices ? a.experts + choices / UP : choices;
-        up_kernel<T, UP><<<dim3(up_x / kUpWaves, (unsigned)most, chunks), 64 * kUpWaves, 0, s>>>(a, w);
-        down_kernel<T, DOWN, 8, false><<<dim3(down_x, chunks), 512, 0, s>>>(a, w);
+        auto most = [&](int size) {  // tiles
+            return (unsigned)(a.experts + choices / size < choices ? a.experts + choices / size : choices);
+        };
+        up_kernel<T, UP><<<dim3(up_x / kTileWaves, most(UP), chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        constexpr int ROWS = 32 * kTileWaves;
+        down_kernel<T, DOWN>
+            <<<dim3((unsigned)((a.width + ROWS - 1) / ROWS), most(DOWN), chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        combine_kernel<T><<<dim3((unsigned)((a.width + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a, w);
     }
     return hipGetLastError();
 }
