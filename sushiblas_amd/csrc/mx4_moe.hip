@@ -3,10 +3,10 @@
 //
 // Kernels, each on what the one before wrote to the workspace:
 //   prepare  the router's logits, and the tokens as bf16 pieces
-//   choose   (more than one token) each token's experts and shares, the choices sorted by expert,
-//            in tiles of a few tokens of one expert
+//   choose   (more than 8 tokens or 64 experts, and two tokens) each token's experts and shares, the
+//            choices sorted by expert, in tiles of a few tokens of one expert
 //   up       a tile by 16 units of the hidden layer a wave: share * silu(G x) * (U x), as bf16 pieces;
-//            of one token it chooses itself, which costs less than a launch
+//            of fewer tokens and experts it chooses itself, which costs less than a launch
 //   down     a tile by 32 results; of one token, 16 results over all of its choices, which the waves share
 //   combine  (more than one token) the sum over a token's choices
 // Products and pieces: mx4_rows.hpp.
@@ -385,15 +385,21 @@ __device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKEN
     return v;
 }
 
-// A tile's tokens times two blocks of 16 rows of each of four waves.  The tokens' terms are in LDS for
-// all of them, a group after another, the next one on its way; rows stay within a wave (mx4_rows.hpp).
+// A tile's tokens times two blocks of 16 rows, by a workgroup of four waves (rows stay within a wave:
+// mx4_rows.hpp).
+//   SPLIT false: the rows are each wave's own, and the tokens' terms are in LDS for all of them, a group
+// after another, the next one on its way.  Tokens are read and laid out once for 128 rows.
+//   SPLIT true: the waves share the terms of the same rows, a group each by turns, and add up at the end.
+// Four times the workgroups, where the others would leave CUs idle.
 constexpr int kTileWaves = 4;
-template <int PIECES, int TOKENS>
+template <int PIECES, int TOKENS, bool SPLIT>
 struct TileProduct {
-    static constexpr int STAGE = tokens_bytes(PIECES, TOKENS), BYTES = 2 * STAGE + kTileWaves * rows4_bytes(2);
-    // a thread's chunks of a piece: of tokens (threadIdx.x + 256 i) / 32
-    static constexpr int LOADS = TOKENS * 32 / (64 * kTileWaves);
-    f32x4 acc[fragments_of(PIECES, TOKENS)][2];
+    static constexpr int STAGE = tokens_bytes(PIECES, TOKENS), STAGES = SPLIT ? kTileWaves : 2;
+    static constexpr int BYTES = STAGES * STAGE + kTileWaves * rows4_bytes(2);
+    static constexpr int FRAGMENTS = fragments_of(PIECES, TOKENS);
+    // a thread's chunks of a piece: of the tokens (its number + THREADS i) / 32
+    static constexpr int THREADS = SPLIT ? 64 : 64 * kTileWaves, LOADS = TOKENS * 32 / THREADS;
+    f32x4 acc[FRAGMENTS][2];  // SPLIT: the first wave's
 
     // s0, s1: the rows, at least one of each; x: the tokens' pieces, `stride` apart, token t's offset_of(t)
     // bytes from there or not there (kOutside).
@@ -401,12 +407,13 @@ struct TileProduct {
     __device__ inline void run(const Source4<1>& s0, const Source4<1>& s1, int nb, const uint8_t* tokens, int64_t stride,
                                F&& offset_of, char* lds, int lane, int wave)
     {
-        const int groups = (nb + 7) / 8;
-        char* own = lds + 2 * STAGE + wave * rows4_bytes(2);
+        constexpr int STEP = SPLIT ? kTileWaves : 1;
+        const int groups = (nb + 7) / 8, me = SPLIT ? lane : threadIdx.x, first = SPLIT ? wave : 0;
+        char *own = lds + STAGES * STAGE + wave * rows4_bytes(2), *stage = lds + (SPLIT ? wave * STAGE : 0);
         int at[LOADS];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int from = offset_of((threadIdx.x + 64 * kTileWaves * i) / 32);
+            const int from = offset_of((me + THREADS * i) / 32);
             at[i] = from == kOutside ? kOutside : from + lane % 32 * 16;
         }
         u32x4 x[LOADS][PIECES];
@@ -416,7 +423,8 @@ struct TileProduct {
                 const __amdgpu_buffer_rsrc_t v = buffer_of(tokens + n * stride, 0x7fffffff);
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i)
-                    x[i][n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], g * 512, 0));
+                    x[i][n] = __builtin_bit_cast(
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(v, at[i], min(g, groups - 1) * 512, 0));
             }
         };
         auto put_tokens = [&](char* to) {
@@ -424,26 +432,29 @@ struct TileProduct {
             for (int n = 0; n < PIECES; ++n)
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const int row = n * TOKENS + (threadIdx.x + 64 * kTileWaves * i) / 32;
+                    const int row = n * TOKENS + (me + THREADS * i) / 32;
                     *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
                 }
         };
         auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (loads go on)
         Rows4<1> w0[2], w1[2];
-        load_tokens(0);
+        load_tokens(first);
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
-            s0.load(w0[d], d, nb - 8 * d);
-            s1.load(w1[d], d, nb - 8 * d);
+            const int g = first + d * STEP;
+            s0.load(w0[d], g, nb - 8 * g);
+            s1.load(w1[d], g, nb - 8 * g);
         }
-        put_tokens(lds);
-        load_tokens(min(1, groups - 1));
-        barrier();
+        if constexpr (!SPLIT) {
+            put_tokens(stage);
+            load_tokens(1);
+            barrier();
+        }
 #pragma unroll
-        for (int f = 0; f < fragments_of(PIECES, TOKENS); ++f) acc[f][0] = acc[f][1] = f32x4{};
-        for (int g = 0; g < groups;) {
+        for (int f = 0; f < FRAGMENTS; ++f) acc[f][0] = acc[f][1] = f32x4{};
+        for (int g = first; g < groups;) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {  // (stage g % 2)
+            for (int d = 0; d < 2; ++d) {  // (not SPLIT: stage g % 2)
                 bf16x8 v[2][8];
                 if (nb - 8 * g < 8) {
                     w0[d].code[0] = first_codes(w0[d].code[0], nb - 8 * g);
@@ -451,14 +462,40 @@ struct TileProduct {
                 }
                 const Rows4<2> both = {{w0[d].v[0], w0[d].v[1], w1[d].v[0], w1[d].v[1]}, {w0[d].code[0], w1[d].code[0]}};
                 fragments(both, own, lane, v);
-                s0.load(w0[d], g + 2, nb - 8 * (g + 2));
-                s1.load(w1[d], g + 2, nb - 8 * (g + 2));
-                put_tokens(lds + (1 - d) * STAGE);  // its last readers passed the barrier before
-                load_tokens(min(g + 2, groups - 1));
-                multiply<PIECES, TOKENS>(acc, v, lds + d * STAGE, lane);
-                barrier();
-                if (++g >= groups) break;
+                const int next = g + 2 * STEP;
+                s0.load(w0[d], next, nb - 8 * next);
+                s1.load(w1[d], next, nb - 8 * next);
+                if constexpr (SPLIT) {
+                    put_tokens(stage);
+                    load_tokens(g + STEP);
+                    multiply<PIECES, TOKENS>(acc, v, stage, lane);
+                } else {
+                    put_tokens(stage + (1 - d) * STAGE);  // its last readers passed the barrier before
+                    load_tokens(g + 2);
+                    multiply<PIECES, TOKENS>(acc, v, stage + d * STAGE, lane);
+                    barrier();
+                }
+                g += STEP;
+                if (g >= groups) break;
             }
+        }
+        if constexpr (SPLIT) {
+            static_assert(kTileWaves * FRAGMENTS * 2 * 64 * 16 <= BYTES, "");
+            f32x4* part = (f32x4*)lds;
+            __syncthreads();
+            if (wave > 0)
+#pragma unroll
+                for (int f = 0; f < FRAGMENTS; ++f)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) part[((wave * FRAGMENTS + f) * 2 + i) * 64 + lane] = acc[f][i];
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int f = 0; f < FRAGMENTS; ++f)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int o = 1; o < kTileWaves; ++o) acc[f][i] += part[((o * FRAGMENTS + f) * 2 + i) * 64 + lane];
         }
     }
 };
@@ -482,18 +519,99 @@ struct Tile {
     }
 };
 
-// 16 units a wave: its rows of G and of U.
-template <typename T, int TOKENS>
+// The same for up to 8 tokens and 64 experts, of which the kernel makes the list itself: an expert's tokens
+// are one tile.  Costs 1 us where a launch and the list's way through memory cost 4.
+constexpr int kFewTokens = 8, kFewExperts = 64;
+template <int TOKENS>
+struct FewTokens {
+    static_assert(TOKENS >= kFewTokens, "");
+    uint32_t tokens_of[kFewExperts];  // as bits
+    int expert_of[kFewTokens * 16];
+    float share_of[kFewTokens * 16];
+
+    __device__ inline bool find(const Mx4MoeArgs& a, const Mx4MoeWork& w, Tile<TOKENS>& tile, int (&choice_of)[TOKENS],
+                                int lane, int wave)
+    {
+        if (threadIdx.x < kFewExperts) tokens_of[threadIdx.x] = 0;
+        __syncthreads();
+        for (int t = wave; t < a.tokens; t += kTileWaves) {
+            const double* logits = (const double*)(a.work + w.logits) + t * a.experts;
+            Chooser<1> from;
+            from.init(logits, a.experts, lane);
+            int mine = 0;
+            for (int k = 0; k < a.topk; ++k) {
+                const int e = from.next(k, lane);
+                if (lane == k) mine = e;
+            }
+            const float p = from.share(logits, a.experts, a.topk, a.normalize, lane);
+            if (lane < a.topk) {
+                expert_of[t * a.topk + lane] = mine;
+                share_of[t * a.topk + lane] = p;
+                atomicOr(&tokens_of[mine], 1u << t);
+            }
+        }
+        __syncthreads();
+        const uint64_t used = __builtin_amdgcn_ballot_w64(tokens_of[lane] != 0);
+        if ((int)blockIdx.y >= __popcll(used)) return false;
+        const int before = __popcll(used & ((1ull << lane) - 1));
+        const uint64_t here = __builtin_amdgcn_ballot_w64((used >> lane & 1) && before == (int)blockIdx.y);
+        tile.expert = __builtin_ctzll(here);
+        const uint32_t mask = __builtin_amdgcn_readfirstlane((int)tokens_of[tile.expert]);
+        tile.count = __popc(mask);
+        if ((int)threadIdx.x < kFewTokens && (mask >> threadIdx.x & 1)) {
+            int c = threadIdx.x * a.topk;
+            while (expert_of[c] != tile.expert) ++c;  // (it is there)
+            choice_of[__popc(mask & ((1u << threadIdx.x) - 1))] = c;
+        }
+        __syncthreads();
+        return true;
+    }
+    // The choices and the list for what comes after; by one wave of one workgroup.
+    __device__ inline void write(const Mx4MoeArgs& a, const Mx4MoeWork& w, int lane)
+    {
+        int* out = (int*)(a.work + w.tiles);
+        const int n = __popc(tokens_of[lane]);
+        const uint64_t used = __builtin_amdgcn_ballot_w64(n > 0);
+        int sum = n;  // of the experts up to this one
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(sum, d);
+            if (lane >= d) sum += v;
+        }
+        if (n > 0) {
+            int* to = out + 2 + 3 * kMoeTiles + __popcll(used & ((1ull << lane) - 1));
+            to[0] = lane;
+            to[kMoeTiles] = sum - n;
+            to[2 * kMoeTiles] = n;
+        }
+        if (lane == 0) out[1] = __popcll(used);
+        for (int c = 0; c < a.tokens * a.topk; c += 64) {  // (shuffles need all lanes)
+            const bool in = c + lane < a.tokens * a.topk;
+            const int e = in ? expert_of[c + lane] : 0, t = (c + lane) / a.topk, from = __shfl(sum - n, e);
+            if (!in) continue;
+            out[2 + 6 * kMoeTiles + from + __popc(tokens_of[e] & ((1u << t) - 1))] = c + lane;
+            if (a.chosen) a.chosen[c + lane] = e;
+            if (a.weights) a.weights[c + lane] = share_of[c + lane];
+        }
+    }
+};
+
+// 16 units a wave (SPLIT: a workgroup): its rows of G and of U.
+template <typename T, int TOKENS, bool SPLIT, bool FEW>
 __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kBf16Pieces<T>;
-    typedef TileProduct<PIECES, TOKENS> product_t;
+    typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ int choice_of[TOKENS];
-    Tile<TOKENS> tile;
-    if (!tile.find(a, w, 0, choice_of)) return;
+    __shared__ typename std::conditional<FEW, FewTokens<TOKENS>, int>::type few;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int j0 = (blockIdx.x * kTileWaves + wave) * 16, nb = (a.width + 31) / 32, rows = min(a.hidden - j0, 16);
+    Tile<TOKENS> tile;
+    if constexpr (FEW) {
+        if (!few.find(a, w, tile, choice_of, lane, wave)) return;
+    } else {
+        if (!tile.find(a, w, 0, choice_of)) return;
+    }
+    const int j0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 16, nb = (a.width + 31) / 32, rows = min(a.hidden - j0, 16);
     Source4<1> sg, su;
     sg.init(a.ld1, a.lds1, rows > 0 ? rows : 1, nb, lane);
     su = sg;
@@ -503,28 +621,35 @@ __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4Mo
     product_t product;
     product.run(sg, su, nb, a.work + w.x, w.x_stride,
                 [&](int t) { return t < tile.count ? choice_of[t] / a.topk * w.x_ld : kOutside; }, lds, lane, wave);
+    if constexpr (FEW)
+        if (blockIdx.x == 0 && blockIdx.y == 0 && wave == kTileWaves - 1) few.write(a, w, lane);
+    if (SPLIT && wave > 0) return;
     const int t = lane % 16, q = lane / 16;
     const f32x4 gate = token_sums<PIECES, TOKENS>(product.acc, 0), up = token_sums<PIECES, TOKENS>(product.acc, 1);
     if (t >= tile.count || t >= TOKENS) return;
-    const float share = ((const float*)(a.work + w.weights))[choice_of[t]];
+    float share;
+    if constexpr (FEW)
+        share = few.share_of[choice_of[t]];
+    else
+        share = ((const float*)(a.work + w.weights))[choice_of[t]];
     float h[8] = {};
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = 4 * q + e < rows ? act_of(gate[e], up[e], share) : 0.0f;
     store_act<T, 4>(a, w, choice_of[t], j0 + 4 * q, h);
 }
 
-// 32 results a wave, of each choice apart.
-template <typename T, int TOKENS>
+// 32 results a wave (SPLIT: a workgroup), of each choice apart.
+template <typename T, int TOKENS, bool SPLIT>
 __global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kActPieces<T>;
-    typedef TileProduct<PIECES, TOKENS> product_t;
+    typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ int choice_of[TOKENS];
     Tile<TOKENS> tile;
     if (!tile.find(a, w, 1, choice_of)) return;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int n0 = (blockIdx.x * kTileWaves + wave) * 32, nb = (a.hidden + 31) / 32;
+    const int n0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 32, nb = (a.hidden + 31) / 32;
     Source4<1> s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {  // (past the last row: that one, not used)
@@ -536,6 +661,7 @@ __global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4
     product_t product;
     product.run(s[0], s[1], nb, a.work + w.act + (size_t)first * w.act_ld, w.act_stride,
                 [&](int t) { return t < tile.count ? (choice_of[t] - first) * w.act_ld : kOutside; }, lds, lane, wave);
+    if (SPLIT && wave > 0) return;
     const int t = lane % 16, q = lane / 16;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -659,20 +785,39 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
         down_one_kernel<T><<<(unsigned)((a.width + 15) / 16), 1024, 0, s>>>(a, w);
     } else {
         prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
-        if (a.experts <= 64)
-            choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
-        else if (a.experts <= 128)
-            choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
-        else
-            choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        const bool few = a.tokens <= kFewTokens && a.experts <= kFewExperts;
+        if (!few) {
+            if (a.experts <= 64)
+                choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+            else if (a.experts <= 128)
+                choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+            else
+                choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        }
         const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
         auto most = [&](int size) {  // tiles
             return (unsigned)(a.experts + choices / size < choices ? a.experts + choices / size : choices);
         };
-        up_kernel<T, UP><<<dim3(up_x / kTileWaves, most(UP), chunks), 64 * kTileWaves, 0, s>>>(a, w);
-        constexpr int ROWS = 32 * kTileWaves;
-        down_kernel<T, DOWN>
-            <<<dim3((unsigned)((a.width + ROWS - 1) / ROWS), most(DOWN), chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        // Rows for each wave from so many workgroups on: fp32 4 x 1024 x 2048, 2 of 8 (64 and 256 workgroups a
+        // product) 28.0 us with both forms, 31.8 with rows for each wave, 31.4 with shared ones; bf16 2 x 4096
+        // x 2048, 4 of 32 (256 both) 46 and 52.
+        constexpr int64_t ENOUGH = 200;
+        const unsigned up_t = most(UP), down_t = most(DOWN), down_x = (unsigned)((a.width + 31) / 32),
+                       down_w = (down_x + kTileWaves - 1) / kTileWaves;
+        const bool rows = (int64_t)(up_x / kTileWaves) * up_t * chunks >= ENOUGH;
+        const dim3 up(rows ? up_x / kTileWaves : up_x, up_t, chunks);
+        if (few && rows)
+            up_kernel<T, UP, false, true><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+        else if (few)
+            up_kernel<T, UP, true, true><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+        else if (rows)
+            up_kernel<T, UP, false, false><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+        else
+            up_kernel<T, UP, true, false><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+        if ((int64_t)down_w * down_t * chunks >= ENOUGH)
+            down_kernel<T, DOWN, false><<<dim3(down_w, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        else
+            down_kernel<T, DOWN, true><<<dim3(down_x, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
         combine_kernel<T><<<dim3((unsigned)((a.width + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a, w);
     }
     return hipGetLastError();
