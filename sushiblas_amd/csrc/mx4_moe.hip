@@ -377,7 +377,10 @@ template <int PIECES, int TOKENS, int N>
 __device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKENS)][N], int i)
 {
     f32x4 v = acc[0][i];
-    if constexpr (TOKENS == 8) {
+    if constexpr (TOKENS == 16) {
+#pragma unroll
+        for (int n = 1; n < PIECES; ++n) v += acc[n][i];
+    } else if constexpr (TOKENS == 8 && PIECES > 1) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], 8);  // (the same in either order)
         if constexpr (PIECES == 3) v += acc[1][i];
@@ -764,18 +767,52 @@ __global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork
     ((T*)a.Y)[n] = (T)y;
 }
 
+// The products of more than one token, in tiles of UP and DOWN; FEW: that choose in the first one.
+template <typename T, int UP, int DOWN, bool FEW>
+void launch_tiles(const Mx4MoeArgs& a, const Mx4MoeWork& w, hipStream_t s)
+{
+    const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
+    if constexpr (!FEW) {
+        if (a.experts <= 64)
+            choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        else if (a.experts <= 128)
+            choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+        else
+            choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+    }
+    const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
+    auto most = [&](int size) {  // tiles
+        return (unsigned)(a.experts + choices / size < choices ? a.experts + choices / size : choices);
+    };
+    // Rows for each wave from so many workgroups on: fp32 4 x 1024 x 2048, 2 of 8 (64 and 256 workgroups a
+    // product) 28.0 us with both forms, 31.8 with rows for each wave, 31.4 with shared ones; bf16 2 x 4096
+    // x 2048, 4 of 32 (256 both) 46 and 52.
+    constexpr int64_t ENOUGH = 200;
+    const unsigned up_x = (unsigned)(w.act_ld / 32);  // 16 units each, to the end of a row of the workspace
+    const unsigned up_t = most(UP), down_t = most(DOWN), down_x = (unsigned)((a.width + 31) / 32),
+                   down_w = (down_x + kTileWaves - 1) / kTileWaves;
+    const bool rows = (int64_t)(up_x / kTileWaves) * up_t * chunks >= ENOUGH;
+    const dim3 up(rows ? up_x / kTileWaves : up_x, up_t, chunks);
+    if (rows)
+        up_kernel<T, UP, false, FEW><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+    else
+        up_kernel<T, UP, true, FEW><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+    if ((int64_t)down_w * down_t * chunks >= ENOUGH)
+        down_kernel<T, DOWN, false><<<dim3(down_w, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
+    else
+        down_kernel<T, DOWN, true><<<dim3(down_x, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
+    combine_kernel<T><<<dim3((unsigned)((a.width + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a, w);
+}
+
 template <typename T>
 hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
 {
     const Mx4MoeWork w = mx4_moe_work(a.tokens, a.width, a.hidden, a.experts, a.topk);
-    constexpr int UP = kBf16Pieces<T> == 1 ? 16 : 8, DOWN = 8;  // tokens of a tile (what fits the LDS)
-    const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
     const int expert_groups = (a.experts + 3) / 4, pieces = (w.x_ld / 16 * a.tokens + 255) / 256;
     const unsigned prepare_x = (unsigned)(expert_groups + pieces);
-    const unsigned up_x = (unsigned)(w.act_ld / 32);  // 16 units each, to the end of a row of the workspace
     if (a.tokens == 1) {
         prepare_kernel<T, 1><<<prepare_x, 256, 0, s>>>(a, w, expert_groups);
-        const dim3 up(up_x, (unsigned)a.topk);
+        const dim3 up((unsigned)(w.act_ld / 32), (unsigned)a.topk);
         if (a.experts <= 64)
             up_one_kernel<T, 1><<<up, 512, 0, s>>>(a, w);
         else if (a.experts <= 128)
@@ -785,40 +822,16 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
         down_one_kernel<T><<<(unsigned)((a.width + 15) / 16), 1024, 0, s>>>(a, w);
     } else {
         prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
-        const bool few = a.tokens <= kFewTokens && a.experts <= kFewExperts;
-        if (!few) {
-            if (a.experts <= 64)
-                choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
-            else if (a.experts <= 128)
-                choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
-            else
-                choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
-        }
-        const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
-        auto most = [&](int size) {  // tiles
-            return (unsigned)(a.experts + choices / size < choices ? a.experts + choices / size : choices);
-        };
-        // Rows for each wave from so many workgroups on: fp32 4 x 1024 x 2048, 2 of 8 (64 and 256 workgroups a
-        // product) 28.0 us with both forms, 31.8 with rows for each wave, 31.4 with shared ones; bf16 2 x 4096
-        // x 2048, 4 of 32 (256 both) 46 and 52.
-        constexpr int64_t ENOUGH = 200;
-        const unsigned up_t = most(UP), down_t = most(DOWN), down_x = (unsigned)((a.width + 31) / 32),
-                       down_w = (down_x + kTileWaves - 1) / kTileWaves;
-        const bool rows = (int64_t)(up_x / kTileWaves) * up_t * chunks >= ENOUGH;
-        const dim3 up(rows ? up_x / kTileWaves : up_x, up_t, chunks);
-        if (few && rows)
-            up_kernel<T, UP, false, true><<<up, 64 * kTileWaves, 0, s>>>(a, w);
-        else if (few)
-            up_kernel<T, UP, true, true><<<up, 64 * kTileWaves, 0, s>>>(a, w);
-        else if (rows)
-            up_kernel<T, UP, false, false><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+        constexpr int UP = kBf16Pieces<T> == 1 ? 16 : 8;
+        const int chunk = a.tokens < kMoeChunk ? a.tokens : kMoeChunk;
+        if (a.tokens <= kFewTokens && a.experts <= kFewExperts)
+            launch_tiles<T, UP, 8, true>(a, w, s);
+        // tiles of 16 where experts have more than 6 tokens on average, as most would need two of 8 (64 x 4096
+        // x 2048, 4 of 32, fp16 117 against 126 us, fp32 145 against 150; 8 tokens of it 78 against 73)
+        else if (chunk * a.topk > 6 * a.experts)
+            launch_tiles<T, 16, 16, false>(a, w, s);
         else
-            up_kernel<T, UP, true, false><<<up, 64 * kTileWaves, 0, s>>>(a, w);
-        if ((int64_t)down_w * down_t * chunks >= ENOUGH)
-            down_kernel<T, DOWN, false><<<dim3(down_w, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
-        else
-            down_kernel<T, DOWN, true><<<dim3(down_x, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
-        combine_kernel<T><<<dim3((unsigned)((a.width + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a, w);
+            launch_tiles<T, UP, 8, false>(a, w, s);
     }
     return hipGetLastError();
 }
