@@ -344,21 +344,25 @@ __global__ void __launch_bounds__(1024) grad_long_kernel(NormGradArgs a)
     }
 }
 
-// W's gradient from its parts: 64 columns a workgroup, its 16 waves every 16th part each.
+// W's gradient from its parts: 64 columns a workgroup at a time, its 16 waves every 16th part each.
 __global__ void __launch_bounds__(1024) parts_kernel(const float* part, int parts, int64_t cols, float* DW)
 {
     __shared__ float sums[16][64];
-    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
-    float v = 0.0f;
-    if (c < cols)
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < cols; c0 += (int64_t)gridDim.x * 64) {
+        const int64_t c = c0 + lane;
+        float v = 0.0f;
+        if (c < cols)
 #pragma unroll 4
-        for (int i = threadIdx.x / 64; i < parts; i += 16) v += part[i * cols + c];
-    sums[threadIdx.x / 64][threadIdx.x % 64] = v;
-    __syncthreads();
-    if (threadIdx.x >= 64 || c >= cols) return;
+            for (int i = wave; i < parts; i += 16) v += part[i * cols + c];
+        __syncthreads();
+        sums[wave][lane] = v;
+        __syncthreads();
+        if (wave > 0 || c >= cols) continue;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += sums[i][threadIdx.x];
-    DW[c] = v;
+        for (int i = 1; i < 16; ++i) v += sums[i][lane];
+        DW[c] = v;
+    }
 }
 
 // Threads form TX pieces of 16 bytes of a row's values by 256 / TX rows.
@@ -523,7 +527,8 @@ hipError_t launch_rms_norm_grad(int dtype, const NormGradArgs& a, hipStream_t s)
         if (e != hipSuccess) return e;
     }
     if (!a.DW) return hipSuccess;
-    parts_kernel<<<(unsigned)((a.cols + 63) / 64), 1024, 0, s>>>(a.part, parts, a.cols, a.DW);
+    const int64_t tiles = (a.cols + 63) / 64;
+    parts_kernel<<<(unsigned)(tiles < 65536 ? tiles : 65536), 1024, 0, s>>>(a.part, parts, a.cols, a.DW);
     return hipGetLastError();
 }
 
