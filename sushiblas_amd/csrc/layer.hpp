@@ -76,15 +76,9 @@ struct Mx4MoeWork {
     size_t x, x_stride;      // tokens as bf16 pieces (up to 3, x_stride bytes apart), zeros to x_ld bytes
     size_t act, act_stride;  // the hidden layer times its share, one row a choice, likewise
     size_t out;              // (more than one token) each choice's results, rows of out_ld floats
-    size_t tiles;            // of each chunk, tiles_bytes apart: what is below, in 32-bit words
-    size_t tiles_bytes, bytes;
+    size_t bytes;
     int x_ld, act_ld, out_ld;
 };
-// A chunk's tiles: their numbers, of the first product and of the second; then their experts, first
-// places and counts; then the choices by place.
-constexpr int kMoeChoices = kMoeChunk * 16, kMoeTiles = kMoeChoices;
-constexpr int kMoeTileWords = 2 + 2 * 3 * kMoeTiles + kMoeChoices;
-
 inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t width, int64_t hidden, int64_t experts, int64_t topk)
 {
     Mx4MoeWork w;
@@ -105,8 +99,6 @@ inline Mx4MoeWork mx4_moe_work(int64_t tokens, int64_t width, int64_t hidden, in
     w.act = take(3 * w.act_stride);
     w.out_ld = (int)((width + 3) / 4 * 4);
     w.out = take(tokens > 1 ? 4 * (size_t)w.out_ld * tokens * topk : 0);
-    w.tiles_bytes = 4 * kMoeTileWords;
-    w.tiles = take((tokens + kMoeChunk - 1) / kMoeChunk * w.tiles_bytes);
     w.bytes = at;
     return w;
 }

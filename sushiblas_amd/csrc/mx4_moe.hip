@@ -3,9 +3,8 @@
 //
 // Kernels, each on what the one before wrote to the workspace:
 //   prepare  the router's logits, and the tokens as bf16 pieces
-//   choose   (more than 8 tokens or 64 experts, and two tokens) each token's experts and shares, the
-//            choices sorted by expert, in tiles of a few tokens of one expert
-//   up       a tile by 16 units of the hidden layer a wave: share * silu(G x) * (U x), as bf16 pieces;
+//   choose   (more than 8 tokens or 64 experts, and two tokens) each token's experts and shares
+//   up       a tile, a few tokens of one expert, by 16 units of the hidden layer a wave: share * silu(G x) * (U x), as bf16 pieces;
 //            of fewer tokens and experts it chooses itself, which costs less than a launch
 //   down     a tile by 32 results; of one token, 16 results over all of its choices, which the waves share
 //   combine  (more than one token) the sum over a token's choices
@@ -191,78 +190,27 @@ struct Chooser {
     }
 };
 
-// A chunk's choices, by expert, in tiles of `up_size` and of `down_size` tokens.
+// A wave to a token.
 template <int EACH>
-__global__ void __launch_bounds__(1024) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w, int up_size, int down_size)
+__global__ void __launch_bounds__(256) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
-    __shared__ uint64_t tokens_of[kMaxExperts];  // as bits
-    __shared__ int expert_of[kMoeChoices], place[kMaxExperts], scan[3][16];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, t0 = blockIdx.x * kMoeChunk;
-    const int count = min(a.tokens - t0, kMoeChunk);
-    if (threadIdx.x < kMaxExperts) tokens_of[threadIdx.x] = 0;
-    __syncthreads();
-    for (int t = wave; t < count; t += 16) {
-        const int c0 = (t0 + t) * a.topk;
-        Chooser<EACH> from;
-        from.init((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts, lane);
-        int mine = 0;
-        for (int k = 0; k < a.topk; ++k) {
-            const int e = from.next(k, lane);
-            if (lane == k) mine = e;
-        }
-        const float p = from.share((const double*)(a.work + w.logits) + (int64_t)(t0 + t) * a.experts, a.experts, a.topk,
-                                   a.normalize, lane);
-        if (lane < a.topk) {
-            expert_of[t * a.topk + lane] = mine;
-            atomicOr((unsigned long long*)&tokens_of[mine], 1ull << t);
-            ((float*)(a.work + w.weights))[c0 + lane] = p;
-            if (a.weights) a.weights[c0 + lane] = p;
-            if (a.chosen) a.chosen[c0 + lane] = mine;
-        }
+    const int lane = threadIdx.x % 64, t = blockIdx.x * 4 + threadIdx.x / 64;
+    if (t >= a.tokens) return;
+    const double* logits = (const double*)(a.work + w.logits) + (int64_t)t * a.experts;
+    Chooser<EACH> from;
+    from.init(logits, a.experts, lane);
+    int mine = 0;
+    for (int k = 0; k < a.topk; ++k) {
+        const int e = from.next(k, lane);
+        if (lane == k) mine = e;
     }
-    __syncthreads();
-    // sums over the experts before: choices, and tiles of either size
-    const int e = threadIdx.x, n = e < kMaxExperts ? __popcll(tokens_of[e]) : 0;
-    const int own[3] = {n, (n + up_size - 1) / up_size, (n + down_size - 1) / down_size};
-    int at[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        at[i] = own[i];
-        for (int d = 1; d < 64; d *= 2) {
-            const int v = __shfl_up(at[i], d);
-            if (lane >= d) at[i] += v;
-        }
-        if (lane == 63) scan[i][wave] = at[i];
-    }
-    __syncthreads();
-    int total[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        total[i] = 0;
-        for (int v = 0; v < 16; ++v) {
-            if (v < wave) at[i] += scan[i][v];
-            total[i] += scan[i][v];
-        }
-        at[i] -= own[i];
-    }
-    if (e < kMaxExperts) place[e] = at[0];
-    int* out = (int*)(a.work + w.tiles + blockIdx.x * w.tiles_bytes);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int size = k ? down_size : up_size;
-        int* to = out + 2 + k * 3 * kMoeTiles;
-        for (int i = 0; i < own[1 + k]; ++i) {
-            to[at[1 + k] + i] = e;
-            to[kMoeTiles + at[1 + k] + i] = at[0] + i * size;
-            to[2 * kMoeTiles + at[1 + k] + i] = min(n - i * size, size);
-        }
-        if (threadIdx.x == 0) out[k] = total[1 + k];
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < count * a.topk; c += 1024) {
-        const int x = expert_of[c], before = __popcll(tokens_of[x] & ((1ull << c / a.topk) - 1));
-        out[2 + 6 * kMoeTiles + place[x] + before] = t0 * a.topk + c;
-    }
+    const float p = from.share(logits, a.experts, a.topk, a.normalize, lane);
+    if (lane >= a.topk) return;
+    const int c = t * a.topk + lane;
+    ((int*)(a.work + w.chosen))[c] = mine;
+    ((float*)(a.work + w.weights))[c] = p;
+    if (a.chosen) a.chosen[c] = mine;
+    if (a.weights) a.weights[c] = p;
 }
 
 // ---- the experts ----
@@ -503,100 +451,106 @@ struct TileProduct {
     }
 };
 
-// What a tile's kernel finds in the list of tiles.
+// A workgroup's tile: the blockIdx.y-th when the chunk's choices are sorted by expert and each expert's
+// tokens, in order, cut into tiles of TOKENS.  Every workgroup sorts them itself, from the experts chosen:
+// as bits, a token chooses an expert once.  (One workgroup that wrote a list for all took 11 us of its
+// one CU for 64 tokens and 32 experts, and the list's way through memory.)
+constexpr int kMoeChoices = kMoeChunk * 16;
 template <int TOKENS>
 struct Tile {
-    int expert, count;
-    __device__ inline bool find(const Mx4MoeArgs& a, const Mx4MoeWork& w, int list, int (&choice_of)[TOKENS])
+    uint64_t tokens_of[kMaxExperts];  // as bits
+    int expert_of[kMoeChoices], choice_of[TOKENS], expert, skip, total, sums[kTileWaves];
+
+    // Before: nothing in tokens_of.
+    __device__ inline void clear()
     {
-        const int* tiles = (const int*)(a.work + w.tiles + blockIdx.z * w.tiles_bytes);
-        const int* own = tiles + 2 + list * 3 * kMoeTiles + blockIdx.y;
-        if ((int)blockIdx.y >= tiles[list]) return false;
-        expert = __builtin_amdgcn_readfirstlane(own[0]);
-        count = __builtin_amdgcn_readfirstlane(own[2 * kMoeTiles]);
-        const int from = own[kMoeTiles];
-        if (threadIdx.x < TOKENS)
-            choice_of[threadIdx.x] = tiles[2 + 6 * kMoeTiles + from + min((int)threadIdx.x, count - 1)];
+        for (int e = threadIdx.x; e < kMaxExperts; e += 64 * kTileWaves) tokens_of[e] = 0;
         __syncthreads();
-        return true;
+    }
+    // A choice of the chunk, by any thread.
+    __device__ inline void put(const Mx4MoeArgs& a, int c, int e)
+    {
+        expert_of[c] = e;
+        atomicOr((unsigned long long*)&tokens_of[e], 1ull << c / a.topk);
+    }
+    __device__ inline void put_all(const Mx4MoeArgs& a, const Mx4MoeWork& w, int first, int count)
+    {
+        for (int c = threadIdx.x; c < count; c += 64 * kTileWaves) put(a, c, ((const int*)(a.work + w.chosen))[first + c]);
+    }
+    // After: whether there is the tile; its tokens' number, its expert and choices (of the chunk).
+    __device__ inline int find(const Mx4MoeArgs& a, int lane, int wave)
+    {
+        __syncthreads();
+        // two experts a thread, of as many waves as that takes: tiles of the experts before
+        constexpr int PER = kMaxExperts / (64 * kTileWaves);
+        static_assert(PER == 2, "");
+        const int used = (a.experts + 2 * 64 - 1) / (2 * 64), e = 2 * threadIdx.x;
+        int n0 = 0, n1 = 0, sum = 0;
+        if (wave < used) {
+            n0 = (__popcll(tokens_of[e]) + TOKENS - 1) / TOKENS;
+            n1 = (__popcll(tokens_of[e + 1]) + TOKENS - 1) / TOKENS;
+            sum = n0 + n1;
+            for (int d = 1; d < 64; d *= 2) {
+                const int v = __shfl_up(sum, d);
+                if (lane >= d) sum += v;
+            }
+            if (lane == 63) sums[wave] = sum;
+        }
+        if (used > 1) __syncthreads();
+        if (wave < used) {
+            for (int v = 0; v < wave; ++v) sum += sums[v];
+            const int at = blockIdx.y - (sum - n0 - n1);
+            if (at >= 0 && at < n0 + n1) {
+                expert = at < n0 ? e : e + 1;
+                skip = (at < n0 ? at : at - n0) * TOKENS;
+            }
+            if (wave == used - 1 && lane == 63) total = sum;
+        }
+        __syncthreads();
+        if ((int)blockIdx.y >= total) return 0;
+        const uint64_t mask = tokens_of[expert];
+        if (threadIdx.x < kMoeChunk && (mask >> threadIdx.x & 1)) {
+            const int place = __popcll(mask & ((1ull << threadIdx.x) - 1)) - skip;
+            if (place >= 0 && place < TOKENS) {
+                int c = threadIdx.x * a.topk;
+                while (expert_of[c] != expert) ++c;  // (it is there)
+                choice_of[place] = c;
+            }
+        }
+        __syncthreads();
+        return min(__popcll(mask) - skip, TOKENS);
     }
 };
 
-// The same for up to 8 tokens and 64 experts, of which the kernel makes the list itself: an expert's tokens
-// are one tile.  Costs 1 us where a launch and the list's way through memory cost 4.
+// Up to so many tokens and experts the first product's workgroups choose, too: 1 us where a launch costs 4.
 constexpr int kFewTokens = 8, kFewExperts = 64;
-template <int TOKENS>
-struct FewTokens {
-    static_assert(TOKENS >= kFewTokens, "");
-    uint32_t tokens_of[kFewExperts];  // as bits
-    int expert_of[kFewTokens * 16];
-    float share_of[kFewTokens * 16];
-
-    __device__ inline bool find(const Mx4MoeArgs& a, const Mx4MoeWork& w, Tile<TOKENS>& tile, int (&choice_of)[TOKENS],
-                                int lane, int wave)
-    {
-        if (threadIdx.x < kFewExperts) tokens_of[threadIdx.x] = 0;
-        __syncthreads();
-        for (int t = wave; t < a.tokens; t += kTileWaves) {
-            const double* logits = (const double*)(a.work + w.logits) + t * a.experts;
-            Chooser<1> from;
-            from.init(logits, a.experts, lane);
-            int mine = 0;
-            for (int k = 0; k < a.topk; ++k) {
-                const int e = from.next(k, lane);
-                if (lane == k) mine = e;
-            }
-            const float p = from.share(logits, a.experts, a.topk, a.normalize, lane);
-            if (lane < a.topk) {
-                expert_of[t * a.topk + lane] = mine;
-                share_of[t * a.topk + lane] = p;
-                atomicOr(&tokens_of[mine], 1u << t);
-            }
-        }
-        __syncthreads();
-        const uint64_t used = __builtin_amdgcn_ballot_w64(tokens_of[lane] != 0);
-        if ((int)blockIdx.y >= __popcll(used)) return false;
-        const int before = __popcll(used & ((1ull << lane) - 1));
-        const uint64_t here = __builtin_amdgcn_ballot_w64((used >> lane & 1) && before == (int)blockIdx.y);
-        tile.expert = __builtin_ctzll(here);
-        const uint32_t mask = __builtin_amdgcn_readfirstlane((int)tokens_of[tile.expert]);
-        tile.count = __popc(mask);
-        if ((int)threadIdx.x < kFewTokens && (mask >> threadIdx.x & 1)) {
-            int c = threadIdx.x * a.topk;
-            while (expert_of[c] != tile.expert) ++c;  // (it is there)
-            choice_of[__popc(mask & ((1u << threadIdx.x) - 1))] = c;
-        }
-        __syncthreads();
-        return true;
-    }
-    // The choices and the list for what comes after; by one wave of one workgroup.
-    __device__ inline void write(const Mx4MoeArgs& a, const Mx4MoeWork& w, int lane)
-    {
-        int* out = (int*)(a.work + w.tiles);
-        const int n = __popc(tokens_of[lane]);
-        const uint64_t used = __builtin_amdgcn_ballot_w64(n > 0);
-        int sum = n;  // of the experts up to this one
-        for (int d = 1; d < 64; d *= 2) {
-            const int v = __shfl_up(sum, d);
-            if (lane >= d) sum += v;
-        }
-        if (n > 0) {
-            int* to = out + 2 + 3 * kMoeTiles + __popcll(used & ((1ull << lane) - 1));
-            to[0] = lane;
-            to[kMoeTiles] = sum - n;
-            to[2 * kMoeTiles] = n;
-        }
-        if (lane == 0) out[1] = __popcll(used);
-        for (int c = 0; c < a.tokens * a.topk; c += 64) {  // (shuffles need all lanes)
-            const bool in = c + lane < a.tokens * a.topk;
-            const int e = in ? expert_of[c + lane] : 0, t = (c + lane) / a.topk, from = __shfl(sum - n, e);
-            if (!in) continue;
-            out[2 + 6 * kMoeTiles + from + __popc(tokens_of[e] & ((1u << t) - 1))] = c + lane;
-            if (a.chosen) a.chosen[c + lane] = e;
-            if (a.weights) a.weights[c + lane] = share_of[c + lane];
-        }
-    }
+struct Shares {
+    float of[kFewTokens * 16];
 };
+template <int TOKENS>
+__device__ inline void choose_few(const Mx4MoeArgs& a, const Mx4MoeWork& w, Tile<TOKENS>& tile, Shares& shares, int lane,
+                                  int wave)
+{
+    for (int t = wave; t < a.tokens; t += kTileWaves) {
+        const double* logits = (const double*)(a.work + w.logits) + t * a.experts;
+        Chooser<1> from;
+        from.init(logits, a.experts, lane);
+        int mine = 0;
+        for (int k = 0; k < a.topk; ++k) {
+            const int e = from.next(k, lane);
+            if (lane == k) mine = e;
+        }
+        const float p = from.share(logits, a.experts, a.topk, a.normalize, lane);
+        if (lane >= a.topk) continue;
+        const int c = t * a.topk + lane;
+        tile.put(a, c, mine);
+        shares.of[c] = p;
+        if (blockIdx.x > 0 || blockIdx.y > 0) continue;
+        ((int*)(a.work + w.chosen))[c] = mine;  // for the second product
+        if (a.chosen) a.chosen[c] = mine;
+        if (a.weights) a.weights[c] = p;
+    }
+}
 
 // 16 units a wave (SPLIT: a workgroup): its rows of G and of U.
 template <typename T, int TOKENS, bool SPLIT, bool FEW>
@@ -605,40 +559,42 @@ __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4Mo
     constexpr int PIECES = kBf16Pieces<T>;
     typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
-    __shared__ int choice_of[TOKENS];
-    __shared__ typename std::conditional<FEW, FewTokens<TOKENS>, int>::type few;
+    __shared__ Tile<TOKENS> tile;
+    __shared__ typename std::conditional<FEW, Shares, int>::type shares;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    Tile<TOKENS> tile;
-    if constexpr (FEW) {
-        if (!few.find(a, w, tile, choice_of, lane, wave)) return;
-    } else {
-        if (!tile.find(a, w, 0, choice_of)) return;
-    }
+    const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
+    tile.clear();
+    if constexpr (FEW)
+        choose_few(a, w, tile, shares, lane, wave);
+    else
+        tile.put_all(a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
+    const int count = tile.find(a, lane, wave);
+    if (count == 0) return;
+    const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
     const int j0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 16, nb = (a.width + 31) / 32, rows = min(a.hidden - j0, 16);
     Source4<1> sg, su;
     sg.init(a.ld1, a.lds1, rows > 0 ? rows : 1, nb, lane);
     su = sg;
     // (past the last unit: the last one's rows, not used)
-    sg.move(a.W1, a.S1, (int64_t)tile.expert * 2 * a.hidden + min(j0, a.hidden - 1));
-    su.move(a.W1, a.S1, (int64_t)tile.expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
+    sg.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + min(j0, a.hidden - 1));
+    su.move(a.W1, a.S1, (int64_t)expert * 2 * a.hidden + a.hidden + min(j0, a.hidden - 1));
     product_t product;
     product.run(sg, su, nb, a.work + w.x, w.x_stride,
-                [&](int t) { return t < tile.count ? choice_of[t] / a.topk * w.x_ld : kOutside; }, lds, lane, wave);
-    if constexpr (FEW)
-        if (blockIdx.x == 0 && blockIdx.y == 0 && wave == kTileWaves - 1) few.write(a, w, lane);
+                [&](int t) { return t < count ? (first + tile.choice_of[t]) / a.topk * w.x_ld : kOutside; }, lds, lane, wave);
     if (SPLIT && wave > 0) return;
     const int t = lane % 16, q = lane / 16;
     const f32x4 gate = token_sums<PIECES, TOKENS>(product.acc, 0), up = token_sums<PIECES, TOKENS>(product.acc, 1);
-    if (t >= tile.count || t >= TOKENS) return;
+    if (t >= count) return;
+    const int choice = first + tile.choice_of[t];
     float share;
     if constexpr (FEW)
-        share = few.share_of[choice_of[t]];
+        share = shares.of[choice];
     else
-        share = ((const float*)(a.work + w.weights))[choice_of[t]];
+        share = ((const float*)(a.work + w.weights))[choice];
     float h[8] = {};
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = 4 * q + e < rows ? act_of(gate[e], up[e], share) : 0.0f;
-    store_act<T, 4>(a, w, choice_of[t], j0 + 4 * q, h);
+    store_act<T, 4>(a, w, choice, j0 + 4 * q, h);
 }
 
 // 32 results a wave (SPLIT: a workgroup), of each choice apart.
@@ -648,22 +604,25 @@ __global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4
     constexpr int PIECES = kActPieces<T>;
     typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
-    __shared__ int choice_of[TOKENS];
-    Tile<TOKENS> tile;
-    if (!tile.find(a, w, 1, choice_of)) return;
+    __shared__ Tile<TOKENS> tile;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
+    tile.clear();
+    tile.put_all(a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
+    const int count = tile.find(a, lane, wave);
+    if (count == 0) return;
+    const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
     const int n0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 32, nb = (a.hidden + 31) / 32;
     Source4<1> s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {  // (past the last row: that one, not used)
         const int at = min(n0 + 16 * i, a.width - 1);
         s[i].init(a.ld2, a.lds2, a.width - at, nb, lane);
-        s[i].move(a.W2, a.S2, (int64_t)tile.expert * a.width + at);
+        s[i].move(a.W2, a.S2, (int64_t)expert * a.width + at);
     }
-    const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
     product_t product;
     product.run(s[0], s[1], nb, a.work + w.act + (size_t)first * w.act_ld, w.act_stride,
-                [&](int t) { return t < tile.count ? (choice_of[t] - first) * w.act_ld : kOutside; }, lds, lane, wave);
+                [&](int t) { return t < count ? tile.choice_of[t] * w.act_ld : kOutside; }, lds, lane, wave);
     if (SPLIT && wave > 0) return;
     const int t = lane % 16, q = lane / 16;
 #pragma unroll
@@ -671,8 +630,8 @@ __global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4
         const f32x4 v = token_sums<PIECES, TOKENS>(product.acc, i);
         const int n = n0 + 16 * i + 4 * q;
         // (rows of `out` are whole 16 bytes)
-        if (t < tile.count && t < TOKENS && n < a.width)
-            *(f32x4*)(a.work + w.out + ((size_t)choice_of[t] * w.out_ld + n) * 4) = v;
+        if (t < count && n < a.width)
+            *(f32x4*)(a.work + w.out + ((size_t)(first + tile.choice_of[t]) * w.out_ld + n) * 4) = v;
     }
 }
 
@@ -774,11 +733,11 @@ void launch_tiles(const Mx4MoeArgs& a, const Mx4MoeWork& w, hipStream_t s)
     const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
     if constexpr (!FEW) {
         if (a.experts <= 64)
-            choose_kernel<1><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+            choose_kernel<1><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
         else if (a.experts <= 128)
-            choose_kernel<2><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+            choose_kernel<2><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
         else
-            choose_kernel<8><<<chunks, 1024, 0, s>>>(a, w, UP, DOWN);
+            choose_kernel<8><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
     }
     const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
     auto most = [&](int size) {  // tiles
