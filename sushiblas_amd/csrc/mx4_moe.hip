@@ -4,8 +4,9 @@
 // Kernels, each on what the one before wrote to the workspace:
 //   prepare  the router's logits, and the tokens as bf16 pieces
 //   choose   (more than 8 tokens or 64 experts, and two tokens) each token's experts and shares
-//   up       a tile, a few tokens of one expert, by 16 units of the hidden layer a wave: share * silu(G x) * (U x), as bf16 pieces;
-//            of fewer tokens and experts it chooses itself, which costs less than a launch
+//   up       a tile, a few tokens of one expert, by 16 units of the hidden layer a wave: share *
+//            silu(G x) * (U x), as bf16 pieces; of fewer tokens and experts it chooses itself, which
+//            costs less than a launch
 //   down     a tile by 32 results; of one token, 16 results over all of its choices, which the waves share
 //   combine  (more than one token) the sum over a token's choices
 // Products and pieces: mx4_rows.hpp.
@@ -456,29 +457,33 @@ struct TileProduct {
 // as bits, a token chooses an expert once.  (One workgroup that wrote a list for all took 11 us of its
 // one CU for 64 tokens and 32 experts, and the list's way through memory.)
 constexpr int kMoeChoices = kMoeChunk * 16;
+struct Choices {  // in the LDS of the product that comes after
+    uint64_t tokens_of[kMaxExperts];  // as bits
+    int expert_of[kMoeChoices];
+};
 template <int TOKENS>
 struct Tile {
-    uint64_t tokens_of[kMaxExperts];  // as bits
-    int expert_of[kMoeChoices], choice_of[TOKENS], expert, skip, total, sums[kTileWaves];
+    int choice_of[TOKENS], expert, skip, total, sums[kTileWaves];
 
     // Before: nothing in tokens_of.
-    __device__ inline void clear()
+    static __device__ inline void clear(Choices& x)
     {
-        for (int e = threadIdx.x; e < kMaxExperts; e += 64 * kTileWaves) tokens_of[e] = 0;
+        for (int e = threadIdx.x; e < kMaxExperts; e += 64 * kTileWaves) x.tokens_of[e] = 0;
         __syncthreads();
     }
     // A choice of the chunk, by any thread.
-    __device__ inline void put(const Mx4MoeArgs& a, int c, int e)
+    static __device__ inline void put(Choices& x, const Mx4MoeArgs& a, int c, int e)
     {
-        expert_of[c] = e;
-        atomicOr((unsigned long long*)&tokens_of[e], 1ull << c / a.topk);
+        x.expert_of[c] = e;
+        atomicOr((unsigned long long*)&x.tokens_of[e], 1ull << c / a.topk);
     }
-    __device__ inline void put_all(const Mx4MoeArgs& a, const Mx4MoeWork& w, int first, int count)
+    static __device__ inline void put_all(Choices& x, const Mx4MoeArgs& a, const Mx4MoeWork& w, int first, int count)
     {
-        for (int c = threadIdx.x; c < count; c += 64 * kTileWaves) put(a, c, ((const int*)(a.work + w.chosen))[first + c]);
+        for (int c = threadIdx.x; c < count; c += 64 * kTileWaves)
+            put(x, a, c, ((const int*)(a.work + w.chosen))[first + c]);
     }
     // After: whether there is the tile; its tokens' number, its expert and choices (of the chunk).
-    __device__ inline int find(const Mx4MoeArgs& a, int lane, int wave)
+    __device__ inline int find(const Choices& x, const Mx4MoeArgs& a, int lane, int wave)
     {
         __syncthreads();
         // two experts a thread, of as many waves as that takes: tiles of the experts before
@@ -487,8 +492,8 @@ struct Tile {
         const int used = (a.experts + 2 * 64 - 1) / (2 * 64), e = 2 * threadIdx.x;
         int n0 = 0, n1 = 0, sum = 0;
         if (wave < used) {
-            n0 = (__popcll(tokens_of[e]) + TOKENS - 1) / TOKENS;
-            n1 = (__popcll(tokens_of[e + 1]) + TOKENS - 1) / TOKENS;
+            n0 = (__popcll(x.tokens_of[e]) + TOKENS - 1) / TOKENS;
+            n1 = (__popcll(x.tokens_of[e + 1]) + TOKENS - 1) / TOKENS;
             sum = n0 + n1;
             for (int d = 1; d < 64; d *= 2) {
                 const int v = __shfl_up(sum, d);
@@ -508,12 +513,12 @@ struct Tile {
         }
         __syncthreads();
         if ((int)blockIdx.y >= total) return 0;
-        const uint64_t mask = tokens_of[expert];
+        const uint64_t mask = x.tokens_of[expert];
         if (threadIdx.x < kMoeChunk && (mask >> threadIdx.x & 1)) {
             const int place = __popcll(mask & ((1ull << threadIdx.x) - 1)) - skip;
             if (place >= 0 && place < TOKENS) {
                 int c = threadIdx.x * a.topk;
-                while (expert_of[c] != expert) ++c;  // (it is there)
+                while (x.expert_of[c] != expert) ++c;  // (it is there)
                 choice_of[place] = c;
             }
         }
@@ -528,7 +533,7 @@ struct Shares {
     float of[kFewTokens * 16];
 };
 template <int TOKENS>
-__device__ inline void choose_few(const Mx4MoeArgs& a, const Mx4MoeWork& w, Tile<TOKENS>& tile, Shares& shares, int lane,
+__device__ inline void choose_few(const Mx4MoeArgs& a, const Mx4MoeWork& w, Choices& choices, Shares& shares, int lane,
                                   int wave)
 {
     for (int t = wave; t < a.tokens; t += kTileWaves) {
@@ -543,7 +548,7 @@ __device__ inline void choose_few(const Mx4MoeArgs& a, const Mx4MoeWork& w, Tile
         const float p = from.share(logits, a.experts, a.topk, a.normalize, lane);
         if (lane >= a.topk) continue;
         const int c = t * a.topk + lane;
-        tile.put(a, c, mine);
+        Tile<TOKENS>::put(choices, a, c, mine);
         shares.of[c] = p;
         if (blockIdx.x > 0 || blockIdx.y > 0) continue;
         ((int*)(a.work + w.chosen))[c] = mine;  // for the second product
@@ -563,12 +568,14 @@ __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4Mo
     __shared__ typename std::conditional<FEW, Shares, int>::type shares;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
-    tile.clear();
+    Choices& choices = *(Choices*)lds;
+    static_assert(sizeof(Choices) <= product_t::BYTES, "");
+    tile.clear(choices);
     if constexpr (FEW)
-        choose_few(a, w, tile, shares, lane, wave);
+        choose_few<TOKENS>(a, w, choices, shares, lane, wave);
     else
-        tile.put_all(a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
-    const int count = tile.find(a, lane, wave);
+        tile.put_all(choices, a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
+    const int count = tile.find(choices, a, lane, wave);
     if (count == 0) return;
     const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
     const int j0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 16, nb = (a.width + 31) / 32, rows = min(a.hidden - j0, 16);
@@ -597,9 +604,10 @@ __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4Mo
     store_act<T, 4>(a, w, choice, j0 + 4 * q, h);
 }
 
-// 32 results a wave (SPLIT: a workgroup), of each choice apart.
+// 32 results a wave (SPLIT: a workgroup), of each choice apart.  Three workgroups to a CU of 16-bit types
+// (64 x 4096 x 2048, 4 of 32: 106 us against 108 by two; fp32 would spill, 139 against 129).
 template <typename T, int TOKENS, bool SPLIT>
-__global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+__global__ void __launch_bounds__(64 * kTileWaves, SPLIT || sizeof(T) == 4 ? 1 : 3) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kActPieces<T>;
     typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
@@ -607,9 +615,11 @@ __global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4
     __shared__ Tile<TOKENS> tile;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int first = blockIdx.z * kMoeChunk * a.topk;  // the chunk's first choice
-    tile.clear();
-    tile.put_all(a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
-    const int count = tile.find(a, lane, wave);
+    Choices& choices = *(Choices*)lds;
+    static_assert(sizeof(Choices) <= product_t::BYTES, "");
+    tile.clear(choices);
+    tile.put_all(choices, a, w, first, min(a.tokens * a.topk - first, kMoeChunk * a.topk));
+    const int count = tile.find(choices, a, lane, wave);
     if (count == 0) return;
     const int expert = __builtin_amdgcn_readfirstlane(tile.expert);
     const int n0 = (SPLIT ? blockIdx.x : blockIdx.x * kTileWaves + wave) * 32, nb = (a.hidden + 31) / 32;
