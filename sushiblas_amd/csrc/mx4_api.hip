@@ -269,7 +269,7 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
         if (SX ? sbx::bad_mx8(X, ldx, SX, ldsx, m, k) : sbx::bad_dense(X, k, ldx, elem))
             return SBX_INVALID_ARGUMENT;
         if (sbx::bad_mx4(B, ldb, SB, ldsb, n, k)) return SBX_INVALID_ARGUMENT;
-        if (ldb > sbx::kMaxRowBytes || ldx * (SX ? 1 : (int64_t)elem) > sbx::kMaxTokenBytes) return SBX_UNSUPPORTED;
+        if (ldb > sbx::kMaxRowBytes || ldx > sbx::kMaxTokenBytes / (SX ? 1 : (int64_t)elem)) return SBX_UNSUPPORTED;
     }
     sbx::Mx4LinearArgs a;
     a.m = (int)m; a.n = (int)n; a.k = (int)k;
@@ -313,7 +313,7 @@ int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t 
     if ((uintptr_t)chosen % 4 || (uintptr_t)weights % 4 || !workspace || (uintptr_t)workspace % 16 ||
         workspace_bytes < sbx_mx4_moe_workspace(tokens, width, hidden, experts, topk))
         return SBX_INVALID_ARGUMENT;
-    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes || ldx * (int64_t)elem > sbx::kMaxMoeTokenBytes)
+    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes || ldx > sbx::kMaxMoeTokenBytes / (int64_t)elem)
         return SBX_UNSUPPORTED;
     sbx::Mx4MoeArgs a;
     a.tokens = (int)tokens; a.width = (int)width; a.hidden = (int)hidden;

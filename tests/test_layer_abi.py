@@ -73,7 +73,7 @@ def test_dequantize_refusals(kw, status):
     (dict(SX=64, ldsx=24), 1), (dict(SX=64, ldsx=36), 1), (dict(B=0), 1), (dict(B=72), 1), (dict(ldb=16), 1),
     (dict(ldb=40), 1), (dict(SB=0), 1), (dict(SB=68), 1), (dict(ldsb=40), 1), (dict(Y=0), 1), (dict(Y=66), 1),
     (dict(ldy=5), 1), (dict(ldb=1 << 23), 2), (dict(SX=64, ldx=(1 << 26) + 16), 2),
-    (dict(ldx=(1 << 24) + 1), 2), (dict(dtype=2, ldx=(1 << 25) + 1), 2)])
+    (dict(ldx=(1 << 24) + 1), 2), (dict(dtype=2, ldx=(1 << 25) + 1), 2), (dict(ldx=1 << 62), 2)])
 def test_linear_refusals(kw, status):
     assert _linear(**kw) == status
 
@@ -87,7 +87,7 @@ def test_linear_refusals(kw, status):
     (dict(lds1=8 * 699), 1), (dict(W2=0), 1), (dict(W2=72), 1), (dict(ld2=32), 1), (dict(S2=0), 1), (dict(S2=68), 1),
     (dict(lds2=8 * 199), 1), (dict(Y=0), 1), (dict(Y=66), 1), (dict(ldy=39), 1), (dict(chosen=66), 1),
     (dict(weights=66), 1), (dict(ws=0), 1), (dict(ws=72), 1), (dict(size=100), 1), (dict(ld1=1 << 23), 2),
-    (dict(ld2=1 << 23), 2), (dict(ldx=1 << 21), 2), (dict(dtype=2, ldx=1 << 22), 2)])
+    (dict(ld2=1 << 23), 2), (dict(ldx=1 << 21), 2), (dict(dtype=2, ldx=1 << 22), 2), (dict(ldx=1 << 62), 2)])
 def test_moe_refusals(kw, status):
     assert _moe(**kw) == status
 
