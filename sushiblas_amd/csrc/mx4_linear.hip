@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
     for (int j = 0; j < YB; ++j) {
         const int first = min(y0 + j * TOKENS, p.m - 1);
         if constexpr (MX8)
-            sa[j].init((const uint8_t*)p.X, p.ldx, p.SX, p.ldsx, first, p.m, nb);
+            sa[j].init((const uint8_t*)p.X, p.ldx, p.SX, p.ldsx, first, p.m, p.k);
         else {
             const int ld = (int)(p.ldx * sizeof(T)), count = min(p.m - first, TOKENS);
             sa[j].init((const T*)p.X + first * p.ldx, (count - 1) * ld + p.k * (int)sizeof(T), p.k,
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
             bf16x8 v[XB][8];
             if (nb - 8 * g < 8)
 #pragma unroll
-                for (int i = 0; i < XB; ++i) w[d].code[i] = first_codes(w[d].code[i], nb - 8 * g);
+                for (int i = 0; i < XB; ++i) w[d].code[i] = first_bytes(w[d].code[i], nb - 8 * g);
             fragments(w[d], own, lane, v);
             sw.load(w[d], g + AHEAD * WAVES, nb - 8 * (g + AHEAD * WAVES));
 #pragma unroll

@@ -285,8 +285,8 @@ __global__ void __launch_bounds__(512, 4) up_one_kernel(Mx4MoeArgs a, Mx4MoeWork
     for (int g = wave; g < groups; g += WAVES) {
         bf16x8 v[2][8];
         if (nb - 8 * g < 8) {
-            wg.code[0] = first_codes(wg.code[0], nb - 8 * g);
-            wu.code[0] = first_codes(wu.code[0], nb - 8 * g);
+            wg.code[0] = first_bytes(wg.code[0], nb - 8 * g);
+            wu.code[0] = first_bytes(wu.code[0], nb - 8 * g);
         }
         const Rows4<2> both = {{wg.v[0], wg.v[1], wu.v[0], wu.v[1]}, {wg.code[0], wu.code[0]}};
         fragments(both, own, lane, v);
@@ -409,8 +409,8 @@ struct TileProduct {
             for (int d = 0; d < 2; ++d) {  // (not SPLIT: stage g % 2)
                 bf16x8 v[2][8];
                 if (nb - 8 * g < 8) {
-                    w0[d].code[0] = first_codes(w0[d].code[0], nb - 8 * g);
-                    w1[d].code[0] = first_codes(w1[d].code[0], nb - 8 * g);
+                    w0[d].code[0] = first_bytes(w0[d].code[0], nb - 8 * g);
+                    w1[d].code[0] = first_bytes(w1[d].code[0], nb - 8 * g);
                 }
                 const Rows4<2> both = {{w0[d].v[0], w0[d].v[1], w1[d].v[0], w1[d].v[1]}, {w0[d].code[0], w1[d].code[0]}};
                 fragments(both, own, lane, v);
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork
             for (int d = 0; d < 2; ++d) {
                 const Place then = after(next);
                 bf16x8 v[1][8];
-                if (nb - 8 * now.g < 8) rows[d].code[0] = first_codes(rows[d].code[0], nb - 8 * now.g);
+                if (nb - 8 * now.g < 8) rows[d].code[0] = first_bytes(rows[d].code[0], nb - 8 * now.g);
                 fragments(rows[d], own, lane, v);
                 load_rows(rows[d], then);
                 sa.put(x, tokens_at, lane);

@@ -97,13 +97,13 @@ struct Source4 {
     }
 };
 
-// The codes of the first `left` blocks, 0 for the others (whose elements are zeros, and whose
-// codes may be NaN's).
-__device__ inline u32x2 first_codes(u32x2 code, int left)
+// The first `left` of eight bytes, zeros for the others: codes of blocks past the last one (whose
+// elements are zeros, and whose codes may be NaN's), 8-bit elements past the last term.
+__device__ inline u32x2 first_bytes(u32x2 x, int left)
 {
     const uint32_t lo = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
     const uint32_t hi = left >= 8 ? ~0u : left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
-    return u32x2{code[0] & lo, code[1] & hi};
+    return u32x2{x[0] & lo, x[1] & hi};
 }
 
 // Four lanes' blocks for the matrix cores: word b of lane group q becomes word q of block b.
@@ -286,12 +286,13 @@ struct Mx8Tokens {
     };
     const uint8_t *rows, *codes;
     int64_t lds;
-    int bytes, count, ld, nb;
+    int bytes, count, ld, nb, k;
 
-    // Rows first .. (n in all) of nb blocks.
-    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n, int nb_)
+    // Rows first .. (n in all) of k terms.
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n, int k_)
     {
-        nb = nb_;
+        k = k_;
+        nb = (k + 31) / 32;
         count = min(n - first, TOKENS);
         ld = (int)ld_;
         lds = lds_;
@@ -315,8 +316,11 @@ struct Mx8Tokens {
             d.code[i] = __builtin_amdgcn_raw_buffer_load_b8(c, inside ? 8 * t + block : kOutside, 0, 0);
         }
     }
-    __device__ inline void put(const Values& d, char* lds_, int, int lane) const
+    __device__ inline void put(Values& d, char* lds_, int g, int lane) const
     {
+        if (256 * g + 256 > k)
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) d.v[i] = first_bytes(d.v[i], k - 256 * g - lane % 32 * 8);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const float scale = scale_of_code(d.code[i] & 255);

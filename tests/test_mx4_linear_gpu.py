@@ -155,6 +155,33 @@ def test_values_that_are_not_finite(cuda, name):
     np.testing.assert_array_equal(ref.f64(Y), want)
 
 
+@pytest.mark.parametrize("mx8", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 7), (1, 9), (2, 31), (5, 33), (16, 250), (40, 262), (3, 319)])
+def test_what_lies_past_the_last_term(cuda, mx8, m, k):
+    """The first k columns of wider operands, X's others NaN: they count nowhere."""
+    import torch
+    import sushiblas_amd as sbx
+    rng = np.random.default_rng(100 * k + m)
+    n, wide = 40, 320
+    wn, wc, w = ref.random_mx4(rng, n, wide, 126, 129)
+    B, SB = ref.packed(cuda, wn, wc)
+    x, SX = rng.integers(-8, 9, (m, wide)), None
+    if mx8:
+        xn, xc = ref.quantize8(x)
+        x = ref.values8(xn, xc, wide)
+        X = xn.reshape(m, wide).copy()
+        X[:, k:] = 0x7F
+        X, SX = torch.from_numpy(X).to(cuda), torch.from_numpy(ref.codes(xc)).to(cuda)
+    else:
+        x = x.astype(np.float64)
+        X = torch.from_numpy(x).float().to(cuda)
+        X[:, k:] = float("nan")
+    Y = torch.empty((m, n), device=cuda)
+    sbx.mx4_linear(sbx.F32, m, n, k, 1.0, X, wide, B, B.shape[1], SB, SB.shape[1], 0.0, Y, n, SX=SX,
+                   ldsx=0 if SX is None else SX.shape[1])
+    np.testing.assert_array_equal(ref.f64(Y), x[:, :k] @ w[:, :k].T)
+
+
 def test_smallest_and_largest_scales(cuda):
     """Codes at both ends; x of the other end, so that products are ordinary."""
     _run(cuda, "f32", 3, 40, 96, codes=[0, 1, 2], x=np.full((3, 96), 2.0 ** 120), exact=False)
