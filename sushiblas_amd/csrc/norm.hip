@@ -187,17 +187,41 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a)
     }
 }
 
-// The gradient of a piece of a row, its input's gradient stored and its share of W's added to dw:
-// dx = s (dy w - h along) + dr with along = s^2 mean(dy w h).
+// What a row's gradient takes from its sums of squares and of dy w h: s = 1 / sqrt(mean + eps) as
+// (s / by) by, by a power of two, since eps may be 0 and s past what 32 bits hold (values below 2^-127) or
+// of few bits there (above 2^126), and m = s mean(dy w h).
+struct RowGrad {
+    float s, by, m;
+    __device__ inline RowGrad(const double (&sum)[2], double cols, double eps)
+    {
+        const double rs = rsqrt(sum[0] / cols + eps);
+        by = rs > 0x1p64 ? 0x1p64f : rs < 0x1p-64 ? 0x1p-64f : 1.0f;
+        s = (float)(rs / by);
+        m = (float)(sum[1] / cols * rs);
+    }
+    // Of a wave's only row, in scalar registers.
+    __device__ inline void keep_once()
+    {
+        auto once = [](float& x) {
+            x = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+        };
+        once(s);
+        once(by);
+        once(m);
+    }
+};
+
+// The gradient of a piece of a row, its input's gradient stored and its share of W's added to dw: with
+// n = h s, dx = s (dy w - n m) + dr.
 template <Cut CUT, typename T>
 __device__ inline void grad_piece(const NormGradArgs& a, int64_t row, int c, const Piece<T>& h, const Piece<T>& dy,
-                                  const Piece<T>& dr, const Piece<T>& w, float s, float along, float (&dw)[Piece<T>::N])
+                                  const Piece<T>& dr, const Piece<T>& w, const RowGrad& by, float (&dw)[Piece<T>::N])
 {
     Piece<T> dx;
 #pragma unroll
     for (int i = 0; i < Piece<T>::N; ++i) {
-        const float g = (float)dy.v[i], x = (float)h.v[i], n = x * s;
-        const float v = s * (g * (float)w.v[i]) - n * along;
+        const float g = (float)dy.v[i], n = (float)h.v[i] * by.by * by.s;
+        const float v = (g * (float)w.v[i] - n * by.m) * by.by * by.s;
         dx.v[i] = (T)(a.DR ? v + (float)dr.v[i] : v);
         dw[i] += g * n;
     }
@@ -256,8 +280,8 @@ __global__ void __launch_bounds__(1024) grad_kernel(NormGradArgs a)
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) grad_sums(h[p], dy[p], w[p], sum);
         row_sums<THREADS>(sum, part, slot);
-        const double rs = rsqrt(sum[0] / (double)a.cols + a.eps);
-        const double along = sum[1] / (double)a.cols * rs * rs;
+        RowGrad by(sum, (double)a.cols, a.eps);
+        if constexpr (THREADS >= 64) by.keep_once();
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             keep_packed(h[p]);
@@ -270,7 +294,7 @@ __global__ void __launch_bounds__(1024) grad_kernel(NormGradArgs a)
         if (inside)
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
-                grad_piece<CUT>(a, row, c0 + p * THREADS * N, h[p], dy[p], dr[p], w[p], (float)rs, (float)along, dw[p]);
+                grad_piece<CUT>(a, row, c0 + p * THREADS * N, h[p], dy[p], dr[p], w[p], by, dw[p]);
     }
     if (!a.DW) return;
     float* to = a.part + blockIdx.x * a.cols;
@@ -313,8 +337,7 @@ __global__ void __launch_bounds__(1024) grad_long_kernel(NormGradArgs a)
             grad_sums(whole_piece<CUT>(H, c, cols), whole_piece<CUT>(DY, c, cols),
                       whole_piece<CUT>(W, c, cols), sum);
         row_sums<1024>(sum, part, slot);
-        const double rs = rsqrt(sum[0] / (double)a.cols + a.eps);
-        const double along = sum[1] / (double)a.cols * rs * rs;
+        const RowGrad by(sum, (double)a.cols, a.eps);
         for (int c = threadIdx.x * N; c < end; c += STEP) {
             typedef Piece<float> four_t;
             float dw[N] = {};
@@ -330,7 +353,7 @@ __global__ void __launch_bounds__(1024) grad_long_kernel(NormGradArgs a)
             Piece<T> dr = {};
             if (a.DR) dr = whole_piece<CUT>((const T*)a.DR + row * a.lddr, c, cols);
             grad_piece<CUT>(a, row, c, whole_piece<CUT>(H, c, cols), whole_piece<CUT>(DY, c, cols), dr,
-                       whole_piece<CUT>(W, c, cols), (float)rs, (float)along, dw);
+                       whole_piece<CUT>(W, c, cols), by, dw);
             if (a.DW) {
                 if (inside)
 #pragma unroll

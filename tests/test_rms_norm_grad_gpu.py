@@ -11,14 +11,15 @@ import layer_reference as ref
 pytestmark = pytest.mark.gpu
 
 
-def _run(cuda, name, rows, cols, dr=True, dw=True, pads=(0, 0, 0, 0), alias="", eps=1e-6, h=None, stream=None):
+def _run(cuda, name, rows, cols, dr=True, dw=True, pads=(0, 0, 0, 0), alias="", eps=1e-6, h=None, stream=None,
+         dy=1.0):
     import torch
     import sushiblas_amd as sbx
     dt, code = ref.types(name)
     rng = np.random.default_rng(rows * 1013 + cols)
     h = rng.normal(size=(rows, cols)) if h is None else h
     H = ref.padded(cuda, h, dt, pads[0])
-    DY = ref.padded(cuda, rng.normal(size=(rows, cols)), dt, pads[1])
+    DY = ref.padded(cuda, rng.normal(size=(rows, cols)) * dy, dt, pads[1])
     DR = ref.padded(cuda, rng.normal(size=(rows, cols)), dt, pads[2]) if dr else None
     W = torch.from_numpy(1 + 0.1 * rng.normal(size=cols)).to(dt).to(cuda)
     with np.errstate(invalid="ignore"):
@@ -82,6 +83,16 @@ def test_values_that_are_not_finite(cuda, cols):
     h[3] = 0.0
     _run(cuda, "f32", 6, cols, h=h, dw=False)
     _run(cuda, "bf16", 6, cols, h=h, dw=False)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [1, 40, 3000, 18000])
+@pytest.mark.parametrize("scale,dy", [(-130, -20), (-100, -20), (-60, 0), (70, 0), (126, 60)])
+def test_far_magnitudes(cuda, name, cols, scale, dy):
+    """1 / rms past what 32 bits hold, below their normal numbers, and between; no eps."""
+    h = np.random.default_rng(cols).uniform(0.5, 1.0, size=(5, cols)) * 2.0 ** scale
+    h[:, ::2] *= -1
+    _run(cuda, name, 5, cols, dr=False, eps=0.0, h=h, dy=2.0 ** dy)
 
 
 def test_no_rows(cuda):
