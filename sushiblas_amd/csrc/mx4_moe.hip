@@ -27,6 +27,23 @@ namespace {
 template <typename T>
 constexpr int kActPieces = sizeof(T) == 4 ? 3 : 2;
 
+// x in the wave's lower half and y in its upper one, each added to its own other half.
+__device__ inline double halves(double x, double y)
+{
+    const uint64_t a = __builtin_bit_cast(uint64_t, x), b = __builtin_bit_cast(uint64_t, y);
+    auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)a, (uint32_t)b, false, false);
+    auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+// The same by rows of 16 lanes: x in the even ones, y in the odd ones.
+__device__ inline double quarters(double x, double y)
+{
+    const uint64_t a = __builtin_bit_cast(uint64_t, x), b = __builtin_bit_cast(uint64_t, y);
+    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)a, (uint32_t)b, false, false);
+    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+
 // Four experts and TOKENS (1 or 4) tokens a workgroup, whose four waves take a quarter of the terms each.
 // Logits in 64 bits, so that which experts are chosen does not depend on the order of the sums.
 // Workgroups past the experts' make pieces.
@@ -98,13 +115,14 @@ __global__ void __launch_bounds__(256) prepare_kernel(Mx4MoeArgs a, Mx4MoeWork w
         for (int j = 0; j < TOKENS; ++j) xe[j] = x[j][whole + threadIdx.x];
         add(we, xe);
     }
+    // Sums over the wave: of four numbers at a time, so that each row of lanes is left with one of them.
+    double* all = &sum[0][0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < TOKENS; ++j) {
-            const double s = sum64(sum[i][j]);
-            if (lane == 0) part[wave][i * TOKENS + j] = s;
-        }
+    for (int i = 0; i < 4 * TOKENS; i += 4) {
+        const double two[2] = {halves(all[i], all[i + 1]), halves(all[i + 2], all[i + 3])};
+        const double s = sum16(quarters(two[0], two[1]));
+        if (lane % 16 == 0) part[wave][i + (lane / 16 % 2 * 2 + lane / 32)] = s;
+    }
     __syncthreads();
     const int i = threadIdx.x / TOKENS, j = threadIdx.x % TOKENS;
     if (i < 4 && e0 + i < a.experts && t0 + j < a.tokens)
