@@ -670,9 +670,15 @@ __global__ void __launch_bounds__(256) combine_kernel(Mx4MoeArgs a, Mx4MoeWork w
     const int n = (blockIdx.x * 256 + threadIdx.x) * 4, t = blockIdx.y;
     if (n >= a.width) return;
     const float* from = (const float*)(a.work + w.out) + (size_t)t * a.topk * w.out_ld + n;
-    f32x4 v = *(const f32x4*)from;
-#pragma unroll 4
-    for (int j = 1; j < a.topk; ++j) v += *(const f32x4*)(from + (size_t)j * w.out_ld);
+    f32x4 v = {};
+    for (int j = 0; j < a.topk; j += 4) {  // four loads under way
+        f32x4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *(const f32x4*)(from + (size_t)min(j + i, a.topk - 1) * w.out_ld);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (j + i < a.topk) v += x[i];
+    }
     T* y = (T*)a.Y + t * a.ldy + n;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
