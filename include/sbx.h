@@ -337,7 +337,7 @@ int sbx_mx8_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, cons
  * (SX NULL) or is an MXFP8 matrix (X, SX), B (n x k) is an MXFP4 matrix, Y (m x n) of
  * dtype.  X is not rounded (but for bits of fp32 values below 2^-133, which do not
  * count); sums are held in 32 bits and rounded to dtype once.  What lies past the
- * k-th term is not used.  BLAS semantics as for GEMM (beta == 0: Y is
+ * k-th term is not used; Y lies apart from X and B.  BLAS semantics as for GEMM (beta == 0: Y is
  * not read; alpha == 0 or k == 0: X and B are not).  Rows are computed apart: those of
  * one call have the bits that they have alone.  m <= 1024, n <= 2^30, k <= 2^23, ldb <
  * 2^23 - 15, a row of X (ldx) at most 2^26 bytes (else SBX_UNSUPPORTED). */
@@ -357,7 +357,8 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  * before W2's they are held as the sum of two bf16 values (F32: three), 16 bits (24) where
  * dtype has 8 or 11.  Sums are held in
  * 32 bits and rounded to dtype once.
- * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.
+ * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.  Y may be X
+ * (same leading dimension).
  * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^18, ld1, ld2 < 2^23 -
  * 15, a row of X (ldx) less than 2^23 - 15 bytes (else SBX_UNSUPPORTED). */
 int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,

@@ -169,6 +169,37 @@ def test_same_bits_again_streams_workspaces_and_replays(cuda):
         assert torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
 
 
+@pytest.mark.parametrize("tokens", [1, 5, 90])
+def test_in_place(cuda, tokens):
+    import torch
+    m = Mixture(cuda, "bf16", 300, 130, 9)
+    x = torch.randn(tokens, 310, device=cuda).bfloat16()
+    y, was = x.clone(), x.clone()
+    m.call(x[:, :300], y[:, :300], 3, False)
+    m.call(x[:, :300], x[:, :300], 3, False)
+    assert torch.equal(x, y) and torch.equal(x[:, 300:], was[:, 300:])
+
+
+def test_two_at_once(cuda):
+    """Calls on two streams, a workspace each, of the same weights."""
+    import torch
+    import sushiblas_amd as sbx
+    m = Mixture(cuda, "f16", 1024, 512, 16)
+    streams, xs, ys = [torch.cuda.Stream() for _ in range(2)], [], []
+    for tokens in (3, 40):
+        xs.append(torch.randn(tokens, 1024, device=cuda).half())
+        ys.append([torch.empty_like(xs[-1]) for _ in range(9)])
+        m.call(xs[-1], ys[-1][0], 4, True)
+    ws = [torch.empty(sbx.mx4_moe_workspace(x.shape[0], 1024, 512, 16, 4), dtype=torch.uint8, device=cuda) for x in xs]
+    torch.cuda.synchronize()
+    for i in range(1, 9):
+        for x, y, s, w in zip(xs, ys, streams, ws):
+            m.call(x, y[i], 4, True, ws=w, stream=s)
+    torch.cuda.synchronize()
+    for y in ys:
+        assert all(torch.equal(y[0], other) for other in y[1:])
+
+
 @pytest.mark.parametrize("name", ref.TYPES)
 @pytest.mark.parametrize("tokens", [1, 6])
 def test_a_step_of_decoding(cuda, name, tokens):
