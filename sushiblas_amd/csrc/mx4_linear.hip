@@ -114,6 +114,97 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
     }
 }
 
+// Many rows of X in pieces: four waves take 32 rows of B each, and tiles of 16 rows of X lie in LDS for all of
+// them, a group after another, the next one on its way; so X is read, and its pieces are made, once for 128
+// rows of B.  Four more waves have the same rows and every other group, so that one's products go on while another
+// waits for LDS (64 x 8192 x 8192 fp16 33.6 us, by four waves alone 41.4, by linear_kernel 44.5; fp32 40.9, 56.3, 66.6).
+//   A row's bits are linear_kernel's: sums of every fourth group stay apart, as its four waves' are.
+//   Bound by a wave's own way through LDS and conversions, which two waves to a SIMD do not hide: bf16,
+// with nothing to split, gains nothing (24.5 against 25.6; 256 x 8192 x 4096 50.2 against 46.0).
+constexpr int kTallRows = 128, kTallTokens = 16;
+template <typename T>
+__global__ void __launch_bounds__(512, 2) linear_tall_kernel(Mx4LinearArgs p)
+{
+    constexpr int WAVES = 4, SETS = 2, TOKENS = kTallTokens, PER = TOKENS / WAVES;
+    typedef DenseTokens<T, PER> tokens_t;
+    constexpr int PIECES = tokens_t::PIECES, FRAGMENTS = fragments_of(PIECES, TOKENS), STAGE = tokens_bytes(PIECES, TOKENS);
+    __shared__ __align__(16) char lds[SETS * (2 * STAGE + WAVES * rows4_bytes(2))];
+    const int lane = threadIdx.x % 64, id = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave = id % WAVES, set = id / WAVES;
+    const int x0 = block_x() * kTallRows, y0 = blockIdx.y * TOKENS;
+    if (x0 >= p.n) return;
+    const int nb = (p.k + 31) / 32, groups = (nb + 7) / 8, n0 = x0 + 32 * wave;
+    char *stage = lds + set * 2 * STAGE, *own = lds + SETS * 2 * STAGE + id * rows4_bytes(2);
+    // (past the last row of B or X: that one, not stored)
+    const int row = min(n0, p.n - 1), first = min(y0 + PER * wave, p.m - 1);
+    Source4<2> sw;
+    sw.init(p.ldb, p.ldsb, p.n - row, nb, lane);
+    sw.move(p.B, p.SB, row);
+    tokens_t sa;
+    const int ld = (int)(p.ldx * sizeof(T)), count = min(p.m - first, PER);
+    sa.init((const T*)p.X + first * p.ldx, (count - 1) * ld + p.k * (int)sizeof(T), p.k,
+            [&](int t) { return t < count ? t * ld : kOutside; }, lane);
+    constexpr int SUMS = 4 / SETS;  // of groups 4 i + SETS u + set
+    f32x4 acc[SUMS][FRAGMENTS][2] = {};
+    Rows4<2> w[2];
+    typename tokens_t::Values a;
+    sa.load(a, set, lane);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) sw.load(w[d], set + SETS * d, nb - 8 * (set + SETS * d));
+    sa.template put<TOKENS>(a, stage, set, lane, PER * wave);
+    sa.load(a, set + SETS, lane);
+    lds_barrier();
+    // (both sets go as often; a group past the last one is zeros)
+    for (int g = set; g - set < groups;) {
+#pragma unroll
+        for (int u = 0; u < SUMS; ++u) {
+            const int d = u % 2;
+            bf16x8 v[2][8];
+            if (nb - 8 * g < 8)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[d].code[i] = first_bytes(w[d].code[i], nb - 8 * g);
+            fragments(w[d], own, lane, v);
+            const int next = g + 2 * SETS;
+            sw.load(w[d], next, nb - 8 * next);
+            sa.template put<TOKENS>(a, stage + (1 - d) * STAGE, g + SETS, lane, PER * wave);  // its last readers passed the barrier before
+            sa.load(a, next, lane);
+            multiply<PIECES, TOKENS>(acc[u], v, stage + d * STAGE, lane);
+            lds_barrier();
+            g += SETS;
+            if (g - set >= groups) break;
+        }
+    }
+    static_assert(WAVES * SUMS * FRAGMENTS * 2 * 64 * 16 <= sizeof(lds), "");
+    f32x4* part = (f32x4*)lds + wave * (SUMS * FRAGMENTS * 2 * 64) + lane;
+    if (set == 1)
+#pragma unroll
+        for (int u = 0; u < SUMS; ++u)
+#pragma unroll
+            for (int x = 0; x < FRAGMENTS; ++x)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) part[((u * FRAGMENTS + x) * 2 + i) * 64] = acc[u][x][i];
+    __syncthreads();
+    const int m = y0 + lane % 16;
+    if (set == 1 || m >= p.m) return;
+    T* Y = (T*)p.Y + m * p.ldy;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f32x4 v = {};
+#pragma unroll
+        for (int u = 0; u < SUMS; ++u) {
+#pragma unroll
+            for (int x = 0; x < FRAGMENTS; ++x) v += acc[u][x][i];
+#pragma unroll
+            for (int x = 0; x < FRAGMENTS; ++x) v += part[((u * FRAGMENTS + x) * 2 + i) * 64];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = n0 + 16 * i + 4 * (lane / 16) + e;
+            if (n < p.n) Y[n] = result<T>(v[e], p.beta != 0.0f ? (float)Y[n] : 0.0f, p);
+        }
+    }
+}
+
 // Fewer terms than a piece has, or none.  A thread to a result.
 template <typename T>
 __global__ void __launch_bounds__(256) few_terms_kernel(Mx4LinearArgs p)
@@ -161,8 +252,19 @@ hipError_t launch(const Mx4LinearArgs& a, hipStream_t s)
     // 8192 x 8192 bf16 27.9 us against 24.9).
     constexpr bool SPLIT = !MX8 && kBf16Pieces<T> > 1;
     if (a.m <= 2) return launch_form<T, MX8, 2, 1>(a, s);
-    if constexpr (SPLIT)
+    if constexpr (SPLIT) {
         if (a.m <= 8) return launch_form<T, MX8, 8, 1>(a, s);
+        // Past one round of those workgroups (two to a CU; one of fp16's two tiles) the other kernel, which has a
+        // round of its own less: fp16 16 x 17000 x 8192 32.6 us against 39.7, but 16 x 12000 x 8192 32.0 against 27.5;
+        // fp32 17 x 8192 x 8192 38.5 against 34.9, but 20 x 9000 x 8192 39.1 against 52.8.
+        const bool two = sizeof(T) == 2 && a.m > 16;
+        const int64_t others = (int64_t)((a.n + 31) / 32) * ((a.m + (two ? 31 : 15)) / (two ? 32 : 16));
+        if (a.n > 16 * 256 && others > (two ? 256 : 512)) {
+            linear_tall_kernel<T><<<grid_of((a.n + kTallRows - 1) / kTallRows,
+                                            (unsigned)((a.m + kTallTokens - 1) / kTallTokens)), 512, 0, s>>>(a);
+            return hipGetLastError();
+        }
+    }
     if constexpr (SPLIT && sizeof(T) == 4)  // (three pieces of 16 tokens would not fit the LDS)
         return launch_form<T, MX8, 8, 2>(a, s);
     else

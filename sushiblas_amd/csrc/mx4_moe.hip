@@ -406,7 +406,6 @@ struct TileProduct {
                     *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
                 }
         };
-        auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (loads go on)
         Rows4<1> w0[2], w1[2];
         load_tokens(first);
 #pragma unroll
@@ -418,7 +417,7 @@ struct TileProduct {
         if constexpr (!SPLIT) {
             put_tokens(stage);
             load_tokens(1);
-            barrier();
+            lds_barrier();
         }
 #pragma unroll
         for (int f = 0; f < FRAGMENTS; ++f) acc[f][0] = acc[f][1] = f32x4{};
@@ -443,7 +442,7 @@ struct TileProduct {
                     put_tokens(stage + (1 - d) * STAGE);  // its last readers passed the barrier before
                     load_tokens(g + 2);
                     multiply<PIECES, TOKENS>(acc, v, stage + d * STAGE, lane);
-                    barrier();
+                    lds_barrier();
                 }
                 g += STEP;
                 if (g >= groups) break;

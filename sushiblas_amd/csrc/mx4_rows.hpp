@@ -199,11 +199,11 @@ constexpr int tokens_bytes(int pieces, int tokens) { return 512 * pieces * token
 constexpr int fragments_of(int pieces, int tokens) { return (pieces * tokens + 15) / 16; }
 
 template <int PIECES, int TOKENS>
-__device__ inline void put_tokens(char* lds, int i, int lane, const bf16x8 (&x)[PIECES])
+__device__ inline void put_tokens(char* lds, int i, int lane, const bf16x8 (&x)[PIECES], int first = 0)
 {
 #pragma unroll
     for (int n = 0; n < PIECES; ++n) {
-        const int row = n * TOKENS + 2 * i + lane / 32;
+        const int row = n * TOKENS + first + 2 * i + lane / 32;
         *(bf16x8*)(lds + row * 512 + (lane % 32 ^ row % 16) * 16) = x[n];
     }
 }
@@ -251,8 +251,9 @@ struct DenseTokens {
                     Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(v, at[i] == kOutside ? kOutside : at[i] + c, 0, 0));
         }
     }
-    // To LDS.
-    __device__ inline void put(Values& d, char* lds, int g, int lane) const
+    // To LDS, as tokens first .. of a tile of TILE.
+    template <int TILE = TOKENS>
+    __device__ inline void put(Values& d, char* lds, int g, int lane, int first = 0) const
     {
         if (256 * g + 256 > k)
 #pragma unroll
@@ -271,7 +272,7 @@ struct DenseTokens {
                 for (int e = 0; e < 8; ++e) f[e] = (float)d.v[i][e / Piece<T>::N].v[e % Piece<T>::N];
                 split(f, x);
             }
-            put_tokens<PIECES, TOKENS>(lds, i, lane, x);
+            put_tokens<PIECES, TILE>(lds, i, lane, x, first);
         }
     }
 };
@@ -377,6 +378,9 @@ struct PieceTokens {
         }
     }
 };
+
+// A workgroup's barrier for what lies in LDS; loads from memory go on.
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // acc[f][i]: rows 4 (lane / 16) + e of block i of w, row 16 f + lane % 16 of the tile in LDS.
 template <int PIECES, int TOKENS, int N>

@@ -78,7 +78,7 @@ def _run(cuda, name, m, n, k, alpha=1.0, beta=0.0, relu=False, mx8=False, pads=(
 SIZES = [(1, 1, 1), (1, 1, 32), (1, 17, 33), (2, 5, 128), (1, 300, 257), (3, 16, 256), (15, 65, 100), (16, 32, 512),
          (17, 31, 1000), (5, 64, 64), (31, 130, 300), (32, 1000, 96), (33, 257, 511), (48, 200, 768), (64, 256, 1024),
          (65, 70, 300), (8, 2000, 2040), (16, 1030, 2049), (1, 5000, 2300), (7, 640, 640), (1, 8193, 70), (4, 9000, 300),
-         (100, 50, 260), (300, 40, 100), (1024, 20, 40)]
+         (100, 50, 260), (300, 40, 100), (1024, 20, 40), (18, 4100, 300), (33, 4225, 2049), (64, 4352, 1024), (200, 4130, 40)]
 
 
 @pytest.mark.parametrize("name", ref.TYPES)
@@ -208,6 +208,35 @@ def test_rows_have_the_bits_that_they_have_alone(cuda):
         sbx.mx4_linear(code, m, n, k, 1.0, X, k, *args, both[0], n)
         for i in range(m):
             sbx.mx4_linear(code, 1, n, k, 1.0, X[i], k, *args, both[1][i], n)
+        assert torch.equal(both[0], both[1])
+
+
+@pytest.mark.parametrize("mx8", [False, True])
+@pytest.mark.parametrize("m,n,k", [(60, 4200, 3001), (17, 4097, 260), (70, 4500, 8), (52, 4200, 1030)])
+def test_rows_of_tall_weights(cuda, mx8, m, n, k):
+    """Among many rows of X and of B: the same bits as alone."""
+    import torch
+    import sushiblas_amd as sbx
+    rng = np.random.default_rng(m)
+    wn, wc, _ = ref.random_mx4(rng, n, k, 110, 140)
+    B, SB = ref.packed(cuda, wn, wc)
+    nb = -(-k // 32)
+    for name in ref.TYPES:
+        dt, code = ref.types(name)
+        kw, alone = {}, {}
+        if mx8:
+            xn, xc = ref.quantize8(rng.normal(size=(m, k)) * np.exp2(rng.integers(-6, 7, (m, k))))
+            X, S = (torch.from_numpy(v).to(cuda) for v in (xn.reshape(m, 32 * nb), ref.codes(xc)))
+            kw = dict(SX=S, ldsx=S.shape[1])
+        else:
+            X = torch.from_numpy(rng.normal(size=(m, k)) * np.exp2(rng.integers(-6, 7, (m, k)))).to(dt).to(cuda)
+        both = [torch.full((m, n + 3), 7.0, dtype=dt, device=cuda) for _ in range(2)]
+        args = (B, B.shape[1], SB, SB.shape[1], 0.0)
+        sbx.mx4_linear(code, m, n, k, 0.5, X, X.shape[1], *args, both[0], n + 3, **kw)
+        for i in range(m):
+            if mx8:  # (a row's codes are a run of 8 bytes in each group's)
+                alone = dict(SX=S[:, 8 * i:], ldsx=S.shape[1])
+            sbx.mx4_linear(code, 1, n, k, 0.5, X[i], X.shape[1], *args, both[1][i], n + 3, **alone)
         assert torch.equal(both[0], both[1])
 
 
