@@ -320,8 +320,8 @@ int sbx_rms_norm(void* stream, int dtype, int64_t rows, int64_t cols, const void
  *        reaches H along the residual), which is X's and R's of sbx_rms_norm alike
  *   DW = the sum over rows of s * DY * H, in 32 bits (NULL: not wanted, and no workspace)
  * s is computed again from H, so the forward call stores none.  DX may be DY or DR
- * (same leading dimension).  The order of DW's sums depends on rows alone.  Without
- * rows DW is zero. */
+ * (same leading dimension).  The order of DW's sums depends on rows, cols and
+ * dtype alone.  Without rows DW is zero. */
 int sbx_rms_norm_grad(void* stream, int dtype, int64_t rows, int64_t cols, const void* H, int64_t ldh,
                       const void* W, double eps, const void* DY, int64_t lddy, const void* DR,
                       int64_t lddr, void* DX, int64_t lddx, float* DW, void* workspace,

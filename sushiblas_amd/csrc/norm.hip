@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(1024) grad_long_kernel(NormGradArgs a)
     }
 }
 
-// W's gradient from its parts: 64 columns a workgroup at a time, its 16 waves every 16th part each.
+// W's gradient from its parts (none: zeros): 64 columns a workgroup at a time, its 16 waves every 16th part each.
 __global__ void __launch_bounds__(1024) parts_kernel(const float* part, int parts, int64_t cols, float* DW)
 {
     __shared__ float sums[16][64];
@@ -473,13 +473,22 @@ hipError_t norm(const NormArgs& a, hipStream_t s)
     }
 }
 
+// The only part is W's gradient.
+NormGradArgs whole(NormGradArgs a, int parts)
+{
+    if (parts == 1) a.part = a.DW;
+    return a;
+}
+
 template <typename T, Cut CUT, int THREADS, int PIECES>
 int launch_grad(const NormGradArgs& a, hipStream_t s)
 {
     constexpr int ROWS = 1024 / THREADS;
+    // Up to two turns go to one workgroup, which writes W's gradient itself: a second launch costs as much or more
+    // (4 x 4096 bf16, one turn, 6.8 us against 10.1; 128 x 128, two, 6.6 against 9.7; 8 x 4096, two, 10.0 either way).
     const int64_t groups = (a.rows + ROWS - 1) / ROWS;
-    const int parts = groups < kNormGradParts ? (int)groups : kNormGradParts;
-    grad_kernel<T, CUT, THREADS, PIECES><<<parts, 1024, 0, s>>>(a);
+    const int parts = groups <= 2 ? 1 : groups < kNormGradParts ? (int)groups : kNormGradParts;
+    grad_kernel<T, CUT, THREADS, PIECES><<<parts, 1024, 0, s>>>(whole(a, parts));
     return parts;
 }
 
@@ -496,7 +505,7 @@ int norm_grad(const NormGradArgs& a, int64_t pieces, hipStream_t s)
         if (pieces <= 1024) return launch_grad<T, CUT, 512, 2>(a, s);
         if (pieces <= 2048) return launch_grad<T, CUT, 1024, 2>(a, s);
         const int parts = a.rows < kNormGradParts ? (int)a.rows : kNormGradParts;
-        grad_long_kernel<T, CUT><<<parts, 1024, 0, s>>>(a);
+        grad_long_kernel<T, CUT><<<parts, 1024, 0, s>>>(whole(a, parts));
         return parts;
     }
     return 0;
@@ -549,7 +558,7 @@ hipError_t launch_rms_norm_grad(int dtype, const NormGradArgs& a, hipStream_t s)
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (!a.DW) return hipSuccess;
+    if (!a.DW || parts == 1) return hipSuccess;
     const int64_t tiles = (a.cols + 63) / 64;
     parts_kernel<<<(unsigned)(tiles < 65536 ? tiles : 65536), 1024, 0, s>>>(a.part, parts, a.cols, a.DW);
     return hipGetLastError();
