@@ -16,14 +16,37 @@ __device__ inline T result(float acc, float y, const Mx4LinearArgs& p)
     return (T)(p.relu ? (v > 0.0f ? v : 0.0f) : v);
 }
 
+// The groups of terms of one of WAVES waves (or of as many sums), one after another: first, first + WAVES, ..;
+// from one of them that differs from block to block of B's rows, and round, where rows lie 4096 bytes apart
+// or a multiple: workgroups that are at the same terms of all rows would meet in the same memory channels
+// (1 x 8192 x 8192 bf16 12.0 us, so 9.3; 1 x 28672 x 8192 28.4, so 24.0.  1 x 8192 x 12288, rows 6144 apart,
+// 12.6, so 12.9).
+template <int WAVES>
+struct Turns {
+    int first, count, start;
+    __device__ inline Turns(const Mx4LinearArgs& p, int first_, int groups, int block)
+    {
+        first = first_;
+        count = (groups - first + WAVES - 1) / WAVES;
+        start = p.ldb % 4096 == 0 && count > 1 ? (int)((uint32_t)block * 2654435761u >> 16) % count : 0;
+    }
+    // The i-th; of i >= count one past the last group (zeros where it is loaded).
+    __device__ inline int group(int i) const
+    {
+        return first + WAVES * (i >= count ? i : i + start < count ? i + start : i + start - count);
+    }
+};
+
+constexpr int kTallRows = 128, kTallTokens = 16;
+
 // A workgroup takes 16 XB rows of B and YB tiles of TOKENS rows of X, its waves a share each of the
 // terms, in groups of 256 by turns; AHEAD groups of B are under way, and of X (of a larger tile than
 // 2 rows the next one alone, for want of registers).  The waves' sums are added up in LDS, in order.
 // Which wave has a term does not depend on m, so a row's bits do not either.
-//   One token is bound by memory: bf16 1 x 28672 x 8192 26.5 us (125 MB, 4.7 TB/s; the product of
-// MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 10.7 (36 MB: 2.6 of it are any kernel's, then the first
-// loads' way, and there is one round).  Four groups ahead in place of two 11.4, blocks that follow one
-// another to a wave in place of turns 11.2 against 11.4.  More tokens are bound by X's way from the
+//   One token is bound by memory: bf16 1 x 28672 x 8192 23.9 us (125 MB, 5.2 TB/s; the product of
+// MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 9.0-9.8 (36 MB: 2.6 of it are any kernel's, then the first
+// loads' way, and there is one round).  Four groups ahead in place of two are slower (11.4 for 10.7 before the
+// groups' order changed).  More tokens are bound by X's way from the
 // L2s, as each workgroup reads all of it: 16 x 28672 x 8192 38 us, loads alone as long (64 rows of B a
 // workgroup take too many registers: 79).
 template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
@@ -59,28 +82,32 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
     typename tokens_t::Values a[AHEAD_X];
     // (no branch around a load, and one past the last group reads zeros or the last group again: the
     // compiler would wait for all of them where paths meet)
+    const Turns<WAVES> own_turns(p, wave, groups, x0 / (PIECES == 1 ? 32 : kTallRows));
+    const int turns = own_turns.count;
+    auto group = [&](int i) { return own_turns.group(i); };
 #pragma unroll
     for (int d = 0; d < AHEAD; ++d) {
-        sw.load(w[d], wave + d * WAVES, nb - 8 * (wave + d * WAVES));
-        if (d < AHEAD_X) sa[0].load(a[d], wave + d * WAVES, lane);
+        const int g = group(d);
+        sw.load(w[d], g, nb - 8 * g);
+        if (d < AHEAD_X) sa[0].load(a[d], g, lane);
     }
-    for (int g = wave; g < groups;) {
+    for (int turn = 0; turn < turns;) {
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d) {
+            const int g = group(turn), next = group(turn + AHEAD), next_x = group(turn + AHEAD_X);
             bf16x8 v[XB][8];
             if (nb - 8 * g < 8)
 #pragma unroll
                 for (int i = 0; i < XB; ++i) w[d].code[i] = first_bytes(w[d].code[i], nb - 8 * g);
             fragments(w[d], own, lane, v);
-            sw.load(w[d], g + AHEAD * WAVES, nb - 8 * (g + AHEAD * WAVES));
+            sw.load(w[d], next, nb - 8 * next);
 #pragma unroll
             for (int j = 0; j < YB; ++j) {
                 sa[j].put(a[d % AHEAD_X], tokens_at, g, lane);
-                sa[j + 1 < YB ? j + 1 : 0].load(a[d % AHEAD_X], j + 1 < YB ? g : g + AHEAD_X * WAVES, lane);
+                sa[j + 1 < YB ? j + 1 : 0].load(a[d % AHEAD_X], j + 1 < YB ? g : next_x, lane);
                 multiply<PIECES, TOKENS>(acc[j], v, tokens_at, lane);
             }
-            g += WAVES;
-            if (g >= groups) break;
+            if (++turn == turns) break;
         }
     }
 
@@ -121,7 +148,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 //   A row's bits are linear_kernel's: sums of every fourth group stay apart, as its four waves' are.
 //   Bound by a wave's own way through LDS and conversions, which two waves to a SIMD do not hide: bf16,
 // with nothing to split, gains nothing (24.5 against 25.6; 256 x 8192 x 4096 50.2 against 46.0).
-constexpr int kTallRows = 128, kTallTokens = 16;
 template <typename T>
 __global__ void __launch_bounds__(512, 2) linear_tall_kernel(Mx4LinearArgs p)
 {
@@ -145,33 +171,35 @@ __global__ void __launch_bounds__(512, 2) linear_tall_kernel(Mx4LinearArgs p)
     sa.init((const T*)p.X + first * p.ldx, (count - 1) * ld + p.k * (int)sizeof(T), p.k,
             [&](int t) { return t < count ? t * ld : kOutside; }, lane);
     constexpr int SUMS = 4 / SETS;  // of groups 4 i + SETS u + set
+    const Turns<4> mine[SUMS] = {{p, set, groups, x0 / kTallRows}, {p, set + SETS, groups, x0 / kTallRows}};
     f32x4 acc[SUMS][FRAGMENTS][2] = {};
-    Rows4<2> w[2];
+    Rows4<2> w[SUMS];
     typename tokens_t::Values a;
-    sa.load(a, set, lane);
+    auto load_rows = [&](int u, int turn) {
+        const int g = mine[u].group(turn);
+        sw.load(w[u], g, nb - 8 * g);
+    };
+    sa.load(a, mine[0].group(0), lane);
 #pragma unroll
-    for (int d = 0; d < 2; ++d) sw.load(w[d], set + SETS * d, nb - 8 * (set + SETS * d));
-    sa.template put<TOKENS>(a, stage, set, lane, PER * wave);
-    sa.load(a, set + SETS, lane);
+    for (int u = 0; u < SUMS; ++u) load_rows(u, 0);
+    sa.template put<TOKENS>(a, stage, mine[0].group(0), lane, PER * wave);
+    sa.load(a, mine[1].group(0), lane);
     lds_barrier();
-    // (both sets go as often; a group past the last one is zeros)
-    for (int g = set; g - set < groups;) {
+    const int turns = (groups + 3) / 4;  // of all: the last one without a group, perhaps
+    for (int turn = 0; turn < turns; ++turn) {
 #pragma unroll
         for (int u = 0; u < SUMS; ++u) {
-            const int d = u % 2;
+            const int g = mine[u].group(turn), then = mine[1 - u].group(turn + u);
             bf16x8 v[2][8];
             if (nb - 8 * g < 8)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) w[d].code[i] = first_bytes(w[d].code[i], nb - 8 * g);
-            fragments(w[d], own, lane, v);
-            const int next = g + 2 * SETS;
-            sw.load(w[d], next, nb - 8 * next);
-            sa.template put<TOKENS>(a, stage + (1 - d) * STAGE, g + SETS, lane, PER * wave);  // its last readers passed the barrier before
-            sa.load(a, next, lane);
-            multiply<PIECES, TOKENS>(acc[u], v, stage + d * STAGE, lane);
+                for (int i = 0; i < 2; ++i) w[u].code[i] = first_bytes(w[u].code[i], nb - 8 * g);
+            fragments(w[u], own, lane, v);
+            load_rows(u, turn + 1);
+            sa.template put<TOKENS>(a, stage + (1 - u) * STAGE, then, lane, PER * wave);  // its last readers passed the barrier before
+            sa.load(a, mine[u].group(turn + 1), lane);
+            multiply<PIECES, TOKENS>(acc[u], v, stage + u * STAGE, lane);
             lds_barrier();
-            g += SETS;
-            if (g - set >= groups) break;
         }
     }
     static_assert(WAVES * SUMS * FRAGMENTS * 2 * 64 * 16 <= sizeof(lds), "");
@@ -233,8 +261,8 @@ hipError_t launch_form(const Mx4LinearArgs& a, hipStream_t s)
         linear_kernel<T, MX8, TOKENS, YB, 1, 8><<<grid_of((a.n + 15) / 16, gy), 512, 0, s>>>(a);
     } else {
         // several workgroups to a CU, of four waves: one's loads go on while another adds up (1 x 28672
-        // x 8192 26.5 us, by eight 28.9).  Two blocks each (16 x 28672 x 8192 38 us, one 45), but for one
-        // token of one piece (28.7 against 26.5)
+        // x 8192, groups in order, 26.5 us, by eight 28.9).  Two blocks each (16 x 28672 x 8192 38 us, one 45), but for one
+        // token of one piece (28.7 against 26.5; 12000 x 4096 8.7 against 7.6)
         constexpr int XB = TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1) ? 1 : 2;
         linear_kernel<T, MX8, TOKENS, YB, XB, 4><<<grid_of((a.n + 16 * XB - 1) / (16 * XB), gy), 256, 0, s>>>(a);
     }

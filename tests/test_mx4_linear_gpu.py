@@ -240,6 +240,37 @@ def test_rows_of_tall_weights(cuda, mx8, m, n, k):
         assert torch.equal(both[0], both[1])
 
 
+@pytest.mark.parametrize("name", ref.TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 300, 2049), (7, 40, 4000), (20, 100, 300), (64, 4352, 1100), (1, 4200, 3000),
+                                   (3, 8200, 1500), (70, 4400, 2300), (12, 16500, 270), (2, 20, 8192)])
+def test_rows_4096_bytes_apart(cuda, name, m, n, k):
+    """Weights whose rows are so far apart, or a multiple: groups of terms in another order."""
+    _run(cuda, name, m, n, k, pads=(0, 0, 0, 256 - -(-k // 32), 0))
+    _run(cuda, name, m, n, k, mx8=True, pads=(0, 0, 0, 512 - -(-k // 32), 0))
+
+
+@pytest.mark.parametrize("m,n,k", [(60, 4200, 3001), (17, 600, 2600), (70, 4500, 2050)])
+def test_rows_4096_bytes_apart_have_the_bits_that_they_have_alone(cuda, m, n, k):
+    import torch
+    import sushiblas_amd as sbx
+    rng = np.random.default_rng(m)
+    wn, wc, _ = ref.random_mx4(rng, n, k, 110, 140)
+    B, SB = ref.packed(cuda, wn, wc, 256 - -(-k // 32))
+    assert B.shape[1] == 4096
+    for name in ref.TYPES:
+        dt, code = ref.types(name)
+        X = torch.from_numpy(rng.normal(size=(m, k)) * np.exp2(rng.integers(-6, 7, (m, k)))).to(dt).to(cuda)
+        X[3, 5], X[m - 1, k - 1] = float("inf"), float("nan")
+        both = [torch.empty((m, n), dtype=dt, device=cuda) for _ in range(2)]
+        args = (B, B.shape[1], SB, SB.shape[1], 0.0)
+        sbx.mx4_linear(code, m, n, k, 1.0, X, k, *args, both[0], n)
+        for i in range(m):
+            sbx.mx4_linear(code, 1, n, k, 1.0, X[i], k, *args, both[1][i], n)
+        fine = ~torch.isnan(both[1])
+        assert torch.equal(both[0][fine], both[1][fine]) and torch.equal(torch.isnan(both[0]), ~fine)
+        assert bool(fine[:3].all()) and not bool(torch.isfinite(both[0][3]).any())
+
+
 def test_another_stream_and_replays(cuda):
     import torch
     import sushiblas_amd as sbx
