@@ -44,8 +44,8 @@ constexpr int kTallRows = 128, kTallTokens = 16;
 // 2 rows the next one alone, for want of registers).  The waves' sums are added up in LDS, in order.
 // Which wave has a term does not depend on m, so a row's bits do not either.
 //   One token is bound by memory: bf16 1 x 28672 x 8192 23.9 us (125 MB, 5.2 TB/s; the product of
-// MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 9.0-9.8 (36 MB: 2.6 of it are any kernel's, then the first
-// loads' way, and there is one round).  Four groups ahead in place of two are slower (11.4 for 10.7 before the
+// MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 8.2-9.8 (36 MB: 2.3 of it are any kernel's, and there is one
+// round).  Four groups ahead in place of two are slower (11.4 for 10.7 before the
 // groups' order changed).  More tokens are bound by X's way from the
 // L2s, as each workgroup reads all of it: 16 x 28672 x 8192 38 us, loads alone as long (64 rows of B a
 // workgroup take too many registers: 79).
