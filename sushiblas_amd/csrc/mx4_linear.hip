@@ -40,20 +40,19 @@ struct Turns {
 constexpr int kTallRows = 128, kTallTokens = 16;
 
 // A workgroup takes 16 XB rows of B and YB tiles of TOKENS rows of X, its waves a share each of the
-// terms, in groups of 256 by turns; AHEAD groups of B are under way, and of X (of a larger tile than
-// 2 rows the next one alone, for want of registers).  The waves' sums are added up in LDS, in order.
+// terms, in groups of 256 by turns; AHEAD groups are under way (2 with one tile of X alone).  The waves' sums
+// are added up in LDS, in order.
 // Which wave has a term does not depend on m, so a row's bits do not either.
 //   One token is bound by memory: bf16 1 x 28672 x 8192 23.9 us (125 MB, 5.2 TB/s; the product of
 // MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 8.2-9.8 (36 MB: 2.3 of it are any kernel's, and there is one
-// round).  Four groups ahead in place of two are slower (11.4 for 10.7 before the
-// groups' order changed).  More tokens are bound by X's way from the
+// round).  More tokens are bound by X's way from the
 // L2s, as each workgroup reads all of it: 16 x 28672 x 8192 38 us, loads alone as long (64 rows of B a
 // workgroup take too many registers: 79).
-template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
+template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES, int AHEAD>
 __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 {
     typedef typename std::conditional<MX8, Mx8Tokens<TOKENS>, DenseTokens<T, TOKENS>>::type tokens_t;
-    constexpr int PIECES = tokens_t::PIECES, FRAGMENTS = fragments_of(PIECES, TOKENS), PITCH = 16 * FRAGMENTS * YB + 4, AHEAD = 2, AHEAD_X = TOKENS == 2 ? AHEAD : 1;
+    constexpr int PIECES = tokens_t::PIECES, FRAGMENTS = fragments_of(PIECES, TOKENS), PITCH = 16 * FRAGMENTS * YB + 4;
     constexpr int OWN = rows4_bytes(XB) + tokens_bytes(PIECES, TOKENS), PART = 16 * PITCH * 4;
     __shared__ __align__(16) char lds[WAVES * (OWN > PART ? OWN : PART)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -79,7 +78,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 
     f32x4 acc[YB][FRAGMENTS][XB] = {};
     Rows4<XB> w[AHEAD];
-    typename tokens_t::Values a[AHEAD_X];
+    typename tokens_t::Values a[AHEAD];
     // (no branch around a load, and one past the last group reads zeros or the last group again: the
     // compiler would wait for all of them where paths meet)
     const Turns<WAVES> own_turns(p, wave, groups, x0 / (PIECES == 1 ? 32 : kTallRows));
@@ -89,12 +88,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
     for (int d = 0; d < AHEAD; ++d) {
         const int g = group(d);
         sw.load(w[d], g, nb - 8 * g);
-        if (d < AHEAD_X) sa[0].load(a[d], g, lane);
+        sa[0].load(a[d], g, lane);
     }
     for (int turn = 0; turn < turns;) {
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d) {
-            const int g = group(turn), next = group(turn + AHEAD), next_x = group(turn + AHEAD_X);
+            const int g = group(turn), next = group(turn + AHEAD);
             bf16x8 v[XB][8];
             if (nb - 8 * g < 8)
 #pragma unroll
@@ -103,8 +102,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
             sw.load(w[d], next, nb - 8 * next);
 #pragma unroll
             for (int j = 0; j < YB; ++j) {
-                sa[j].put(a[d % AHEAD_X], tokens_at, g, lane);
-                sa[j + 1 < YB ? j + 1 : 0].load(a[d % AHEAD_X], j + 1 < YB ? g : next_x, lane);
+                sa[j].put(a[d], tokens_at, g, lane);
+                sa[j + 1 < YB ? j + 1 : 0].load(a[d], j + 1 < YB ? g : next, lane);
                 multiply<PIECES, TOKENS>(acc[j], v, tokens_at, lane);
             }
             if (++turn == turns) break;
@@ -251,6 +250,22 @@ __global__ void __launch_bounds__(256) few_terms_kernel(Mx4LinearArgs p)
     *y = result<T>(sum, p.beta != 0.0f ? (float)*y : 0.0f, p);
 }
 
+template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
+void start(const Mx4LinearArgs& a, unsigned gy, hipStream_t s)
+{
+    const dim3 grid = grid_of((a.n + 16 * XB - 1) / (16 * XB), gy);
+    // One group of terms under way (1 x 12000 x 4096 bf16 7.3 us, with two 7.9; 16 x 12000 x 4096 of 8 bits 11.2 and
+    // 12.1; fp32 1 x 20000 x 6000 17.3 and 20.4, 8 x 8192 x 4096 10.3 and 11.1); of one token in one piece
+    // two where a wave has eight turns (2 x 8192 x 16384 16.1, with one 17.7; 1 x 28672 x 8192 24.1 and 24.7; but
+    // 1 x 16384 x 8192 15.3 and 14.7).  Three and four are slower.
+    if constexpr (TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1))
+        if (a.k > 7 * 256 * WAVES) {
+            linear_kernel<T, MX8, TOKENS, YB, XB, WAVES, 2><<<grid, 64 * WAVES, 0, s>>>(a);
+            return;
+        }
+    linear_kernel<T, MX8, TOKENS, YB, XB, WAVES, 1><<<grid, 64 * WAVES, 0, s>>>(a);
+}
+
 template <typename T, bool MX8, int TOKENS, int YB>
 hipError_t launch_form(const Mx4LinearArgs& a, hipStream_t s)
 {
@@ -258,13 +273,13 @@ hipError_t launch_form(const Mx4LinearArgs& a, hipStream_t s)
     if (a.n <= 16 * 256) {
         // one block of B's rows a workgroup, of which a CU has one: eight waves (1 x 4096 x 16384 9.8 us, by
         // four 12.2)
-        linear_kernel<T, MX8, TOKENS, YB, 1, 8><<<grid_of((a.n + 15) / 16, gy), 512, 0, s>>>(a);
+        start<T, MX8, TOKENS, YB, 1, 8>(a, gy, s);
     } else {
         // several workgroups to a CU, of four waves: one's loads go on while another adds up (1 x 28672
         // x 8192, groups in order, 26.5 us, by eight 28.9).  Two blocks each (16 x 28672 x 8192 38 us, one 45), but for one
         // token of one piece (28.7 against 26.5; 12000 x 4096 8.7 against 7.6)
         constexpr int XB = TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1) ? 1 : 2;
-        linear_kernel<T, MX8, TOKENS, YB, XB, 4><<<grid_of((a.n + 16 * XB - 1) / (16 * XB), gy), 256, 0, s>>>(a);
+        start<T, MX8, TOKENS, YB, XB, 4>(a, gy, s);
     }
     return hipGetLastError();
 }
