@@ -361,8 +361,11 @@ __device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKEN
 // after another, the next one on its way.  Tokens are read and laid out once for 128 rows.
 //   SPLIT true: the waves share the terms of the same rows, a group each by turns, and add up at the end.
 // Four times the workgroups, where the others would leave CUs idle.
+//   AHEAD: groups of rows under way.  One is enough where a CU has several workgroups (8 x 4096 x 2048, 4 of 32:
+// fp32 74 us, with two 85, fp16 70 and 72), but for the first product of tokens of one piece (16 x 2048 x 1024,
+// 8 of 64, bf16: 59.3, with two 57.6).
 constexpr int kTileWaves = 4;
-template <int PIECES, int TOKENS, bool SPLIT>
+template <int PIECES, int TOKENS, bool SPLIT, int AHEAD>
 struct TileProduct {
     static constexpr int STAGE = tokens_bytes(PIECES, TOKENS), STAGES = SPLIT ? kTileWaves : 2;
     static constexpr int BYTES = STAGES * STAGE + kTileWaves * rows4_bytes(2);
@@ -406,10 +409,10 @@ struct TileProduct {
                     *(u32x4*)(to + row * 512 + (lane % 32 ^ row % 16) * 16) = x[i][n];
                 }
         };
-        Rows4<1> w0[2], w1[2];
+        Rows4<1> w0[AHEAD], w1[AHEAD];
         load_tokens(first);
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
+        for (int d = 0; d < AHEAD; ++d) {
             const int g = first + d * STEP;
             s0.load(w0[d], g, nb - 8 * g);
             s1.load(w1[d], g, nb - 8 * g);
@@ -426,14 +429,14 @@ struct TileProduct {
             for (int d = 0; d < 2; ++d) {  // (not SPLIT: stage g % 2)
                 bf16x8 v[2][8];
                 if (nb - 8 * g < 8) {
-                    w0[d].code[0] = first_bytes(w0[d].code[0], nb - 8 * g);
-                    w1[d].code[0] = first_bytes(w1[d].code[0], nb - 8 * g);
+                    w0[d % AHEAD].code[0] = first_bytes(w0[d % AHEAD].code[0], nb - 8 * g);
+                    w1[d % AHEAD].code[0] = first_bytes(w1[d % AHEAD].code[0], nb - 8 * g);
                 }
-                const Rows4<2> both = {{w0[d].v[0], w0[d].v[1], w1[d].v[0], w1[d].v[1]}, {w0[d].code[0], w1[d].code[0]}};
+                const Rows4<2> both = {{w0[d % AHEAD].v[0], w0[d % AHEAD].v[1], w1[d % AHEAD].v[0], w1[d % AHEAD].v[1]}, {w0[d % AHEAD].code[0], w1[d % AHEAD].code[0]}};
                 fragments(both, own, lane, v);
-                const int next = g + 2 * STEP;
-                s0.load(w0[d], next, nb - 8 * next);
-                s1.load(w1[d], next, nb - 8 * next);
+                const int next = g + AHEAD * STEP;
+                s0.load(w0[d % AHEAD], next, nb - 8 * next);
+                s1.load(w1[d % AHEAD], next, nb - 8 * next);
                 if constexpr (SPLIT) {
                     put_tokens(stage);
                     load_tokens(g + STEP);
@@ -579,7 +582,7 @@ template <typename T, int TOKENS, bool SPLIT, bool FEW>
 __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kBf16Pieces<T>;
-    typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
+    typedef TileProduct<PIECES, TOKENS, SPLIT, PIECES == 1 ? 2 : 1> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ Tile<TOKENS> tile;
     __shared__ typename std::conditional<FEW, Shares, int>::type shares;
@@ -627,7 +630,7 @@ template <typename T, int TOKENS, bool SPLIT>
 __global__ void __launch_bounds__(64 * kTileWaves, SPLIT || sizeof(T) == 4 ? 1 : 3) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
     constexpr int PIECES = kActPieces<T>;
-    typedef TileProduct<PIECES, TOKENS, SPLIT> product_t;
+    typedef TileProduct<PIECES, TOKENS, SPLIT, 1> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ Tile<TOKENS> tile;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
