@@ -722,26 +722,20 @@ __global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork
             sa.move([&](int t) { return t > 0 ? kOutside : row; }, lane);
             sa.load(x, p.g);
         };
-        Rows4<1> rows[2];
+        Rows4<1> rows;
         Place now{from / groups, from % groups}, next = after(now);
-        load_rows(rows[0], now);
-        load_rows(rows[1], next);
+        load_rows(rows, now);
         load_tokens(now);
-        for (int u = from; u < to;) {
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const Place then = after(next);
-                bf16x8 v[1][8];
-                if (nb - 8 * now.g < 8) rows[d].code[0] = first_bytes(rows[d].code[0], nb - 8 * now.g);
-                fragments(rows[d], own, lane, v);
-                load_rows(rows[d], then);
-                sa.put(x, tokens_at, lane);
-                load_tokens(next);
-                multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
-                now = next;
-                next = then;
-                if (++u == to) break;
-            }
+        for (int u = from; u < to; ++u) {
+            bf16x8 v[1][8];
+            if (nb - 8 * now.g < 8) rows.code[0] = first_bytes(rows.code[0], nb - 8 * now.g);
+            fragments(rows, own, lane, v);
+            load_rows(rows, next);
+            sa.put(x, tokens_at, lane);
+            load_tokens(next);
+            multiply<PIECES, TOKENS>(acc, v, tokens_at, lane);
+            now = next;
+            next = after(next);
         }
     }
     // pieces are in columns 0, 2 and 4
