@@ -172,15 +172,10 @@ __global__ void __launch_bounds__(512, 2) linear_tall_kernel(Mx4LinearArgs p)
     constexpr int SUMS = 4 / SETS;  // of groups 4 i + SETS u + set
     const Turns<4> mine[SUMS] = {{p, set, groups, x0 / kTallRows}, {p, set + SETS, groups, x0 / kTallRows}};
     f32x4 acc[SUMS][FRAGMENTS][2] = {};
-    Rows4<2> w[SUMS];
+    Rows4<2> w;
     typename tokens_t::Values a;
-    auto load_rows = [&](int u, int turn) {
-        const int g = mine[u].group(turn);
-        sw.load(w[u], g, nb - 8 * g);
-    };
     sa.load(a, mine[0].group(0), lane);
-#pragma unroll
-    for (int u = 0; u < SUMS; ++u) load_rows(u, 0);
+    sw.load(w, mine[0].group(0), nb - 8 * mine[0].group(0));
     sa.template put<TOKENS>(a, stage, mine[0].group(0), lane, PER * wave);
     sa.load(a, mine[1].group(0), lane);
     lds_barrier();
@@ -192,9 +187,9 @@ __global__ void __launch_bounds__(512, 2) linear_tall_kernel(Mx4LinearArgs p)
             bf16x8 v[2][8];
             if (nb - 8 * g < 8)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) w[u].code[i] = first_bytes(w[u].code[i], nb - 8 * g);
-            fragments(w[u], own, lane, v);
-            load_rows(u, turn + 1);
+                for (int i = 0; i < 2; ++i) w.code[i] = first_bytes(w.code[i], nb - 8 * g);
+            fragments(w, own, lane, v);
+            sw.load(w, then, nb - 8 * then);
             sa.template put<TOKENS>(a, stage + (1 - u) * STAGE, then, lane, PER * wave);  // its last readers passed the barrier before
             sa.load(a, mine[u].group(turn + 1), lane);
             multiply<PIECES, TOKENS>(acc[u], v, stage + u * STAGE, lane);
