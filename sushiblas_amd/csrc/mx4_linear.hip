@@ -292,8 +292,8 @@ hipError_t launch(const Mx4LinearArgs& a, hipStream_t s)
     if (a.m <= 2) return launch_form<T, MX8, 2, 1>(a, s);
     if constexpr (SPLIT) {
         if (a.m <= 8) return launch_form<T, MX8, 8, 1>(a, s);
-        // Past one round of those workgroups (two to a CU; one of fp16's two tiles) the other kernel, which has a
-        // round of its own less: fp16 16 x 17000 x 8192 32.6 us against 39.7, but 16 x 12000 x 8192 32.0 against 27.5;
+        // Past one round of those workgroups (two to a CU; one of fp16's two tiles) the other kernel, which takes four
+        // times the rows of B a workgroup: fp16 16 x 17000 x 8192 32.6 us against 39.7, but 16 x 12000 x 8192 32.0 against 27.5;
         // fp32 17 x 8192 x 8192 38.5 against 34.9, but 20 x 9000 x 8192 39.1 against 52.8.
         const bool two = sizeof(T) == 2 && a.m > 16;
         const int64_t others = (int64_t)((a.n + 31) / 32) * ((a.m + (two ? 31 : 15)) / (two ? 32 : 16));
