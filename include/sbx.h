@@ -354,9 +354,8 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  * W1, S1: an MXFP4 matrix of experts * 2 * hidden rows over width, expert e's G at rows
  * e * 2 * hidden, its U hidden rows later.  W2, S2: of experts * width rows over hidden.
  * Activations are not rounded before W1's product (but for bits of fp32 values below 2^-133);
- * before W2's they are held as the sum of two bf16 values (F32: three), 16 bits (24) where
- * dtype has 8 or 11.  Sums are held in
- * 32 bits and rounded to dtype once.
+ * before W2's they are held as the sum of three bf16 values, 24 bits.  Sums are held in 32 bits and
+ * rounded to dtype once.
  * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.  Y may be X
  * (same leading dimension).
  * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^18, ld1, ld2 < 2^23 -

@@ -23,9 +23,10 @@ namespace {
 
 // ---- the router ----
 
-// Pieces that an activation is held in before the second product: of fp32 all of its bits, else 16.
-template <typename T>
-constexpr int kActPieces = sizeof(T) == 4 ? 3 : 2;
+// Pieces that an activation is held in before the second product: the 24 bits of 32, of every type.  Two
+// (16 bits) take less of the second product (64 x 4096 x 2048, 4 of 32, bf16 106 us against 111, 8 tokens 70.6
+// and 73.0, one token alike), but where an expert's terms cancel what is left has none of a result's own bits.
+constexpr int kActPieces = 3;
 
 // x in the wave's lower half and y in its upper one, each added to its own other half.
 __device__ inline double halves(double x, double y)
@@ -235,13 +236,13 @@ __global__ void __launch_bounds__(256) choose_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 // ---- the experts ----
 
 // The hidden layer's values, times their shares, as pieces.
-template <typename T, int N>
+template <int N>
 __device__ inline void store_act(const Mx4MoeArgs& a, const Mx4MoeWork& w, int choice, int unit, const float (&h)[8])
 {
-    bf16x8 to[kActPieces<T>];
+    bf16x8 to[kActPieces];
     split(h, to);
 #pragma unroll
-    for (int n = 0; n < kActPieces<T>; ++n) {
+    for (int n = 0; n < kActPieces; ++n) {
         uint8_t* at = a.work + w.act + n * w.act_stride + (size_t)choice * w.act_ld + 2 * unit;
         const u32x4 v = __builtin_bit_cast(u32x4, to[n]);
         if constexpr (N == 8)
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(512, 4) up_one_kernel(Mx4MoeArgs a, Mx4MoeWork
     float all[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) all[i] = __shfl(h, (int)(threadIdx.x * 8 + i) % 16);
-    if (threadIdx.x < 2) store_act<T, 8>(a, w, choice, j0 + 8 * threadIdx.x, all);
+    if (threadIdx.x < 2) store_act<8>(a, w, choice, j0 + 8 * threadIdx.x, all);
 }
 
 // A wave's sums of a tile (PIECES of a token in as many columns), of tokens lane % TOKENS.
@@ -621,15 +622,14 @@ __global__ void __launch_bounds__(64 * kTileWaves) up_kernel(Mx4MoeArgs a, Mx4Mo
     float h[8] = {};
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = 4 * q + e < rows ? act_of(gate[e], up[e], share) : 0.0f;
-    store_act<T, 4>(a, w, choice, j0 + 4 * q, h);
+    store_act<4>(a, w, choice, j0 + 4 * q, h);
 }
 
-// 32 results a wave (SPLIT: a workgroup), of each choice apart.  Three workgroups to a CU of 16-bit types
-// (64 x 4096 x 2048, 4 of 32: 106 us against 108 by two; fp32 would spill, 139 against 129).
+// 32 results a wave (SPLIT: a workgroup), of each choice apart.
 template <typename T, int TOKENS, bool SPLIT>
-__global__ void __launch_bounds__(64 * kTileWaves, SPLIT || sizeof(T) == 4 ? 1 : 3) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
+__global__ void __launch_bounds__(64 * kTileWaves) down_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
-    constexpr int PIECES = kActPieces<T>;
+    constexpr int PIECES = kActPieces;
     typedef TileProduct<PIECES, TOKENS, SPLIT, 1> product_t;
     __shared__ __align__(16) char lds[product_t::BYTES];
     __shared__ Tile<TOKENS> tile;
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Mx4MoeArgs a, Mx4MoeWork w
 template <typename T>
 __global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork w)
 {
-    constexpr int WAVES = 16, TOKENS = 2, PIECES = kActPieces<T>, OWN = rows4_bytes(1) + tokens_bytes(PIECES, TOKENS);
+    constexpr int WAVES = 16, TOKENS = 2, PIECES = kActPieces, OWN = rows4_bytes(1) + tokens_bytes(PIECES, TOKENS);
     __shared__ __align__(16) char lds[WAVES * OWN];
     __shared__ float part[WAVES][16];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
