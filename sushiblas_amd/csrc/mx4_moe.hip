@@ -251,7 +251,14 @@ __device__ inline void store_act(const Mx4MoeArgs& a, const Mx4MoeWork& w, int c
             *(u32x2*)at = u32x2{v[0], v[1]};
     }
 }
-__device__ inline float act_of(float gate, float up, float share) { return share * (gate / (1.0f + expf(-gate)) * up); }
+// share * silu(gate) * up.  exp(-gate) passes 32 bits from -88.7 on, where silu times a large up is still an
+// ordinary number: so by e = exp(-|gate| / 2), of which negative gates take 1 / (1 + 1 / e^2) = e e / (1 + e^2),
+// one e before up and one after.
+__device__ inline float act_of(float gate, float up, float share)
+{
+    const float e = expf(-0.5f * fabsf(gate)), by = gate < 0.0f ? e : 1.0f;
+    return share * (gate * by / (1.0f + e * e) * up * by);
+}
 
 // The only token's: 16 units of the expert that is its choice blockIdx.y, by eight waves that share the terms.
 //   Two workgroups to a CU, for which the registers of a second group of terms ahead are too many: 2048

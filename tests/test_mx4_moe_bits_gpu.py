@@ -64,3 +64,41 @@ def test_activations_keep_32_bits(cuda, name, tokens, width, hidden, experts, to
             off[t] += np.abs(m.w2[order[t, j]]) @ np.abs(a) * (2.0 ** -20 + 2.0 ** -22 + (hidden + topk + 4) * 2.0 ** -24)
     got = ref.f64(Y)
     assert (np.abs(got - y) <= off + ref.HALF[name] * (np.abs(y) + off) + ref.TINY[name]).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 6, 70])
+def test_silu_of_far_gates(cuda, name, tokens):
+    """Gates from -160 to 90 with ups of 2^100: silu is of use as long as 32 bits hold its product with them,
+    which is below exp(-88), where exp(-gate) passes their range."""
+    import torch
+    width, hidden = 16, 260
+    m = Mixture(cuda, name, width, hidden, 2)
+    n1, c1 = np.zeros((2, 2 * hidden, 1, 32), np.uint8), np.full((2, 2 * hidden, 1), 127, np.uint8)
+    n1[:, np.arange(hidden), 0, np.arange(hidden) % 8] = 2  # the gates: x of one of the first 8 columns
+    n1[:, hidden:, 0, 8] = 2
+    c1[:, hidden:] = 227
+    n2, c2 = np.zeros((2, width, 9, 32), np.uint8), np.full((2, width, 9), 127, np.uint8)
+    n2[:, np.arange(width), 0, np.arange(width)] = 2  # a result: one unit of the hidden layer
+    n1, c1, n2, c2 = n1.reshape(-1, 1, 32), c1.reshape(-1, 1), n2.reshape(-1, 9, 32), c2.reshape(-1, 9)
+    m.w1 = mx4.values(n1, c1, width).reshape(2, 2 * hidden, width)
+    m.w2 = mx4.values(n2, c2, hidden).reshape(2, width, hidden)
+    m.W1, m.S1 = ref.packed(cuda, n1, c1)
+    m.W2, m.S2 = ref.packed(cuda, n2, c2)
+    x = np.zeros((tokens, width))
+    x[:, :8] = -np.array([160, 130, 104, 100, 95, 90, 86, -90]) + np.arange(tokens)[:, None] % 4
+    x[:, 8] = 1.0
+    X = ref.padded(cuda, x, m.dt, 0)
+    x = ref.f64(X)
+    Y = torch.zeros((tokens, width), dtype=m.dt, device=cuda)
+    m.call(X, Y, 1, True)
+    torch.cuda.synchronize()
+    order, _, _ = ref.route(x, m.wr, 1, True)
+    want = np.empty((tokens, width))
+    for t in range(tokens):
+        z = m.w1[order[t, 0]] @ x[t]
+        want[t] = m.w2[order[t, 0]] @ (z[:hidden] / (1 + np.exp(-z[:hidden])) * z[hidden:])
+    # as above, one term a sum; pieces are of bf16, which ends at 2^-133
+    off = np.abs(want) * (2.0 ** -20 + 2.0 ** -22 + 2.0 ** -23) + 2.0 ** -133
+    got = ref.f64(Y)
+    assert (np.abs(got - want) <= off + ref.HALF[name] * (np.abs(want) + off) + ref.TINY[name]).all()
