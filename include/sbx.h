@@ -329,15 +329,18 @@ int sbx_rms_norm_grad(void* stream, int dtype, int64_t rows, int64_t cols, const
 size_t sbx_rms_norm_grad_workspace(int64_t rows, int64_t cols);
 
 /* The values an MXFP8 matrix (P, S as above) stands for, rounded to dtype
- * (F32: exact). */
+ * (F32: exact, below 2^128). */
 int sbx_mx8_dequantize(void* stream, int dtype, int64_t rows, int64_t cols, const void* P,
                        int64_t ldp, const void* S, int64_t lds, void* Y, int64_t ldy);
 
 /* Y = epilogue(alpha * X * B^T + beta * Y) for a few rows: X (m x k) keeps its type
  * (SX NULL) or is an MXFP8 matrix (X, SX), B (n x k) is an MXFP4 matrix, Y (m x n) of
- * dtype.  X is not rounded (but for bits of fp32 values below 2^-133, which do not
- * count); sums are held in 32 bits and rounded to dtype once.  What lies past the
- * k-th term is not used; Y lies apart from X and B.  BLAS semantics as for GEMM (beta == 0: Y is
+ * dtype.  X is not rounded (but for bits of fp32 and MXFP8 values below 2^-133, which do not
+ * count); sums are held in 32 bits and rounded to dtype once.  A value of 2^128 or more, which 32
+ * bits do not hold either (MXFP4's of 4 and 6 under code 253 and of 2 and more under 254, MXFP8's under
+ * codes from 247 on; no quantiser here writes one), is an infinity: results that it is a term of are
+ * infinite or NaN, and those of a row of B that has it past the k-th term, in the same block, may be
+ * NaN.  What else lies past the k-th term is not used; Y lies apart from X and B.  BLAS semantics as for GEMM (beta == 0: Y is
  * not read; alpha == 0 or k == 0: X and B are not).  Rows are computed apart: those of
  * one call have the bits that they have alone.  m <= 1024, n <= 2^30, k <= 2^23, ldb <
  * 2^23 - 15, a row of X (ldx) at most 2^26 bytes (else SBX_UNSUPPORTED). */
@@ -353,6 +356,7 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  *   y = sum_j p_j * W2_e (silu(G_e x) * (U_e x)),  silu(z) = z / (1 + exp(-z)),  e the j-th expert
  * W1, S1: an MXFP4 matrix of experts * 2 * hidden rows over width, expert e's G at rows
  * e * 2 * hidden, its U hidden rows later.  W2, S2: of experts * width rows over hidden.
+ * For W1 and W2 sbx_mx4_linear's words about values past 32 bits hold.
  * Activations are not rounded before W1's product (but for bits of fp32 values below 2^-133);
  * before W2's they are held as the sum of three bf16 values, 24 bits.  Sums are held in 32 bits and
  * rounded to dtype once.

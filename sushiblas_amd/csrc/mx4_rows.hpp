@@ -1,11 +1,15 @@
 // mx4_rows.hpp -- products of rows of an MXFP4 matrix with a few tokens whose values keep their
 // type or are MXFP8, a group of 256 terms at a time, by single waves.
 //
-// Both operands go to the bf16 matrix cores.  An MXFP4 or MXFP8 value is a bf16 one, its block's
-// code included, whatever the code (elements have 2 and 4 bits, and bf16 fp32's exponents); dense
+// Both operands go to the bf16 matrix cores.  An MXFP4 value is a bf16 one, its block's code included
+// (elements have 2 bits, and bf16 fp32's exponents), and so is an MXFP8 one (4 bits); dense
 // values are exact sums of bf16 pieces: bf16 as they are, fp16 as 2 (8 and 3 bits), fp32 as 3 (8
-// each).  So products are exact (down to 2^-133 where bf16 ends), and sums are held in fp32.  The
-// scaled 4- and 8-bit instruction would take an eighth of the time, but it aligns the 128 terms of
+// each).  So products are exact, and sums are held in fp32.  Two ends are bf16's: what of an MXFP8 value or a
+// piece lies below 2^-133 is rounded to it (codes 0 to 2, whose least bits are 2^-136), and a value of 2^128
+// or more, MXFP4's under codes 253 and 254 and MXFP8's from 247 on, is an infinity, behind the last term
+// too, where X's zeros make it NaN; neither quantiser writes one.  (To clear such elements there took 2-3 % of
+// the small calls: moe 1 x 2048 x 1024, 8 of 64, 16.4 -> 16.9 us in a graph, though no group of it is ragged.)
+//   The scaled 4- and 8-bit instruction would take an eighth of the time, but it aligns the 128 terms of
 // a product to their largest, and drops what lies some 2^-14 below: blocks with small scales beside
 // one with a large one (1000 terms with codes 2^50 apart: off by 5e-5 of the result).
 //
