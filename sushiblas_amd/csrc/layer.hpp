@@ -66,9 +66,6 @@ struct Mx4MoeArgs {
     uint8_t* work;
 };
 
-// A mixture is computed for 64 tokens at a time (kernels' z): tokens of other chunks share no tile.
-constexpr int kMoeChunk = 64;
-
 // A mixture's workspace: offsets of its parts, each 256-byte aligned.
 struct Mx4MoeWork {
     size_t logits;           // tokens x experts, 64 bits

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "layer.hpp"
+#include "layer_plan.hpp"
 #include "mx4_rows.hpp"
 
 namespace sbx {
@@ -245,68 +246,52 @@ __global__ void __launch_bounds__(256) few_terms_kernel(Mx4LinearArgs p)
     *y = result<T>(sum, p.beta != 0.0f ? (float)*y : 0.0f, p);
 }
 
-template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES>
-void start(const Mx4LinearArgs& a, unsigned gy, hipStream_t s)
+template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES, int AHEAD>
+void start(const Mx4LinearArgs& a, hipStream_t s)
 {
-    const dim3 grid = grid_of((a.n + 16 * XB - 1) / (16 * XB), gy);
-    // One group of terms under way (1 x 12000 x 4096 bf16 7.3 us, with two 7.9; 16 x 12000 x 4096 of 8 bits 11.2 and
-    // 12.1; fp32 1 x 20000 x 6000 17.3 and 20.4, 8 x 8192 x 4096 10.3 and 11.1); of one token in one piece
-    // two where a wave has eight turns (2 x 8192 x 16384 16.1, with one 17.7; 1 x 28672 x 8192 24.1 and 24.7; but
-    // 1 x 16384 x 8192 15.3 and 14.7).  Three and four are slower.
-    if constexpr (TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1))
-        if (a.k > 7 * 256 * WAVES) {
-            linear_kernel<T, MX8, TOKENS, YB, XB, WAVES, 2><<<grid, 64 * WAVES, 0, s>>>(a);
-            return;
-        }
-    linear_kernel<T, MX8, TOKENS, YB, XB, WAVES, 1><<<grid, 64 * WAVES, 0, s>>>(a);
+    const unsigned gy = (unsigned)((a.m + TOKENS * YB - 1) / (TOKENS * YB));
+    linear_kernel<T, MX8, TOKENS, YB, XB, WAVES, AHEAD>
+        <<<grid_of((a.n + 16 * XB - 1) / (16 * XB), gy), 64 * WAVES, 0, s>>>(a);
 }
 
 template <typename T, bool MX8, int TOKENS, int YB>
-hipError_t launch_form(const Mx4LinearArgs& a, hipStream_t s)
+void launch_rows(const Mx4LinearPlan& p, const Mx4LinearArgs& a, hipStream_t s)
 {
-    const unsigned gy = (unsigned)((a.m + TOKENS * YB - 1) / (TOKENS * YB));
-    if (a.n <= 16 * 256) {
-        // one block of B's rows a workgroup, of which a CU has one: eight waves (1 x 4096 x 16384 9.8 us, by
-        // four 12.2)
-        start<T, MX8, TOKENS, YB, 1, 8>(a, gy, s);
+    if constexpr (TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1)) {
+        if (p.ahead == 2)
+            p.waves == 8 ? start<T, MX8, 2, YB, 1, 8, 2>(a, s) : start<T, MX8, 2, YB, 1, 4, 2>(a, s);
+        else
+            p.waves == 8 ? start<T, MX8, 2, YB, 1, 8, 1>(a, s) : start<T, MX8, 2, YB, 1, 4, 1>(a, s);
     } else {
-        // several workgroups to a CU, of four waves: one's loads go on while another adds up (1 x 28672
-        // x 8192, groups in order, 26.5 us, by eight 28.9).  Two blocks each (16 x 28672 x 8192 38 us, one 45), but for one
-        // token of one piece (28.7 against 26.5; 12000 x 4096 8.7 against 7.6)
-        constexpr int XB = TOKENS == 2 && (MX8 || kBf16Pieces<T> == 1) ? 1 : 2;
-        start<T, MX8, TOKENS, YB, XB, 4>(a, gy, s);
+        p.waves == 8 ? start<T, MX8, TOKENS, YB, 1, 8, 1>(a, s) : start<T, MX8, TOKENS, YB, 2, 4, 1>(a, s);
     }
-    return hipGetLastError();
 }
 
 template <typename T, bool MX8>
 hipError_t launch(const Mx4LinearArgs& a, hipStream_t s)
 {
-    if (a.k == 0 || (!MX8 && a.k < 8)) {
+    constexpr int PIECES = MX8 ? 1 : kBf16Pieces<T>;
+    const Mx4LinearPlan p = mx4_linear_plan(PIECES, MX8, a.m, a.n, a.k);
+    if (p.form == Mx4LinearPlan::FewTerms) {
         few_terms_kernel<T><<<grid_of((a.n + 255) / 256, (unsigned)a.m), 256, 0, s>>>(a);
-        return hipGetLastError();
-    }
-    // Up to two tiles a workgroup; more rows of X read B again (four would take too many registers: 64 x
-    // 8192 x 8192 bf16 27.9 us against 24.9).
-    constexpr bool SPLIT = !MX8 && kBf16Pieces<T> > 1;
-    if (a.m <= 2) return launch_form<T, MX8, 2, 1>(a, s);
-    if constexpr (SPLIT) {
-        if (a.m <= 8) return launch_form<T, MX8, 8, 1>(a, s);
-        // Past one round of those workgroups (two to a CU; one of fp16's two tiles) the other kernel, which takes four
-        // times the rows of B a workgroup: fp16 16 x 17000 x 8192 32.6 us against 39.7, but 16 x 12000 x 8192 32.0 against 27.5;
-        // fp32 17 x 8192 x 8192 38.5 against 34.9, but 20 x 9000 x 8192 39.1 against 52.8.
-        const bool two = sizeof(T) == 2 && a.m > 16;
-        const int64_t others = (int64_t)((a.n + 31) / 32) * ((a.m + (two ? 31 : 15)) / (two ? 32 : 16));
-        if (a.n > 16 * 256 && others > (two ? 256 : 512)) {
+    } else if (p.form == Mx4LinearPlan::Tall) {
+        if constexpr (PIECES > 1)
             linear_tall_kernel<T><<<grid_of((a.n + kTallRows - 1) / kTallRows,
                                             (unsigned)((a.m + kTallTokens - 1) / kTallTokens)), 512, 0, s>>>(a);
-            return hipGetLastError();
+    } else if (p.tokens == 2) {
+        launch_rows<T, MX8, 2, 1>(p, a, s);
+    } else if (p.tokens == 8) {
+        if constexpr (PIECES > 1) {
+            if (p.tiles == 1) {
+                launch_rows<T, MX8, 8, 1>(p, a, s);
+            } else if constexpr (PIECES == 3) {
+                launch_rows<T, MX8, 8, 2>(p, a, s);
+            }
         }
+    } else if constexpr (PIECES < 3) {
+        p.tiles == 1 ? launch_rows<T, MX8, 16, 1>(p, a, s) : launch_rows<T, MX8, 16, 2>(p, a, s);
     }
-    if constexpr (SPLIT && sizeof(T) == 4)  // (three pieces of 16 tokens would not fit the LDS)
-        return launch_form<T, MX8, 8, 2>(a, s);
-    else
-        return a.m <= 16 ? launch_form<T, MX8, 16, 1>(a, s) : launch_form<T, MX8, 16, 2>(a, s);
+    return hipGetLastError();
 }
 
 }  // namespace

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "layer.hpp"
+#include "layer_plan.hpp"
 #include "mx4_rows.hpp"
 
 namespace sbx {
@@ -372,7 +373,6 @@ __device__ inline f32x4 token_sums(const f32x4 (&acc)[fragments_of(PIECES, TOKEN
 //   AHEAD: groups of rows under way.  One is enough where a CU has several workgroups (8 x 4096 x 2048, 4 of 32:
 // fp32 74 us, with two 85, fp16 70 and 72), but for the first product of tokens of one piece (16 x 2048 x 1024,
 // 8 of 64, bf16: 59.3, with two 57.6).
-constexpr int kTileWaves = 4;
 template <int PIECES, int TOKENS, bool SPLIT, int AHEAD>
 struct TileProduct {
     static constexpr int STAGE = tokens_bytes(PIECES, TOKENS), STAGES = SPLIT ? kTileWaves : 2;
@@ -555,8 +555,6 @@ struct Tile {
     }
 };
 
-// Up to so many tokens and experts the first product's workgroups choose, too: 1 us where a launch costs 4.
-constexpr int kFewTokens = 8, kFewExperts = 64;
 struct Shares {
     float of[kFewTokens * 16];
 };
@@ -765,38 +763,27 @@ __global__ void __launch_bounds__(1024) down_one_kernel(Mx4MoeArgs a, Mx4MoeWork
 
 // The products of more than one token, in tiles of UP and DOWN; FEW: that choose in the first one.
 template <typename T, int UP, int DOWN, bool FEW>
-void launch_tiles(const Mx4MoeArgs& a, const Mx4MoeWork& w, hipStream_t s)
+void launch_tiles(const Mx4MoePlan& p, const Mx4MoeArgs& a, const Mx4MoeWork& w, hipStream_t s)
 {
-    const unsigned chunks = (unsigned)((a.tokens + kMoeChunk - 1) / kMoeChunk);
     if constexpr (!FEW) {
-        if (a.experts <= 64)
-            choose_kernel<1><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
-        else if (a.experts <= 128)
-            choose_kernel<2><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
+        const unsigned waves = (unsigned)((a.tokens + 3) / 4);
+        if (p.each == 1)
+            choose_kernel<1><<<waves, 256, 0, s>>>(a, w);
+        else if (p.each == 2)
+            choose_kernel<2><<<waves, 256, 0, s>>>(a, w);
         else
-            choose_kernel<8><<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a, w);
+            choose_kernel<8><<<waves, 256, 0, s>>>(a, w);
     }
-    const int choices = (a.tokens < kMoeChunk ? a.tokens : kMoeChunk) * a.topk;
-    auto most = [&](int size) {  // tiles
-        return (unsigned)(a.experts + choices / size < choices ? a.experts + choices / size : choices);
-    };
-    // Rows for each wave from so many workgroups on: fp32 4 x 1024 x 2048, 2 of 8 (64 and 256 workgroups a
-    // product) 28.0 us with both forms, 31.8 with rows for each wave, 31.4 with shared ones; bf16 2 x 4096
-    // x 2048, 4 of 32 (256 both) 46 and 52.
-    constexpr int64_t ENOUGH = 200;
     const unsigned up_x = (unsigned)(w.act_ld / 32);  // 16 units each, to the end of a row of the workspace
-    const unsigned up_t = most(UP), down_t = most(DOWN), down_x = (unsigned)((a.width + 31) / 32),
-                   down_w = (down_x + kTileWaves - 1) / kTileWaves;
-    const bool rows = (int64_t)(up_x / kTileWaves) * up_t * chunks >= ENOUGH;
-    const dim3 up(rows ? up_x / kTileWaves : up_x, up_t, chunks);
-    if (rows)
-        up_kernel<T, UP, false, FEW><<<up, 64 * kTileWaves, 0, s>>>(a, w);
+    const unsigned down_x = (unsigned)((a.width + 31) / 32), down_w = (down_x + kTileWaves - 1) / kTileWaves;
+    if (p.up_rows)
+        up_kernel<T, UP, false, FEW><<<dim3(up_x / kTileWaves, p.up_tiles, p.chunks), 64 * kTileWaves, 0, s>>>(a, w);
     else
-        up_kernel<T, UP, true, FEW><<<up, 64 * kTileWaves, 0, s>>>(a, w);
-    if ((int64_t)down_w * down_t * chunks >= ENOUGH)
-        down_kernel<T, DOWN, false><<<dim3(down_w, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        up_kernel<T, UP, true, FEW><<<dim3(up_x, p.up_tiles, p.chunks), 64 * kTileWaves, 0, s>>>(a, w);
+    if (p.down_rows)
+        down_kernel<T, DOWN, false><<<dim3(down_w, p.down_tiles, p.chunks), 64 * kTileWaves, 0, s>>>(a, w);
     else
-        down_kernel<T, DOWN, true><<<dim3(down_x, down_t, chunks), 64 * kTileWaves, 0, s>>>(a, w);
+        down_kernel<T, DOWN, true><<<dim3(down_x, p.down_tiles, p.chunks), 64 * kTileWaves, 0, s>>>(a, w);
     combine_kernel<T><<<dim3((unsigned)((a.width + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a, w);
 }
 
@@ -804,14 +791,15 @@ template <typename T>
 hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
 {
     const Mx4MoeWork w = mx4_moe_work(a.tokens, a.width, a.hidden, a.experts, a.topk);
+    const Mx4MoePlan p = mx4_moe_plan(kBf16Pieces<T>, a.tokens, a.width, a.hidden, a.experts, a.topk);
     const int expert_groups = (a.experts + 3) / 4, pieces = (w.x_ld / 16 * a.tokens + 255) / 256;
     const unsigned prepare_x = (unsigned)(expert_groups + pieces);
-    if (a.tokens == 1) {
+    if (p.one) {
         prepare_kernel<T, 1><<<prepare_x, 256, 0, s>>>(a, w, expert_groups);
         const dim3 up((unsigned)(w.act_ld / 32), (unsigned)a.topk);
-        if (a.experts <= 64)
+        if (p.each == 1)
             up_one_kernel<T, 1><<<up, 512, 0, s>>>(a, w);
-        else if (a.experts <= 128)
+        else if (p.each == 2)
             up_one_kernel<T, 2><<<up, 512, 0, s>>>(a, w);
         else
             up_one_kernel<T, 8><<<up, 512, 0, s>>>(a, w);
@@ -819,15 +807,12 @@ hipError_t launch(const Mx4MoeArgs& a, hipStream_t s)
     } else {
         prepare_kernel<T, 4><<<dim3(prepare_x, (unsigned)((a.tokens + 3) / 4)), 256, 0, s>>>(a, w, expert_groups);
         constexpr int UP = kBf16Pieces<T> == 1 ? 16 : 8;
-        const int chunk = a.tokens < kMoeChunk ? a.tokens : kMoeChunk;
-        if (a.tokens <= kFewTokens && a.experts <= kFewExperts)
-            launch_tiles<T, UP, 8, true>(a, w, s);
-        // tiles of 16 where experts have more than 6 tokens on average, as most would need two of 8 (64 x 4096
-        // x 2048, 4 of 32, fp16 117 against 126 us, fp32 145 against 150; 8 tokens of it 78 against 73)
-        else if (chunk * a.topk > 6 * a.experts)
-            launch_tiles<T, 16, 16, false>(a, w, s);
+        if (p.few)
+            launch_tiles<T, UP, 8, true>(p, a, w, s);
+        else if (p.down == 16)
+            launch_tiles<T, 16, 16, false>(p, a, w, s);
         else
-            launch_tiles<T, UP, 8, false>(a, w, s);
+            launch_tiles<T, UP, 8, false>(p, a, w, s);
     }
     return hipGetLastError();
 }
