@@ -1,0 +1,39 @@
+"""GPU tests of the mixture's forms, as layer_sizes.py lists them (and test_layer_plan.py checks):
+several groups of terms where waves have rows of their own, and choices among more experts than a wave
+has lanes."""
+import numpy as np
+import pytest
+
+import layer_reference as ref
+import layer_sizes as sizes
+from test_mx4_moe_gpu import Mixture, _x
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("name", ref.TYPES)
+@pytest.mark.parametrize("tokens,width,hidden,experts,topk", sizes.ROWS)
+def test_mixtures_of_several_groups(cuda, name, tokens, width, hidden, experts, topk):
+    Mixture(cuda, name, width, hidden, experts).check(_x(tokens, width), topk)
+
+
+@pytest.mark.parametrize("name", ref.TYPES)
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("tokens,experts,topk", sizes.CHOICES)
+def test_choices(cuda, name, normalize, tokens, experts, topk):
+    Mixture(cuda, name, 80, 48, experts).check(_x(tokens, 80), topk, normalize)
+
+
+@pytest.mark.parametrize("name", ref.TYPES)
+@pytest.mark.parametrize("experts", [68, 128, 131, 300])
+@pytest.mark.parametrize("tokens", [1, 5, 9])
+def test_equal_logits_of_far_experts_go_by_index(cuda, name, experts, tokens):
+    """Equal ones among a lane's own and other lanes', as the highest of all; and all equal."""
+    same = [e for e in (3, 67, 130, 195, 299) if e < experts] + [9, 40]
+    m = Mixture(cuda, name, 96, 32, experts, same=same)
+    x = 3.0 * m.wr[same[0]] * (1 + np.arange(tokens))[:, None]  # whose logits are the highest for experts like it
+    order = ref.route(ref.rounded_to(x, m.dt), m.wr, len(same), True)[0]
+    assert (order == np.sort(same)).all()
+    m.check(x, len(same))
+    m.check(x, 2, False)
+    m.check(np.zeros((tokens, 96)), 12)
