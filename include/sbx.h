@@ -363,7 +363,7 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.  Y may be X
  * (same leading dimension).
  * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^18, ld1, ld2 < 2^23 -
- * 15, a row of X (ldx) less than 2^23 - 15 bytes (else SBX_UNSUPPORTED). */
+ * 15, of several tokens a row of X (ldx) less than 2^23 - 15 bytes (else SBX_UNSUPPORTED). */
 int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t hidden,
                 int64_t experts, int64_t topk, const void* X, int64_t ldx, const void* WR,
                 int64_t ldwr, int normalize, const void* W1, int64_t ld1, const void* S1,

@@ -19,7 +19,7 @@ constexpr int64_t kMaxRowBytes = ((int64_t)1 << 23) - 16;
 // what a mixture of experts takes: few tokens, and choices that fit its kernels' tables
 // (the rows of all experts together are within kMaxSide then)
 constexpr int64_t kMaxTokens = 256, kMaxExperts = 512, kMaxTopk = 16, kMaxLayer = (int64_t)1 << 18;
-constexpr int64_t kMaxMoeTokenBytes = ((int64_t)1 << 23) - 16;  // of a row of X: 256 rows stay within 32-bit offsets
+constexpr int64_t kMaxMoeTokenBytes = ((int64_t)1 << 23) - 16;  // of a row of X, if there are several (the weights' bound; the kernels' offsets there have 64 bits)
 constexpr int64_t kMaxLinearRows = 1024;
 constexpr int64_t kMaxTokenBytes = (int64_t)1 << 26;  // of a row of X: 16 rows stay within 32-bit offsets
 
@@ -313,7 +313,8 @@ int sbx_mx4_moe(void* stream, int dtype, int64_t tokens, int64_t width, int64_t 
     if ((uintptr_t)chosen % 4 || (uintptr_t)weights % 4 || !workspace || (uintptr_t)workspace % 16 ||
         workspace_bytes < sbx_mx4_moe_workspace(tokens, width, hidden, experts, topk))
         return SBX_INVALID_ARGUMENT;
-    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes || ldx > sbx::kMaxMoeTokenBytes / (int64_t)elem)
+    if (ld1 > sbx::kMaxRowBytes || ld2 > sbx::kMaxRowBytes ||
+        (tokens > 1 && ldx > sbx::kMaxMoeTokenBytes / (int64_t)elem))
         return SBX_UNSUPPORTED;
     sbx::Mx4MoeArgs a;
     a.tokens = (int)tokens; a.width = (int)width; a.hidden = (int)hidden;

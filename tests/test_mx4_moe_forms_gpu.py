@@ -37,3 +37,24 @@ def test_equal_logits_of_far_experts_go_by_index(cuda, name, experts, tokens):
     m.check(x, len(same))
     m.check(x, 2, False)
     m.check(np.zeros((tokens, 96)), 12)
+
+
+@pytest.mark.parametrize("ldx", [1 << 21, 1 << 40, 1 << 62])
+def test_one_token_has_no_next_row(cuda, ldx):
+    """Its leading dimension is not used: any is taken (of several tokens 2^23 bytes are refused)."""
+    import torch
+    import sushiblas_amd as sbx
+    m = Mixture(cuda, "f32", 40, 30, 5)
+    X = torch.randn(1, 40, device=cuda)
+    Y, want = torch.zeros_like(X), torch.zeros_like(X)
+    m.call(X, want, 2, True)
+    size = sbx.mx4_moe_workspace(1, 40, 30, 5, 2)
+    ws = torch.empty(size, dtype=torch.uint8, device=cuda)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    args = (40, 30, 5, 2, p(X), ldx, p(m.WR), m.WR.shape[1], 1, p(m.W1), m.W1.shape[1], p(m.S1), m.S1.shape[1], p(m.W2),
+            m.W2.shape[1], p(m.S2), m.S2.shape[1], p(Y), 40, None, None, p(ws), size)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert sbx.lib().sbx_mx4_moe(stream, sbx.F32, 2, *args) != 0
+    assert sbx.lib().sbx_mx4_moe(stream, sbx.F32, 1, *args) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(Y, want)
