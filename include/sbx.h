@@ -360,6 +360,8 @@ int sbx_mx4_linear(void* stream, int dtype, int64_t m, int64_t n, int64_t k, flo
  * Activations are not rounded before W1's product (but for bits of fp32 values below 2^-133);
  * before W2's they are held as the sum of three bf16 values, 24 bits.  Sums are held in 32 bits and
  * rounded to dtype once.
+ * A token's result has the same bits in calls of the same sizes, wherever it stands and whatever the
+ * others are; in a call of another number of tokens its sums may be in another order.
  * chosen (int32), weights (p): tokens x topk, packed; NULL: not wanted.  Y may be X
  * (same leading dimension).
  * tokens <= 256, topk <= 16, experts <= 512, width and hidden <= 2^18, ld1, ld2 < 2^23 -

@@ -58,3 +58,24 @@ def test_one_token_has_no_next_row(cuda, ldx):
     assert sbx.lib().sbx_mx4_moe(stream, sbx.F32, 1, *args) == 0
     torch.cuda.synchronize()
     assert torch.equal(Y, want)
+
+
+@pytest.mark.parametrize("name", ref.TYPES)
+@pytest.mark.parametrize("tokens,width,hidden,experts,topk", [(6, 300, 520, 9, 3), (40, 1024, 512, 16, 4), (30, 520, 96, 70, 2),
+                                                              (150, 130, 300, 6, 2)])
+def test_a_token_has_the_same_bits_anywhere(cuda, name, tokens, width, hidden, experts, topk):
+    """In another place, among other tokens, of a call of the same sizes."""
+    import torch
+    m = Mixture(cuda, name, width, hidden, experts)
+    X = ref.padded(cuda, _x(tokens, width), m.dt, 0)
+    Y, got = torch.zeros_like(X), torch.zeros_like(X)
+    m.call(X, Y, topk, True)
+    order = torch.randperm(tokens, device=cuda, generator=torch.Generator(cuda).manual_seed(1))
+    m.call(X[order].contiguous(), got, topk, True)
+    assert torch.equal(got, Y[order])
+    m.call(X[order.argsort()[:1]].repeat(tokens, 1), got, topk, True)
+    assert all(torch.equal(got[i], got[0]) for i in range(tokens))
+    others = ref.padded(cuda, _x(tokens, width, 3), m.dt, 0)
+    others[tokens // 2] = X[1]
+    m.call(others, got, topk, True)
+    assert torch.equal(got[tokens // 2], Y[1])
