@@ -95,9 +95,11 @@ inline Mx4MoePlan mx4_moe_plan(int pieces, int tokens, int width, int hidden, in
     p.chunks = (unsigned)((tokens + kMoeChunk - 1) / kMoeChunk);
     p.up_tiles = most(p.up);
     p.down_tiles = most(p.down);
-    // Rows for each wave from so many workgroups on: fp32 4 x 1024 x 2048, 2 of 8 (64 and 256 workgroups a
-    // product) 28.0 us with both forms, 31.8 with rows for each wave, 31.4 with shared ones; bf16 2 x 4096
-    // x 2048, 4 of 32 (256 both) 46 and 52.
+    // Rows for each wave from so many workgroups on.  Of 1, 100, 200, 300 and never, at 11 sizes of each type, 200
+    // is the best or within 5 % of it at 28 of 33 and 14 % off at most; from 1 on, 200 and never, us in a graph:
+    //   bf16 2 x 2048 x 1024, 2 of 8 25.4, 19.4, 19.4;  3 of it, 3 of 16 26.0, 23.0, 23.5;  4 x 1024 x 2048, 2 of 8
+    //   26.1, 21.4, 23.8;  12 x 1024 x 1024, 2 of 16 24.3, 23.7, 26.5;  2 x 4096 x 2048, 4 of 32 37.4, 38.1, 44.7;
+    //   fp16 4 x 4096 x 2048, 2 of 8 39.1, 40.2, 35.4;  fp32 8 x 1500 x 700, 2 of 16 26.8, 28.3, 28.8
     constexpr int64_t ENOUGH = 200;
     const int64_t up_wide = (hidden + 255) / 256 * 4, down_wide = ((width + 31) / 32 + kTileWaves - 1) / kTileWaves;
     p.up_rows = up_wide * p.up_tiles * p.chunks >= ENOUGH;

@@ -98,6 +98,9 @@ struct __attribute__((packed, aligned(sizeof(T)))) Eight {
 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int kRsrcWord3 = 0x00020000;  // of a buffer of bytes
 
 // Sixteen bytes of neighbouring values: what a lane stores at once, so that a wave's instruction
 // writes whole lines (fp32 in two such pieces a lane, 32 bytes apart between lanes: 8192^2

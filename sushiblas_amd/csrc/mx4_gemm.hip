@@ -11,13 +11,11 @@
 #include <type_traits>
 
 #include "mx4.hpp"
-#include "mx4_group.hpp"
 #include "mx4_plan.hpp"
 #include "mx4_strip.hpp"
 
 namespace sbx {
 namespace {
-
 
 // c += b * a^T, with byte H of the codes.  As assembly, so that the sums stay
 // where they are: given the builtin, the compiler moves the 256 sums of a 128 x 128
@@ -36,6 +34,13 @@ __device__ inline void mma(f32x4& c, i32x4 b, int code_b, i32x4 a, int code_a)
                      "cbsz:4 blgp:4"
                      : "+a"(c)
                      : "v"(b), "v"(a), "v"(code_b), "v"(code_a));
+}
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ inline i32x8 widen(i32x4 v)
+{
+    return i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
 }
 
 template <int MB, int NB>
@@ -435,6 +440,63 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mx4_gemm_kernel(Mx4GemmA
 // x 8192 27 us (4.6 TB/s; a copy reaches 5.2).  Blocks of 64 neighbouring bytes an instruction, in
 // place of 32 a lane, took as long.
 constexpr int kSkinnyWaves = 8;
+
+template <int N>
+struct Group {
+    i32x4 v[N][2];
+    int code[N];  // two codes in its low bytes
+};
+
+// The rows of an operand that a workgroup takes, and the lane's place in them (mx4_strip.hpp).
+template <int N>
+struct Strip {
+    const uint8_t *rows, *codes;
+    int64_t lds;
+    int bytes, count, ld, lane, at[N], code_at;
+
+    __device__ inline void init(const uint8_t* P, int64_t ld_, const uint8_t* S, int64_t lds_, int first, int n,
+                                int nb, int lane_)
+    {
+        count = min(n - first, 16 * N);
+        ld = (int)ld_;
+        lds = lds_;
+        lane = lane_;
+        rows = P + first * ld_;
+        bytes = strip_bytes(count, ld, nb);
+        codes = S + 8 * (int64_t)first;
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = strip_lane(lane, i, count, ld);
+        code_at = lane % 16 * 8 + lane / 16 * 2;
+    }
+
+    // Group g (256 terms), with `left` blocks up to the last: zeros, not from memory, past it
+    // and past the last row.  The codes of a group's 8 blocks are all there.
+    __device__ inline void load(Group<N>& d, int g, int left) const
+    {
+        const __amdgpu_buffer_rsrc_t v =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(rows), (short)0, bytes, kRsrcWord3);
+        const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(codes) + g * lds, (short)0, left > 0 ? 8 * count : 0, kRsrcWord3);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int from = strip_scalar(i, g, count, ld, left);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                d.v[i][h] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                          v, strip_vector(at[i], lane, h, left), from, 0));
+            d.code[i] = __builtin_amdgcn_raw_buffer_load_b16(c, code_at + 128 * i, 0, 0);
+        }
+    }
+};
+
+// Codes past the last block may be NaN's and are cleared (the elements there are zeros):
+// `mine` of the lane's two blocks are inside.
+template <int N>
+__device__ inline void clip(Group<N>& d, int mine)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) d.code[i] = mine >= 2 ? d.code[i] : mine == 1 ? d.code[i] & 0xff : 0;
+}
 
 template <typename T, int YB, int XB, bool XA>
 __global__ void __launch_bounds__(64 * kSkinnyWaves, YB * XB >= 4 ? 2 : 4) mx4_skinny_kernel(Mx4GemmArgs p)

@@ -28,7 +28,6 @@
 #include <type_traits>
 
 #include "layer.hpp"
-#include "mx4_group.hpp"
 #include "mx4_strip.hpp"
 #include "pieces.hpp"
 
