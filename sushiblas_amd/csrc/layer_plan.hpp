@@ -85,7 +85,8 @@ inline Mx4MoePlan mx4_moe_plan(int pieces, int tokens, int width, int hidden, in
     const int chunk = tokens < kMoeChunk ? tokens : kMoeChunk, choices = chunk * topk;
     p.few = tokens <= kFewTokens && experts <= kFewExperts;
     // tiles of 16 where experts have more than 6 tokens on average, as most would need two of 8 (64 x 4096
-    // x 2048, 4 of 32, fp16 117 against 126 us, fp32 145 against 150; 8 tokens of it 78 against 73)
+    // x 2048, 4 of 32, fp16 113 against 120 us, fp32 124 against 130; 24 tokens of it 106 against 98 and 118
+    // against 99)
     const bool many = !p.few && choices > 6 * experts;
     p.up = many || pieces == 1 ? 16 : 8;
     p.down = many ? 16 : 8;

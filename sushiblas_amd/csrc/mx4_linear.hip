@@ -46,9 +46,10 @@ constexpr int kTallRows = 128, kTallTokens = 16;
 // Which wave has a term does not depend on m, so a row's bits do not either.
 //   One token is bound by memory: bf16 1 x 28672 x 8192 23.9 us (125 MB, 5.2 TB/s; the product of
 // MXFP4 operands, mx4_gemm.hip, 29.0), 1 x 8192 x 8192 8.2-9.8 (36 MB: 2.3 of it are any kernel's, and there is one
-// round).  More tokens are bound by X's way from the
-// L2s, as each workgroup reads all of it: 16 x 28672 x 8192 38 us, loads alone as long (64 rows of B a
-// workgroup take too many registers: 79).
+// round).  More tokens are bound by the operands' way through LDS to the matrix cores, which their loads do
+// not quite hide behind: without any load bf16 16 x 28672 x 8192 takes 21.5 of its 35 us (with X's alone,
+// which each workgroup reads all of, 23.6, with B's 28.5) and 64 x 8192 x 8192 19.1 of 22.1; conversions
+// take one (64 rows of B a workgroup take too many registers: 79).
 template <typename T, bool MX8, int TOKENS, int YB, int XB, int WAVES, int AHEAD>
 __global__ void __launch_bounds__(64 * WAVES, 2) linear_kernel(Mx4LinearArgs p)
 {

@@ -25,8 +25,8 @@ namespace {
 // ---- the router ----
 
 // Pieces that an activation is held in before the second product: the 24 bits of 32, of every type.  Two
-// (16 bits) take less of the second product (64 x 4096 x 2048, 4 of 32, bf16 106 us against 111, 8 tokens 70.6
-// and 73.0, one token alike), but where an expert's terms cancel what is left has none of a result's own bits.
+// (16 bits) take less of the second product (64 x 4096 x 2048, 4 of 32, bf16 105 us against 112, 8 tokens 70.6
+// and 73.0, one token 15.2 and 15.5), but where an expert's terms cancel what is left has none of a result's own bits.
 constexpr int kActPieces = 3;
 
 // x in the wave's lower half and y in its upper one, each added to its own other half.
